@@ -14,7 +14,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(_HERE, "csrc")
 LIB_PATH = os.path.join(_HERE, "libactnn_hip.so")
 SOURCES = ["minimax.hip", "pack_mixed.hip", "pack_single.hip", "mask_ops.hip", "maxpool.hip",
-           "linear_gw.hip", "misc.hip", "calc_precision.cpp", "calc_precision_dev.hip", "batch_norm.hip"]
+           "linear_gw.hip", "misc.hip", "calc_precision.cpp", "calc_precision_dev.hip", "batch_norm.hip", "tokens.hip"]
 HIPCC_FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared",
     "-ffp-contract=off",                      # bit-exact quantiser: no implicit FMA
@@ -84,6 +84,8 @@ SIGNATURES = {
                                     c_i32, c_i32, c_i32, c_vp, c_i64, c_vp],
     "actnn_linear_grad_weight_q2": [c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_i64,
                                     c_i32, c_i32, c_i32, c_vp],
+    "actnn_tokens_quantize": [c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_i64, c_i32, c_vp],
+    "actnn_tokens_dequantize": [c_vp, c_i64, c_vp, c_vp, c_i64, c_i64, c_i32, c_vp],
     "actnn_stream_copy": [c_vp, c_vp, c_i64, c_vp],
     "actnn_matrix_pipe_probe": [c_vp, c_vp, c_i32, c_i32, c_vp],
     "actnn_batch_norm_workspace_bytes": [c_i64, c_i64, c_i64, c_i32, c_i32],

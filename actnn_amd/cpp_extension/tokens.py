@@ -1,0 +1,33 @@
+"""8-bit tokens: rows of features kept as int8 codes with one fp32 scale a row (no reference counterpart).
+
+A token is the last dimension of a tensor [..., K]: a word's hidden state, a row of a linear layer's input, or the channels of
+one pixel of a channels-last image.  Its codes are 127 x / max|x|, rounded to the nearest whole number (halves away from
+zero), its scale is max|x| / 127.  Unlike the streams of `quantization` they are symmetric about zero and rounded the
+same way each time, so that a product in 8-bit integers can read them as they are; the same codes are the checkpoint that the
+weight gradient reads in the backward pass.
+
+A row without a magnitude of 2^-100 or more (a padded token) has scale 0 and codes 0.  A row that holds a NaN or an
+infinity has scale NaN: everything made from it is NaN.
+
+Codes come in rows that begin at multiples of 16 bytes (their stride is K rounded up to 16), the layout the kernels read;
+codes laid out otherwise are taken too, and copied first.  Everything runs on the current stream of the tensors' device.
+"""
+import torch
+
+from . import _glue as g
+
+
+def _dtype_code(dtype, what):
+    if dtype not in g.DTYPE_CODE:
+        raise RuntimeError(f"{what}: float32, float16 or bfloat16 expected, got {dtype}")
+    return g.DTYPE_CODE[dtype]
+
+
+def quantize_tokens(data):
+    """-> (codes, scale): int8 [..., K] and fp32 [...] of a float32, float16 or bfloat16 tensor [..., K]."""
+    return g.host().quantize_tokens(data)
+
+
+def dequantize_tokens(codes, scale, dtype=torch.float32):
+    """codes * scale, rounded once to `dtype`."""
+    return g.host().dequantize_tokens(codes, scale, _dtype_code(dtype, "dequantize_tokens"))

@@ -590,6 +590,103 @@ PyObject* max_pool2d_backward(PyObject* const* a, Py_ssize_t n) {
   return wrap(out);
 }
 
+// ---------------------------------------------------------------------------- 8-bit tokens
+bool is_float(const Tensor& t) {
+  return t.scalar_type() == at::kFloat || t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16;
+}
+void check_float(const Tensor& t, const char* name) {
+  TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor!");
+  TORCH_CHECK(is_float(t), "The type of ", name, " is not correct!");
+}
+int64_t whole16(int64_t n) { return (n + 15) / 16 * 16; }
+
+// Rows of a tensor [..., K], an element apart from each other in a row and `ld` elements from row to row.
+struct Rows {
+  Tensor held;
+  int64_t M, K, ld;
+  Rows(const Tensor& t, const char* name) {
+    check_float(t, name);
+    TORCH_CHECK(t.dim() >= 1 && t.size(-1) >= 1, name, " must have rows of at least one element");
+    K = t.size(-1);
+    M = t.numel() / K;
+    held = t.dim() == 2 ? t : t.reshape({M, K});
+    if (K > 1 && held.stride(1) != 1) held = held.contiguous();
+    ld = M > 1 ? held.stride(0) : K;
+  }
+};
+// Codes [..., K] as the kernels take them: rows at multiples of 16 bytes, the last one's 16 bytes whole in memory.  What
+// quantize_tokens returns is laid out like that, anything else is copied.
+struct CodeRows {
+  Tensor held;
+  int64_t M, K, ld;
+  CodeRows(const Tensor& t, const char* name) {
+    TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor!");
+    TORCH_CHECK(t.scalar_type() == at::kChar, "The type of ", name, " is not correct!");
+    TORCH_CHECK(t.dim() >= 1 && t.size(-1) >= 1, name, " must have rows of at least one code");
+    K = t.size(-1);
+    M = t.numel() / K;
+    held = t.dim() == 2 ? t : t.reshape({M, K});
+    ld = M > 1 ? held.stride(0) : whole16(K);
+    const bool fits = (K == 1 || held.stride(1) == 1) && ld >= K && ld % 16 == 0 &&
+                      reinterpret_cast<uintptr_t>(held.data_ptr()) % 16 == 0 &&
+                      held.storage_offset() + (M - 1) * ld + whole16(K) <= static_cast<int64_t>(held.storage().nbytes());
+    if (!fits && M > 0) {
+      const Tensor laid = at::empty({M, whole16(K)}, held.options());
+      laid.narrow(1, 0, K).copy_(held);
+      held = laid.narrow(1, 0, K);
+      ld = whole16(K);
+    }
+  }
+  int8_t* data() const { return static_cast<int8_t*>(held.data_ptr()); }
+};
+Tensor row_scales(const Tensor& t, int64_t rows, const Tensor& like, const char* name) {
+  TORCH_CHECK(t.device() == like.device(), name, " must be on the same device");
+  TORCH_CHECK(t.scalar_type() == at::kFloat, "The type of ", name, " is not correct!");
+  TORCH_CHECK(t.numel() == rows, name, " must have one value for each row, ", rows, ", and has ", t.numel());
+  return t.contiguous();
+}
+// new codes and scales for rows of the shape of `like`
+struct NewCodes {
+  Tensor codes, scale;
+  explicit NewCodes(const Tensor& like) {
+    std::vector<int64_t> size(like.sizes().begin(), like.sizes().end());
+    const int64_t K = size.back();
+    size.back() = whole16(K);
+    codes = empty(size, like, at::kChar);
+    size.pop_back();
+    scale = empty(size, like, at::kFloat);
+    if (K % 16) codes = codes.narrow(-1, 0, K);
+  }
+};
+
+// data -> codes, scale
+PyObject* quantize_tokens(PyObject* const* a, Py_ssize_t n) {
+  Args args(a, n, 1);
+  const Tensor data = args.tensor();
+  const Rows rows(data, "data");
+  const c10::DeviceGuard guard(data.device());
+  const NewCodes out(data);
+  launch("quantize_tokens", [&] {
+    return actnn_tokens_quantize(ptr(rows.held), rows.ld, static_cast<int8_t*>(ptr(out.codes)), whole16(rows.K), f32(out.scale),
+                                 rows.M, rows.K, code_of(data.scalar_type()), stream_of(data));
+  });
+  return tuple_of(out.codes, out.scale);
+}
+// codes, scale, dtype -> values
+PyObject* dequantize_tokens(PyObject* const* a, Py_ssize_t n) {
+  Args args(a, n, 3);
+  const Tensor codes = args.tensor(), given = args.tensor();
+  const auto dtype = type_of(args.integer());
+  const CodeRows rows(codes, "codes");
+  const Tensor scale = row_scales(given, rows.M, codes, "scale");
+  const c10::DeviceGuard guard(codes.device());
+  const Tensor out = empty(codes.sizes(), codes, dtype);
+  launch("dequantize_tokens", [&] {
+    return actnn_tokens_dequantize(rows.data(), rows.ld, f32(scale), ptr(out), rows.M, rows.K, code_of(dtype), stream_of(codes));
+  });
+  return wrap(out);
+}
+
 template <PyObject* (*F)(PyObject* const*, Py_ssize_t)>
 PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -601,7 +698,8 @@ PyMethodDef methods[] = {
     ACTNN_CALL(quantize_rows), ACTNN_CALL(quantize_rows_fixed), ACTNN_CALL(unpack_rows_mixed), ACTNN_CALL(unpack_rows_fixed),
     ACTNN_CALL(relu_forward), ACTNN_CALL(relu_backward), ACTNN_CALL(dropout_forward), ACTNN_CALL(dropout_backward),
     ACTNN_CALL(batch_norm_geometry), ACTNN_CALL(batch_norm_forward_quantize), ACTNN_CALL(batch_norm_forward), ACTNN_CALL(batch_norm_backward),
-    ACTNN_CALL(batch_norm_backward_packed), ACTNN_CALL(max_pool2d_forward), ACTNN_CALL(max_pool2d_backward), {nullptr, nullptr, 0, nullptr}};
+    ACTNN_CALL(batch_norm_backward_packed), ACTNN_CALL(max_pool2d_forward), ACTNN_CALL(max_pool2d_backward),
+    ACTNN_CALL(quantize_tokens), ACTNN_CALL(dequantize_tokens), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods};
 
 }  // namespace

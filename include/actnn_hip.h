@@ -506,6 +506,21 @@ int actnn_batch_norm_backward_packed_add_relu(const int32_t* packed, const int32
                                           int64_t N, int64_t C, int64_t HW, int dtype, int channels_last,
                                           void* stream);
 
+/* ---------------------------------------------------------------------------------
+ * 8-bit tokens (no reference counterpart).  A token is a row of K features; codes[M, K] are int8 with one fp32 scale a
+ * row:  top = max_k |x|,  code = sign(x) floor(127 |x| / top + 1/2) exactly (halves away from zero),  scale = top / 127
+ * (for the few tops at the end of fp32 whose codes would come back infinite: the next smaller number).
+ * A row without a magnitude of 2^-100 or more has scale 0 and codes 0, a row that holds a NaN or an infinity has scale
+ * NaN and codes 0.  Rows of codes are ldc bytes apart, ldc a multiple of 16 and at least K, the first 16-byte aligned;
+ * the bytes between K and the next multiple of 16 belong to the row: written as zeros here, read and ignored elsewhere.
+ * ------------------------------------------------------------------------------- */
+/* data: rows of K elements, `ld` elements apart (any ld >= 0), at any element address. */
+int actnn_tokens_quantize(const void* data, int64_t ld, int8_t* codes, int64_t ldc, float* scale, int64_t M, int64_t K,
+                          int dtype, void* stream);
+/* out[M, K] (contiguous, dtype) = codes * scale, rounded once; out at any element address. */
+int actnn_tokens_dequantize(const int8_t* codes, int64_t ldc, const float* scale, void* out, int64_t M, int64_t K,
+                            int dtype, void* stream);
+
 /* Plain device-to-device streaming copy of `bytes` bytes (16-byte aligned pointers and
  * size); used by the benchmark to calibrate bandwidth counters.  No reference counterpart. */
 int actnn_stream_copy(const void* src, void* dst, int64_t bytes, void* stream);

@@ -31,3 +31,18 @@ def quantize_tokens(data):
 def dequantize_tokens(codes, scale, dtype=torch.float32):
     """codes * scale, rounded once to `dtype`."""
     return g.host().dequantize_tokens(codes, scale, _dtype_code(dtype, "dequantize_tokens"))
+
+
+def matmul_tokens(codes, scale, weight_codes, weight_scale, bias=None, dtype=torch.float32):
+    """scale[m] * weight_scale[o] * sum_k codes[m, k] * weight_codes[o, k] + bias[o] -> [..., O] in `dtype`.
+
+    The weight is kept as tokens itself (`quantize_tokens` of a linear layer's [O, K] weight: one scale for each output
+    channel).  The sums are 32-bit integers and exact, for up to 131071 features."""
+    return g.host().matmul_tokens(codes, scale, weight_codes, weight_scale, bias, _dtype_code(dtype, "matmul_tokens"))
+
+
+def linear_tokens(data, weight_codes, weight_scale, bias=None, keep=False):
+    """matmul_tokens(*quantize_tokens(data), ...) in the type of `data`.  With `keep` also the tokens as they were
+    multiplied, which are the checkpoint that linear_tokens_grad_weight reads: (output, codes, scale)."""
+    out, codes, scale = g.host().linear_tokens(data, weight_codes, weight_scale, bias, bool(keep))
+    return (out, codes, scale) if keep else out

@@ -627,7 +627,7 @@ struct CodeRows {
     M = t.numel() / K;
     held = t.dim() == 2 ? t : t.reshape({M, K});
     ld = M > 1 ? held.stride(0) : whole16(K);
-    const bool fits = (K == 1 || held.stride(1) == 1) && ld >= K && ld % 16 == 0 &&
+    const bool fits = ld < (1 << 23) && (K == 1 || held.stride(1) == 1) && ld >= K && ld % 16 == 0 &&
                       reinterpret_cast<uintptr_t>(held.data_ptr()) % 16 == 0 &&
                       held.storage_offset() + (M - 1) * ld + whole16(K) <= static_cast<int64_t>(held.storage().nbytes());
     if (!fits && M > 0) {
@@ -687,6 +687,66 @@ PyObject* dequantize_tokens(PyObject* const* a, Py_ssize_t n) {
   return wrap(out);
 }
 
+// A weight kept as tokens, one scale for each output channel, and the bias: what linear_tokens and matmul_tokens share.
+struct Weight {
+  CodeRows rows;
+  Tensor scale, bias;
+  Weight(const Tensor& codes, const Tensor& scales, const Tensor& given_bias, const Tensor& like, int64_t K)
+      : rows(codes, "weight_codes") {
+    TORCH_CHECK(codes.dim() == 2, "The dimension of weight_codes is not correct!");
+    TORCH_CHECK(codes.device() == like.device(), "weight_codes must be on the same device");
+    TORCH_CHECK(rows.K == K, "weight_codes have ", rows.K, " features, the tokens ", K);
+    TORCH_CHECK(K <= 131071, "the integer sum takes 131071 features at most, got ", K);
+    scale = row_scales(scales, rows.M, codes, "weight_scale");
+    if (given_bias.defined()) {
+      check_float(given_bias, "bias");
+      TORCH_CHECK(given_bias.device() == like.device(), "bias must be on the same device");
+      TORCH_CHECK(given_bias.numel() == rows.M, "bias must have one value for each output, ", rows.M, ", and has ", given_bias.numel());
+      bias = given_bias.detach().to(at::kFloat).contiguous();
+    }
+  }
+};
+Tensor product_of(const CodeRows& x, const Tensor& scale, const Weight& w, at::IntArrayRef lead, at::ScalarType dtype) {
+  std::vector<int64_t> size(lead.begin(), lead.end());
+  size.back() = w.rows.M;
+  const Tensor out = empty(size, x.held, dtype);
+  const int64_t bytes = actnn_tokens_matmul_workspace_bytes(x.M, x.K, w.rows.M);
+  const Tensor workspace = bytes > 0 ? empty({bytes}, x.held, at::kByte) : Tensor();
+  launch("matmul_tokens", [&] {
+    return actnn_tokens_matmul(x.data(), x.ld, f32(scale), w.rows.data(), w.rows.ld, f32(w.scale), f32(w.bias), ptr(out), x.M,
+                               x.K, w.rows.M, code_of(dtype), ptr(workspace), bytes, stream_of(x.held));
+  });
+  return out;
+}
+// codes, scale, weight codes, weight scale, bias | None, dtype -> product
+PyObject* matmul_tokens(PyObject* const* a, Py_ssize_t n) {
+  Args args(a, n, 6);
+  const Tensor codes = args.tensor(), given = args.tensor(), wcodes = args.tensor(), wscale = args.tensor(), bias = args.optional();
+  const auto dtype = type_of(args.integer());
+  const CodeRows x(codes, "codes");
+  const c10::DeviceGuard guard(codes.device());
+  const Tensor scale = row_scales(given, x.M, codes, "scale");
+  const Weight w(wcodes, wscale, bias, codes, x.K);
+  return wrap(product_of(x, scale, w, codes.sizes(), dtype));
+}
+// data, weight codes, weight scale, bias | None, whether the tokens are kept -> product, codes | None, scale | None
+PyObject* linear_tokens(PyObject* const* a, Py_ssize_t n) {
+  Args args(a, n, 5);
+  const Tensor data = args.tensor(), wcodes = args.tensor(), wscale = args.tensor(), bias = args.optional();
+  const bool keep = args.flag();
+  const Rows rows(data, "data");
+  const c10::DeviceGuard guard(data.device());
+  const Weight w(wcodes, wscale, bias, data, rows.K);
+  const NewCodes kept(data);
+  const CodeRows x(kept.codes, "codes");
+  launch("linear_tokens", [&] {
+    return actnn_tokens_quantize(ptr(rows.held), rows.ld, x.data(), x.ld, f32(kept.scale), rows.M, rows.K,
+                                 code_of(data.scalar_type()), stream_of(data));
+  });
+  const Tensor out = product_of(x, kept.scale, w, data.sizes(), data.scalar_type());
+  return keep ? tuple_of(out, kept.codes, kept.scale) : tuple_of(out, Tensor(), Tensor());
+}
+
 template <PyObject* (*F)(PyObject* const*, Py_ssize_t)>
 PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -699,7 +759,7 @@ PyMethodDef methods[] = {
     ACTNN_CALL(relu_forward), ACTNN_CALL(relu_backward), ACTNN_CALL(dropout_forward), ACTNN_CALL(dropout_backward),
     ACTNN_CALL(batch_norm_geometry), ACTNN_CALL(batch_norm_forward_quantize), ACTNN_CALL(batch_norm_forward), ACTNN_CALL(batch_norm_backward),
     ACTNN_CALL(batch_norm_backward_packed), ACTNN_CALL(max_pool2d_forward), ACTNN_CALL(max_pool2d_backward),
-    ACTNN_CALL(quantize_tokens), ACTNN_CALL(dequantize_tokens), {nullptr, nullptr, 0, nullptr}};
+    ACTNN_CALL(quantize_tokens), ACTNN_CALL(dequantize_tokens), ACTNN_CALL(matmul_tokens), ACTNN_CALL(linear_tokens), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods};
 
 }  // namespace

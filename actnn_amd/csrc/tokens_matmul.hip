@@ -1,0 +1,393 @@
+// Matrix product in 8-bit integers with a scale for each token and each output channel:
+//
+//     y[m, o] = scale[m] * weight_scale[o] * sum_k codes[m, k] * weight_codes[o, k]  (+ bias[o])
+//
+// The sum is a 32-bit integer and exact (K <= 131071: K * 2^14 < 2^31); it is converted to fp32, multiplied by the two scales,
+// the bias is added, and the result is rounded to the output's type.  Sums that are split over blocks or waves are
+// added as integers: the order does not matter.
+//
+// Three kernels share the work by the number of tokens:
+//   * few tokens: bound by reading the weight once.  No tiles: a wave's lanes load their 16 bytes of 16 channels' rows
+//     straight into the operand registers of v_mfma_i32_16x16x64_i8, the waves of a block share the features of the same
+//     channels and add their sums in LDS.
+//   * tiles of 64, 128 or 256 channels by as many tokens, for everything else: v_mfma_i32_32x32x32_i8 out of LDS.  Two buffers of
+//     128 features; both operands go from global memory straight into LDS (global_load_lds, 16 bytes a lane), rows as they lie in
+//     memory, their eight 16-byte chunks at chunk ^ (row / 2) % 8: 16 rows of two banks' widths meet every bank once.
+//   * tiles that do not fill the chip take slices of the features; a second kernel adds the slices.
+// Rows and channels past the end are read from the last one and not stored; features past the end are read from the
+// step's first chunk and masked out of the weight's operand.
+#include <type_traits>
+
+#include "token_math.h"
+
+namespace actnn {
+namespace {
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x16 __attribute__((ext_vector_type(16)));
+
+constexpr int kThreads = 256;
+constexpr int64_t kMostFeatures = 131071;               // the integer sum of so many products fits 32 bits
+constexpr int64_t kMostStride = 0x7fffff;               // 256 rows of so many bytes stay below 2 GiB
+
+template <int N> struct Const { static constexpr int value = N; };
+template <int N, typename F> ACTNN_DEV void for_each(F&& f) {
+  if constexpr (N > 0) {
+    for_each<N - 1>(f);
+    f(Const<N - 1>{});
+  }
+}
+
+typedef __attribute__((address_space(3))) uint8_t* lds_ptr_t;
+ACTNN_DEV uint32_t lds_address(const void* p) {
+  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint8_t*)p;
+}
+ACTNN_DEV u32x4 lds_load16(uint32_t address) {
+  return *reinterpret_cast<const __attribute__((address_space(3))) u32x4*>((lds_ptr_t)(uintptr_t)address);
+}
+
+// the first `valid` of 16 bytes, the others 0
+ACTNN_DEV u32x4 first_bytes(u32x4 v, int valid) {
+  uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int n = valid - 4 * i;
+    w[i] = n >= 4 ? w[i] : n <= 0 ? 0u : w[i] & ((1u << (8 * n)) - 1u);
+  }
+  return (u32x4){w[0], w[1], w[2], w[3]};
+}
+
+struct Product {
+  const int8_t* x;                       // token codes [M, K], rows `ldx` bytes apart
+  const float* xs;
+  const int8_t* w;                       // weight codes [O, K]
+  const float* ws;
+  const float* bias;                     // [O] or null
+  void* y;                               // [M, O]; slices: int32 [slices][M, O]
+  int64_t ldx, ldw;
+  int M, K, O;
+};
+
+// four consecutive channels of a token, from their integer sums
+template <typename TY> ACTNN_DEV void put4(const Product& p, int64_t token, int channel, const int (&sum)[4]) {
+  if (token >= p.M) return;
+  TY* to = static_cast<TY*>(p.y) + token * p.O + channel;
+  float v[4];
+  const float xs = p.xs[token];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int c = channel + i < p.O ? channel + i : p.O - 1;
+    v[i] = (float)sum[i] * xs * p.ws[c];
+    if (p.bias) v[i] += p.bias[c];
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (channel + i < p.O) Conv<TY>::store(to, i, v[i]);
+}
+template <> ACTNN_DEV void put4<int>(const Product& p, int64_t token, int channel, const int (&sum)[4]) {
+  if (token >= p.M) return;
+  int* to = static_cast<int*>(p.y) + token * p.O + channel;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (channel + i < p.O) to[i] = sum[i];
+}
+
+// ------------------------------------------------------------------------------------------
+// Tiles.  Four waves, two by two; a wave has NA x NE fragments of 32 channels x 32 tokens.
+// ------------------------------------------------------------------------------------------
+template <typename TY, int NA, int NE>
+__global__ __launch_bounds__(kThreads, 1) void tokens_tile_kernel(Product p, int slices, int steps_per_slice) {
+  constexpr int BO = 64 * NA, BT = 64 * NE, BK = 128;
+  constexpr int kBuffer = (BO + BT) * BK;
+  constexpr int kGroup = NA * NE, kSlots = 4 * kGroup, kFragments = NA + NE;
+  constexpr int kReads = (kFragments + kGroup - 1) / kGroup;          // fragment reads beside an MFMA
+  constexpr int kPieces = kBuffer / (kThreads * 16);                  // direct loads of a wave and step
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[2 * kBuffer];
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wr = wave & 1, wn = wave >> 1;
+  const int tiles_o = (p.O + BO - 1) / BO, tiles_t = (p.M + BT - 1) / BT;
+  const int slice = slices > 1 ? blockIdx.x / (tiles_o * tiles_t) : 0;
+  int tile = slices > 1 ? blockIdx.x % (tiles_o * tiles_t) : blockIdx.x;
+  if (slices == 1 && tiles_t % 8 == 0) {
+    // blocks are dealt round-robin to the 8 XCDs: each gets whole panels of tokens, which stay in its L2
+    const int xcd = blockIdx.x & 7, i = blockIdx.x >> 3;
+    tile = (xcd * (tiles_t / 8) + i / tiles_o) * tiles_o + i % tiles_o;
+  }
+  const int t0 = tile / tiles_o * BT, o0 = tile % tiles_o * BO;
+  const int all_steps = (p.K + BK - 1) / BK;
+  const int first = slice * steps_per_slice;
+  int steps = all_steps - first;
+  if (slices > 1 && steps > steps_per_slice) steps = steps_per_slice;
+  if (slices > 1) p.y = static_cast<int*>(p.y) + (int64_t)slice * p.M * p.O;
+  const int chunks = (p.K + 15) / 16;
+
+  // ---- direct loads: piece j is 8 rows of the weight's tile or, behind those, of the tokens'
+  const int row_in = lane >> 3;
+  const int chunk = (lane & 7) ^ (((wave & 1) << 2) | (row_in >> 1));
+  uint32_t off[kPieces];
+#pragma unroll
+  for (int i = 0; i < kPieces; ++i) {
+    const int row = 8 * (wave + 4 * i) + row_in;
+    if (i < BO / 32) {
+      const int at = o0 + row < p.O ? row : p.O - 1 - o0;
+      off[i] = (uint32_t)at * (uint32_t)p.ldw + (uint32_t)chunk * 16u;
+    } else {
+      const int at = t0 + row - BO < p.M ? row - BO : p.M - 1 - t0;
+      off[i] = (uint32_t)at * (uint32_t)p.ldx + (uint32_t)chunk * 16u;
+    }
+  }
+  const int8_t* wp = p.w + (int64_t)o0 * p.ldw;
+  const int8_t* xp = p.x + (int64_t)t0 * p.ldx;
+  auto load_piece = [&](int buffer, int step, auto I) {
+    constexpr int i = decltype(I)::value;
+    uint32_t at = off[i];
+    if (step * 8 + chunk >= chunks) at -= (uint32_t)chunk * 16u;       // past the row's end: the step's first chunk
+    const int8_t* base = (i < BO / 32 ? wp : xp) + (int64_t)step * BK;
+    load_to_lds16_base(base, at, smem + buffer * kBuffer + (wave + 4 * i) * 1024);
+  };
+
+  // ---- fragments: lane -> row lane % 32, features 32 kb + 16 (lane / 32) ..
+  const uint32_t lds0 = lds_address(smem);
+  const uint32_t in_row = (uint32_t)(lane & 31) * BK + (uint32_t)((((lane >> 5) ^ (lane >> 1)) & 7) << 4);
+  const uint32_t at_w = lds0 + (uint32_t)(wr * 32 * NA) * BK + in_row;
+  const uint32_t at_x = lds0 + (uint32_t)(BO + wn * 32 * NE) * BK + in_row;
+
+  i32x16 acc[NE][NA];
+#pragma unroll
+  for (int e = 0; e < NE; ++e)
+#pragma unroll
+    for (int a = 0; a < NA; ++a)
+#pragma unroll
+      for (int c = 0; c < 16; ++c) acc[e][a][c] = 0;
+  u32x4 fw[2][NA], fx[2][NE];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+#pragma unroll
+    for (int a = 0; a < NA; ++a) fw[h][a] = (u32x4){0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int e = 0; e < NE; ++e) fx[h][e] = (u32x4){0u, 0u, 0u, 0u};
+  }
+  // valid: bytes of the weight's fragment that exist (16 but in the last step)
+  auto read_fragment = [&](auto BUF, auto KB, auto F, auto TAIL, int step) {
+    constexpr int kb = decltype(KB)::value, f = decltype(F)::value;
+    constexpr uint32_t buf = decltype(BUF)::value * kBuffer;
+    if constexpr (f < NA) {
+      u32x4 v = lds_load16((at_w ^ (kb << 5)) + buf + f * 32 * BK);
+      if constexpr (decltype(TAIL)::value != 0) v = first_bytes(v, p.K - (step * BK + kb * 32 + (lane >> 5) * 16));
+      fw[kb & 1][f] = v;
+    } else {
+      fx[kb & 1][f - NA] = lds_load16((at_x ^ (kb << 5)) + buf + (f - NA) * 32 * BK);
+    }
+  };
+  auto mma = [&](auto KB, int e, int a) {
+    constexpr int h = decltype(KB)::value & 1;
+    acc[e][a] = __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(i32x4, fw[h][a]), __builtin_bit_cast(i32x4, fx[h][e]),
+                                                      acc[e][a], 0, 0, 0);
+  };
+
+  // Between two barriers: the MFMAs of the last k-block of the step before (its fragments are in registers) and of the
+  // first three of this step, the fragments of each k-block read beside the MFMAs of the one before, and the direct loads of
+  // the next step into the other buffer.
+  auto step = [&](auto BUF, auto TAIL, int t) {
+    constexpr int buf = decltype(BUF)::value;
+    for_each<kSlots>([&](auto S) {
+      constexpr int slot = decltype(S)::value, in = slot % kGroup;
+      mma(Const<(slot / kGroup + 3) % 4>{}, in / NA, in % NA);
+      for_each<kReads>([&](auto R) {
+        constexpr int f = in * kReads + decltype(R)::value;
+        if constexpr (f < kFragments) read_fragment(Const<buf>{}, Const<slot / kGroup>{}, Const<f>{}, TAIL, first + t);
+      });
+      if constexpr (slot < kPieces) {
+        if (t + 1 < steps) load_piece(1 - buf, first + t + 1, Const<slot>{});
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    });
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+  };
+  static_assert(kPieces <= kSlots, "a direct load beside each of the first MFMAs");
+  for_each<kPieces>([&](auto I) { load_piece(0, first, I); });
+  __builtin_amdgcn_s_waitcnt(0);
+  __syncthreads();
+  const int whole = p.K % BK == 0 || first + steps < all_steps ? steps : steps - 1;   // steps without a tail
+  int t = 0;
+  for (; t + 2 <= whole; t += 2) {
+    step(Const<0>{}, Const<0>{}, t);
+    step(Const<1>{}, Const<0>{}, t + 1);
+  }
+  if (t < whole) {
+    step(Const<0>{}, Const<0>{}, t);
+    ++t;
+    if (t < steps) step(Const<1>{}, Const<1>{}, t);
+  } else if (t < steps) {
+    step(Const<0>{}, Const<1>{}, t);
+  }
+  for_each<kGroup>([&](auto G) { mma(Const<3>{}, decltype(G)::value / NA, decltype(G)::value % NA); });
+
+  // accumulator register c of a lane: channel 8 (c / 4) + 4 (lane / 32) + c % 4 of the fragment, token lane % 32
+#pragma unroll
+  for (int e = 0; e < NE; ++e) {
+    const int64_t token = t0 + wn * 32 * NE + 32 * e + (lane & 31);
+#pragma unroll
+    for (int a = 0; a < NA; ++a) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int channel = o0 + wr * 32 * NA + 32 * a + 8 * q + 4 * (lane >> 5);
+        const int sum[4] = {acc[e][a][4 * q], acc[e][a][4 * q + 1], acc[e][a][4 * q + 2], acc[e][a][4 * q + 3]};
+        if (channel < p.O) put4<TY>(p, token, channel, sum);
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------
+// Few tokens: 16 channels a block, MT tiles of 16 tokens, the waves share the features in pieces of 64.
+// ------------------------------------------------------------------------------------------
+template <typename TY, int MT, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void tokens_few_kernel(Product p) {
+  constexpr int kAhead = 4;
+  __shared__ i32x4 s_sum[WAVES][MT][64];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int o0 = blockIdx.x * 16;
+  const int row = lane & 15, part = lane >> 4;
+  const int8_t* wp = p.w + (int64_t)(o0 + row < p.O ? o0 + row : p.O - 1) * p.ldw;
+  const int8_t* xp[MT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) xp[i] = p.x + (int64_t)(16 * i + row < p.M ? 16 * i + row : p.M - 1) * p.ldx;
+  i32x4 acc[MT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) acc[i] = (i32x4){0, 0, 0, 0};
+  const int pieces = (p.K + 63) / 64;
+  for (int c0 = wave; c0 < pieces; c0 += kAhead * WAVES) {
+    u32x4 fw[kAhead], fx[kAhead][MT];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      int k = (c0 + j * WAVES) * 64 + part * 16;
+      k = k < p.K ? k : 0;                                             // (masked below)
+      fw[j] = load16(wp + k);
+#pragma unroll
+      for (int i = 0; i < MT; ++i) fx[j][i] = load16(xp[i] + k);
+    }
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const int k = (c0 + j * WAVES) * 64 + part * 16;
+      if (k + 16 > p.K) fw[j] = first_bytes(fw[j], p.K - k);
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+        acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, fw[j]), __builtin_bit_cast(i32x4, fx[j][i]),
+                                                       acc[i], 0, 0, 0);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < MT; ++i) s_sum[wave][i][lane] = acc[i];
+  __syncthreads();
+  // accumulator register c of a lane: channel 4 (lane / 16) + c, token lane % 16
+  for (int i = threadIdx.x; i < MT * 64; i += 64 * WAVES) {
+    i32x4 v = s_sum[0][i >> 6][i & 63];
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) v += s_sum[w][i >> 6][i & 63];
+    const int sum[4] = {v.x, v.y, v.z, v.w};
+    const int channel = o0 + 4 * ((i & 63) >> 4);
+    if (channel < p.O) put4<TY>(p, 16 * (i >> 6) + (i & 15), channel, sum);
+  }
+}
+
+// the sum of the slices
+template <typename TY>
+__global__ __launch_bounds__(kThreads) void tokens_sum_slices_kernel(Product p, const int* __restrict__ part, int slices) {
+  const int64_t n = (int64_t)p.M * p.O;
+  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < n; i += (int64_t)gridDim.x * kThreads) {
+    int sum = 0;
+    for (int s = 0; s < slices; ++s) sum += part[s * n + i];
+    const int64_t token = i / p.O;
+    const int channel = (int)(i - token * p.O);
+    float v = (float)sum * p.xs[token] * p.ws[channel];
+    if (p.bias) v += p.bias[channel];
+    Conv<TY>::store(static_cast<TY*>(p.y), i, v);
+  }
+}
+
+// Which kernel: tile edge (0: few tokens) and slices of the features.
+struct Plan { int edge, slices, steps_per_slice; };
+Plan plan_of(int64_t M, int64_t K, int64_t O) {
+  if (M <= 64) return Plan{0, 1, 0};
+  constexpr int64_t kCUs = 256;
+  const int64_t steps = (K + 127) / 128;
+  auto tiles = [&](int64_t edge) { return ((M + edge - 1) / edge) * ((O + edge - 1) / edge); };
+  const int edge = tiles(256) >= kCUs ? 256 : tiles(128) >= kCUs ? 128 : 64;
+  int64_t slices = 1;
+  if (tiles(edge) < kCUs) {
+    slices = kCUs / tiles(edge);
+    if (slices > steps / 4) slices = steps / 4;                        // four steps at least
+    if (slices < 1) slices = 1;
+  }
+  const int64_t per = (steps + slices - 1) / slices;
+  return Plan{edge, (int)((steps + per - 1) / per), (int)per};
+}
+
+template <typename TY, int N> void launch_tiles(const Product& p, const Plan& plan, int64_t blocks, hipStream_t s) {
+  tokens_tile_kernel<TY, N, N><<<dim3((unsigned)blocks), dim3(kThreads), 0, s>>>(p, plan.slices, plan.steps_per_slice);
+}
+template <typename TY> void launch_edge(const Product& p, const Plan& plan, int64_t blocks, hipStream_t s) {
+  if (plan.edge == 256) launch_tiles<TY, 4>(p, plan, blocks, s);
+  else if (plan.edge == 128) launch_tiles<TY, 2>(p, plan, blocks, s);
+  else launch_tiles<TY, 1>(p, plan, blocks, s);
+}
+
+template <typename TY> int product(const Product& p, void* workspace, int64_t workspace_bytes, hipStream_t s) {
+  Plan plan = plan_of(p.M, p.K, p.O);
+  if (plan.edge == 0) {
+    const dim3 grid((unsigned)((p.O + 15) / 16)), blk(512);
+    if (p.M <= 16) tokens_few_kernel<TY, 1, 8><<<grid, blk, 0, s>>>(p);
+    else if (p.M <= 32) tokens_few_kernel<TY, 2, 8><<<grid, blk, 0, s>>>(p);
+    else tokens_few_kernel<TY, 4, 8><<<grid, blk, 0, s>>>(p);
+    ACTNN_RETURN_LAUNCH_STATUS();
+  }
+  const int64_t n = (int64_t)p.M * p.O;
+  if (plan.slices > 1 && (!workspace || workspace_bytes < 4 * n * plan.slices)) plan = Plan{plan.edge, 1, 0};
+  const int64_t blocks = (p.M + plan.edge - 1) / plan.edge * ((p.O + plan.edge - 1) / plan.edge) * plan.slices;
+  if (blocks > 0x7fffffffLL) return ACTNN_EINVAL;
+  if (plan.slices == 1) {
+    launch_edge<TY>(p, plan, blocks, s);
+  } else {
+    if (!aligned16(workspace)) return ACTNN_EALIGN;
+    Product parts = p;
+    parts.y = workspace;
+    launch_edge<int>(parts, plan, blocks, s);
+    const int64_t sums = (n + kThreads - 1) / kThreads;
+    tokens_sum_slices_kernel<TY><<<dim3((unsigned)(sums < 4096 ? sums : 4096)), dim3(kThreads), 0, s>>>(
+        p, static_cast<const int*>(workspace), plan.slices);
+  }
+  ACTNN_RETURN_LAUNCH_STATUS();
+}
+
+}  // namespace
+}  // namespace actnn
+
+extern "C" int64_t actnn_tokens_matmul_workspace_bytes(int64_t M, int64_t K, int64_t O) {
+  using namespace actnn;
+  if (M < 1 || K < 1 || O < 1 || M > 0x7fffff00LL || O > 0x7fffff00LL || K > kMostFeatures) return 0;
+  const Plan plan = plan_of(M, K, O);
+  return plan.slices > 1 ? 4 * M * O * plan.slices : 0;
+}
+
+extern "C" int actnn_tokens_matmul(const int8_t* codes, int64_t ldc, const float* scale, const int8_t* weight_codes,
+                                   int64_t ldw, const float* weight_scale, const float* bias, void* out, int64_t M,
+                                   int64_t K, int64_t O, int dtype, void* workspace, int64_t workspace_bytes, void* stream) {
+  using namespace actnn;
+  if (M < 0 || O < 0 || K < 1 || K > kMostFeatures || M > 0x7fffff00LL || O > 0x7fffff00LL) return ACTNN_EINVAL;
+  if (ldc < K || ldc % 16 || ldc > kMostStride || ldw < K || ldw % 16 || ldw > kMostStride) return ACTNN_EINVAL;
+  if (dtype != ACTNN_F32 && dtype != ACTNN_F16 && dtype != ACTNN_BF16) return ACTNN_EDTYPE;
+  if (M == 0 || O == 0) return ACTNN_OK;
+  if (!codes || !scale || !weight_codes || !weight_scale || !out) return ACTNN_EINVAL;
+  if (!aligned16(codes) || !aligned16(weight_codes) || reinterpret_cast<uintptr_t>(out) % (dtype == ACTNN_F32 ? 4 : 2) != 0)
+    return ACTNN_EALIGN;
+  const Product p{codes, scale, weight_codes, weight_scale, bias, out, ldc, ldw, (int)M, (int)K, (int)O};
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (dtype == ACTNN_F32) return product<float>(p, workspace, workspace_bytes, s);
+  if (dtype == ACTNN_F16) return product<__half>(p, workspace, workspace_bytes, s);
+  return product<bf16_t>(p, workspace, workspace_bytes, s);
+}

@@ -520,6 +520,14 @@ int actnn_tokens_quantize(const void* data, int64_t ld, int8_t* codes, int64_t l
 /* out[M, K] (contiguous, dtype) = codes * scale, rounded once; out at any element address. */
 int actnn_tokens_dequantize(const int8_t* codes, int64_t ldc, const float* scale, void* out, int64_t M, int64_t K,
                             int dtype, void* stream);
+/* out[M, O] (contiguous, dtype, at any element address) = scale[m] * weight_scale[o] * sum_k codes[m, k] * weight_codes[o, k]
+ * + bias[o] (fp32 or null): tokens times a weight kept as tokens itself, one scale for each of its O rows.  The sum is exact
+ * (K <= 131071); strides up to 2^23 - 1 bytes.  Shapes that fill the chip only when their sums are split want a
+ * workspace of _workspace_bytes (0: none; without one the call is slower, its results the same). */
+int64_t actnn_tokens_matmul_workspace_bytes(int64_t M, int64_t K, int64_t O);
+int actnn_tokens_matmul(const int8_t* codes, int64_t ldc, const float* scale, const int8_t* weight_codes, int64_t ldw,
+                        const float* weight_scale, const float* bias, void* out, int64_t M, int64_t K, int64_t O,
+                        int dtype, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* Plain device-to-device streaming copy of `bytes` bytes (16-byte aligned pointers and
  * size); used by the benchmark to calibrate bandwidth counters.  No reference counterpart. */

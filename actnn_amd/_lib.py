@@ -15,7 +15,7 @@ CSRC = os.path.join(_HERE, "csrc")
 LIB_PATH = os.path.join(_HERE, "libactnn_hip.so")
 SOURCES = ["minimax.hip", "pack_mixed.hip", "pack_single.hip", "mask_ops.hip", "maxpool.hip",
            "linear_gw.hip", "misc.hip", "calc_precision.cpp", "calc_precision_dev.hip", "batch_norm.hip", "tokens.hip",
-           "tokens_matmul.hip"]
+           "tokens_matmul.hip", "tokens_grad.hip"]
 HIPCC_FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared",
     "-ffp-contract=off",                      # bit-exact quantiser: no implicit FMA
@@ -89,6 +89,8 @@ SIGNATURES = {
     "actnn_tokens_dequantize": [c_vp, c_i64, c_vp, c_vp, c_i64, c_i64, c_i32, c_vp],
     "actnn_tokens_matmul_workspace_bytes": [c_i64, c_i64, c_i64],
     "actnn_tokens_matmul": [c_vp, c_i64, c_vp, c_vp, c_i64, c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_i32, c_vp, c_i64, c_vp],
+    "actnn_tokens_grad_weight_workspace_bytes": [c_i64, c_i64, c_i64],
+    "actnn_tokens_grad_weight": [c_vp, c_i64, c_vp, c_i64, c_vp, c_vp, c_i64, c_i64, c_i64, c_i32, c_i32, c_vp, c_i64, c_vp],
     "actnn_stream_copy": [c_vp, c_vp, c_i64, c_vp],
     "actnn_matrix_pipe_probe": [c_vp, c_vp, c_i32, c_i32, c_vp],
     "actnn_batch_norm_workspace_bytes": [c_i64, c_i64, c_i64, c_i32, c_i32],
@@ -129,6 +131,7 @@ SIGNATURES = {
 _RESTYPES = {"actnn_strerror": ctypes.c_char_p, "actnn_version": ctypes.c_char_p,
              "actnn_linear_grad_weight_workspace_bytes": ctypes.c_int64,
              "actnn_tokens_matmul_workspace_bytes": ctypes.c_int64,
+             "actnn_tokens_grad_weight_workspace_bytes": ctypes.c_int64,
              "actnn_batch_norm_workspace_bytes": ctypes.c_int64,
              "actnn_batch_norm_forward_static_limit": ctypes.c_int64,
              "actnn_batch_norm_backward_sumsq_entries": ctypes.c_int64}

@@ -46,3 +46,11 @@ def linear_tokens(data, weight_codes, weight_scale, bias=None, keep=False):
     multiplied, which are the checkpoint that linear_tokens_grad_weight reads: (output, codes, scale)."""
     out, codes, scale = g.host().linear_tokens(data, weight_codes, weight_scale, bias, bool(keep))
     return (out, codes, scale) if keep else out
+
+
+def linear_tokens_grad_weight(grad_output, codes, scale, dtype=None):
+    """grad_output[..., O]^T @ (codes * scale)[..., K] -> [O, K], summed over all tokens in fp32: the weight gradient of
+    a linear layer from the tokens it kept.  grad_output is float16 or bfloat16 (the values of the codes are rounded to its type
+    on their way into the product); the result comes in its type, or with `dtype` in float32."""
+    return g.host().linear_tokens_grad_weight(grad_output, codes, scale,
+                                              None if dtype is None else _dtype_code(dtype, "linear_tokens_grad_weight"))

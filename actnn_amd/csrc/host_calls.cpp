@@ -746,6 +746,42 @@ PyObject* linear_tokens(PyObject* const* a, Py_ssize_t n) {
   const Tensor out = product_of(x, kept.scale, w, data.sizes(), data.scalar_type());
   return keep ? tuple_of(out, kept.codes, kept.scale) : tuple_of(out, Tensor(), Tensor());
 }
+// grad_output, codes, scale, dtype -> gradient of the weight
+PyObject* linear_tokens_grad_weight(PyObject* const* a, Py_ssize_t n) {
+  Args args(a, n, 4);
+  const Tensor grad = args.tensor(), codes = args.tensor(), given = args.tensor();
+  TORCH_CHECK(grad.is_cuda(), "grad_output must be a CUDA tensor!");
+  const auto type = grad.scalar_type();
+  TORCH_CHECK(type == at::kHalf || type == at::kBFloat16, "The type of grad_output is not correct!");
+  const auto dtype = args.at[args.i] == Py_None ? type : type_of(args.integer());
+  TORCH_CHECK(dtype == type || dtype == at::kFloat, "the weight's gradient comes in the type of grad_output or in float32");
+  const CodeRows x(codes, "codes");
+  TORCH_CHECK(codes.device() == grad.device(), "codes must be on the same device");
+  TORCH_CHECK(grad.dim() == codes.dim() && grad.dim() >= 1 && grad.sizes().slice(0, grad.dim() - 1) == codes.sizes().slice(0, codes.dim() - 1),
+              "grad_output ", grad.sizes(), " and codes ", codes.sizes(), " are not of the same tokens");
+  const c10::DeviceGuard guard(grad.device());
+  const Tensor scale = row_scales(given, x.M, codes, "scale");
+  const int64_t O = grad.size(-1);
+  const Tensor out = empty({O, x.K}, grad, dtype);
+  if (O == 0) return wrap(out);
+  if (x.M == 0) return wrap(out.zero_());
+  Tensor rows = grad.detach().reshape({x.M, O});
+  if (O > 1 && rows.stride(1) != 1) rows = rows.contiguous();
+  int64_t ld = x.M > 1 ? rows.stride(0) : O;
+  if ((x.M - 1) * ld + O < 8) {                          // the kernel reads 16 bytes at least
+    const Tensor room = at::zeros({x.M, 8}, rows.options());
+    room.narrow(1, 0, O).copy_(rows);
+    rows = room;
+    ld = 8;
+  }
+  const int64_t bytes = actnn_tokens_grad_weight_workspace_bytes(x.M, O, x.K);
+  const Tensor workspace = bytes > 0 ? empty({bytes}, grad, at::kByte) : Tensor();
+  launch("linear_tokens_grad_weight", [&] {
+    return actnn_tokens_grad_weight(ptr(rows), ld, x.data(), x.ld, f32(scale), ptr(out), x.M, O, x.K, code_of(type),
+                                    code_of(dtype), ptr(workspace), bytes, stream_of(grad));
+  });
+  return wrap(out);
+}
 
 template <PyObject* (*F)(PyObject* const*, Py_ssize_t)>
 PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t n) {
@@ -759,7 +795,8 @@ PyMethodDef methods[] = {
     ACTNN_CALL(relu_forward), ACTNN_CALL(relu_backward), ACTNN_CALL(dropout_forward), ACTNN_CALL(dropout_backward),
     ACTNN_CALL(batch_norm_geometry), ACTNN_CALL(batch_norm_forward_quantize), ACTNN_CALL(batch_norm_forward), ACTNN_CALL(batch_norm_backward),
     ACTNN_CALL(batch_norm_backward_packed), ACTNN_CALL(max_pool2d_forward), ACTNN_CALL(max_pool2d_backward),
-    ACTNN_CALL(quantize_tokens), ACTNN_CALL(dequantize_tokens), ACTNN_CALL(matmul_tokens), ACTNN_CALL(linear_tokens), {nullptr, nullptr, 0, nullptr}};
+    ACTNN_CALL(quantize_tokens), ACTNN_CALL(dequantize_tokens), ACTNN_CALL(matmul_tokens), ACTNN_CALL(linear_tokens),
+    ACTNN_CALL(linear_tokens_grad_weight), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods};
 
 }  // namespace

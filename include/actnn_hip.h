@@ -528,6 +528,14 @@ int64_t actnn_tokens_matmul_workspace_bytes(int64_t M, int64_t K, int64_t O);
 int actnn_tokens_matmul(const int8_t* codes, int64_t ldc, const float* scale, const int8_t* weight_codes, int64_t ldw,
                         const float* weight_scale, const float* bias, void* out, int64_t M, int64_t K, int64_t O,
                         int dtype, void* workspace, int64_t workspace_bytes, void* stream);
+/* grad_w[O, I] (contiguous, out_dtype: that of grad_out or fp32) = grad_out[M, O]^T @ (codes * scale)[M, I], the values of the
+ * codes rounded to grad_out's type (fp16 or bf16), the sum in fp32.  Rows of grad_out are ldg elements apart, at any
+ * element address; a grad_out of fewer than 8 elements wants ldg >= 8 and that much memory for each row.  M >= 1.
+ * Workspace as above. */
+int64_t actnn_tokens_grad_weight_workspace_bytes(int64_t M, int64_t O, int64_t I);
+int actnn_tokens_grad_weight(const void* grad_out, int64_t ldg, const int8_t* codes, int64_t ldc, const float* scale,
+                             void* grad_w, int64_t M, int64_t O, int64_t I, int go_dtype, int out_dtype, void* workspace,
+                             int64_t workspace_bytes, void* stream);
 
 /* Plain device-to-device streaming copy of `bytes` bytes (16-byte aligned pointers and
  * size); used by the benchmark to calibrate bandwidth counters.  No reference counterpart. */

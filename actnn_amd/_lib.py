@@ -15,7 +15,7 @@ CSRC = os.path.join(_HERE, "csrc")
 LIB_PATH = os.path.join(_HERE, "libactnn_hip.so")
 SOURCES = ["minimax.hip", "pack_mixed.hip", "pack_single.hip", "mask_ops.hip", "maxpool.hip",
            "linear_gw.hip", "misc.hip", "calc_precision.cpp", "calc_precision_dev.hip", "batch_norm.hip", "tokens.hip",
-           "tokens_matmul.hip", "tokens_grad.hip"]
+           "tokens_matmul.hip", "tokens_grad.hip", "group_norm.hip"]
 HIPCC_FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared",
     "-ffp-contract=off",                      # bit-exact quantiser: no implicit FMA
@@ -91,6 +91,11 @@ SIGNATURES = {
     "actnn_tokens_matmul": [c_vp, c_i64, c_vp, c_vp, c_i64, c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_i32, c_vp, c_i64, c_vp],
     "actnn_tokens_grad_weight_workspace_bytes": [c_i64, c_i64, c_i64],
     "actnn_tokens_grad_weight": [c_vp, c_i64, c_vp, c_i64, c_vp, c_vp, c_i64, c_i64, c_i64, c_i32, c_i32, c_vp, c_i64, c_vp],
+    "actnn_group_norm_workspace_bytes": [c_i64, c_i64, c_i64, c_i64, c_i32, c_i32],
+    # x weight bias y mean rstd codes scale | N C pixels groups | eps activation dtype | ws ws_bytes stream
+    "actnn_group_norm_forward": [c_vp] * 8 + [c_i64] * 4 + [ctypes.c_double, c_i32, c_i32, c_vp, c_i64, c_vp],
+    # dy codes scale x weight bias mean rstd dx dweight dbias | N C pixels groups | activation dtype | ws ws_bytes stream
+    "actnn_group_norm_backward": [c_vp] * 11 + [c_i64] * 4 + [c_i32, c_i32, c_vp, c_i64, c_vp],
     "actnn_stream_copy": [c_vp, c_vp, c_i64, c_vp],
     "actnn_matrix_pipe_probe": [c_vp, c_vp, c_i32, c_i32, c_vp],
     "actnn_batch_norm_workspace_bytes": [c_i64, c_i64, c_i64, c_i32, c_i32],
@@ -131,6 +136,7 @@ SIGNATURES = {
 _RESTYPES = {"actnn_strerror": ctypes.c_char_p, "actnn_version": ctypes.c_char_p,
              "actnn_linear_grad_weight_workspace_bytes": ctypes.c_int64,
              "actnn_tokens_matmul_workspace_bytes": ctypes.c_int64,
+             "actnn_group_norm_workspace_bytes": ctypes.c_int64,
              "actnn_tokens_grad_weight_workspace_bytes": ctypes.c_int64,
              "actnn_batch_norm_workspace_bytes": ctypes.c_int64,
              "actnn_batch_norm_forward_static_limit": ctypes.c_int64,

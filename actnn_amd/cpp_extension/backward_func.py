@@ -448,3 +448,30 @@ def layer_norm_backward_cuda(dY, X, mean, rstd, gamma, M, N, grad_input_mask):
     shape = None if gamma is None else gamma.shape
     return (None if dX is None else dX.view_as(X), None if dgamma is None or shape is None else dgamma.view(shape),
             None if dbeta is None or shape is None else dbeta.view(shape))
+
+
+# ------------------------------------------------------------------------------------------
+# group norm with its activation, channels last (no reference counterpart)
+# ------------------------------------------------------------------------------------------
+_ACTIVATIONS = {None: 0, "silu": 1}
+
+
+def _activation(activation):
+    if activation not in _ACTIVATIONS:
+        raise RuntimeError(f"group norm: the activation is None or 'silu', got {activation!r}")
+    return _ACTIVATIONS[activation]
+
+
+def hip_group_norm_forward(input, num_groups, weight, bias, eps, activation=None, keep=False):
+    """-> (output, mean, rstd, codes, scale): activation(group_norm(input)) of a float32, float16 or bfloat16 tensor
+    [N, C, ...] that is channels last - the channels of a pixel side by side in memory, as in torch.channels_last and in any
+    [N, C] tensor.  mean and rstd are fp32 [N, num_groups].  With `keep` the input also comes as int8 codes (laid out like it) with
+    one fp32 scale for each sample and group, what hip_group_norm_backward needs of it; None, None otherwise."""
+    return _glue.host().group_norm_forward(input, num_groups, weight, bias, eps, _activation(activation), keep)
+
+
+def hip_group_norm_backward(grad_output, codes, scale, num_groups, weight, bias, mean, rstd, activation=None, input=None):
+    """-> (grad_input, grad_weight, grad_bias) of hip_group_norm_forward, computed at the values the codes stand for, or
+    at `input` itself (codes and scale None).  The parameters' gradients are fp32, None without the parameter."""
+    return _glue.host().group_norm_backward(grad_output, codes, scale, input, num_groups, weight, bias, mean, rstd,
+                                            _activation(activation))

@@ -783,6 +783,141 @@ PyObject* linear_tokens_grad_weight(PyObject* const* a, Py_ssize_t n) {
   return wrap(out);
 }
 
+// ---------------------------------------------------------------------------- group norm
+// [N, C, ...] channels last as [N, ..., C], which is how it lies in memory; `dense`: it does
+struct Pixels {
+  Tensor held;
+  bool dense;
+  int64_t N, C, count = 1;
+  explicit Pixels(const Tensor& t, const char* name) {
+    check_float(t, name);
+    set(t, name);
+  }
+  Pixels(const Tensor& t, const char* name, at::ScalarType dtype) {
+    TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor!");
+    TORCH_CHECK(t.scalar_type() == dtype, "The type of ", name, " is not correct!");
+    set(t, name);
+  }
+  // a tensor of the same shape and layout, and its view in the order of the channels first
+  Tensor empty_like(at::ScalarType dtype) const { return empty(held.sizes(), held, dtype); }
+  static Tensor channels_first(const Tensor& t) {
+    if (t.dim() == 2) return t;
+    std::vector<int64_t> order{0, t.dim() - 1};
+    for (int64_t d = 1; d + 1 < t.dim(); ++d) order.push_back(d);
+    return t.permute(order);
+  }
+
+ private:
+  void set(const Tensor& t, const char* name) {
+    TORCH_CHECK(t.dim() >= 2, "The dimension of ", name, " is not correct!");
+    N = t.size(0);
+    C = t.size(1);
+    for (int64_t d = 2; d < t.dim(); ++d) count *= t.size(d);
+    std::vector<int64_t> order{0};
+    for (int64_t d = 2; d < t.dim(); ++d) order.push_back(d);
+    order.push_back(1);
+    held = t.dim() == 2 ? t : t.permute(order);
+    dense = held.is_contiguous();
+  }
+};
+struct GroupNorm {
+  int64_t groups;
+  Tensor weight, bias;
+  int activation;
+  GroupNorm(int64_t g, const Tensor& w, const Tensor& b, int64_t act, const Pixels& x) : groups(g), activation((int)act) {
+    TORCH_CHECK(groups >= 1 && x.C >= 1 && x.C % groups == 0, "the channels, ", x.C, ", must be a multiple of the groups, ", groups);
+    weight = parameter(w, x, "weight");
+    bias = parameter(b, x, "bias");
+  }
+  static Tensor parameter(const Tensor& t, const Pixels& x, const char* name) {
+    if (!t.defined()) return t;
+    check_float(t, name);
+    TORCH_CHECK(t.device() == x.held.device(), name, " must be on the same device");
+    TORCH_CHECK(t.numel() == x.C, name, " must have one value for each channel, ", x.C, ", and has ", t.numel());
+    return t.detach().to(at::kFloat).contiguous();
+  }
+};
+// (the kernels read 16 bytes: what torch allocates has room for them, a view at the end of a smaller tensor may not)
+Tensor with_room(const Tensor& t) { return t.nbytes() < 16 ? t.clone() : t; }
+
+// input, groups, weight | None, bias | None, eps, activation, whether the input is kept
+//   -> output, mean, rstd, codes | None, scale | None
+PyObject* group_norm_forward(PyObject* const* a, Py_ssize_t n) {
+  Args args(a, n, 7);
+  const Tensor input = args.tensor().detach();
+  const int64_t groups = args.integer();
+  const Tensor given_weight = args.optional(), given_bias = args.optional();
+  const double eps = args.number();
+  const int64_t activation = args.integer();
+  const bool keep = args.flag();
+  const Pixels x(input, "input");
+  TORCH_CHECK(x.dense, "input must be channels last: [N, C, ...] with the channels of a pixel side by side in memory");
+  const c10::DeviceGuard guard(input.device());
+  const GroupNorm norm(groups, given_weight, given_bias, activation, x);
+  const auto dtype = input.scalar_type();
+  const int code = code_of(dtype);
+  const Tensor from = with_room(x.held), y = x.empty_like(dtype);
+  const Tensor mean = empty({x.N, groups}, input, at::kFloat), rstd = empty({x.N, groups}, input, at::kFloat);
+  const Tensor codes = keep ? x.empty_like(at::kChar) : Tensor(), scale = keep ? empty({x.N, groups}, input, at::kFloat) : Tensor();
+  const int64_t bytes = actnn_group_norm_workspace_bytes(x.N, x.C, x.count, groups, code, 0);
+  const Tensor workspace = empty({bytes > 0 ? bytes : 0}, input, at::kByte);
+  if (x.count == 0) {
+    mean.zero_();
+    rstd.zero_();
+    if (keep) scale.zero_();
+  }
+  launch("group_norm_forward", [&] {
+    return actnn_group_norm_forward(ptr(from), f32(norm.weight), f32(norm.bias), ptr(y), f32(mean), f32(rstd),
+                                    static_cast<int8_t*>(ptr(codes)), f32(scale), x.N, x.C, x.count, groups, eps,
+                                    norm.activation, code, ptr(workspace), bytes, stream_of(input));
+  });
+  return tuple_of(Pixels::channels_first(y), mean, rstd, keep ? Pixels::channels_first(codes) : Tensor(), scale);
+}
+
+// grad_output, codes | None, scale | None, input | None, groups, weight | None, bias | None, mean, rstd, activation
+//   -> gradients of the input, the weight and the bias (None where there is none)
+PyObject* group_norm_backward(PyObject* const* a, Py_ssize_t n) {
+  Args args(a, n, 10);
+  const Tensor grad_output = args.tensor().detach();
+  const Tensor codes = args.optional(), given_scale = args.optional(), input = args.optional();
+  const int64_t groups = args.integer();
+  const Tensor given_weight = args.optional(), given_bias = args.optional(), given_mean = args.tensor(), given_rstd = args.tensor();
+  const int64_t activation = args.integer();
+  TORCH_CHECK(codes.defined() != input.defined() && codes.defined() == given_scale.defined(),
+              "group_norm_backward: either codes and scale or the input");
+  Pixels dy(grad_output, "grad_output");
+  const c10::DeviceGuard guard(grad_output.device());
+  const auto dtype = grad_output.scalar_type();
+  const Tensor& saved = codes.defined() ? codes : input;
+  const Pixels x(saved.detach(), codes.defined() ? "codes" : "input", codes.defined() ? at::kChar : dtype);
+  TORCH_CHECK(saved.sizes() == grad_output.sizes(), "grad_output ", grad_output.sizes(), " and the saved input ", saved.sizes(),
+              " are not of the same shape");
+  TORCH_CHECK(saved.device() == grad_output.device(), "the saved input must be on the same device");
+  const GroupNorm norm(groups, given_weight, given_bias, activation, dy);
+  const Tensor mean = row_scales(given_mean, dy.N * groups, grad_output, "mean");
+  const Tensor rstd = row_scales(given_rstd, dy.N * groups, grad_output, "rstd");
+  const Tensor scale = codes.defined() ? row_scales(given_scale, dy.N * groups, grad_output, "scale") : Tensor();
+  const Tensor grad = with_room(dy.held.contiguous()), kept = codes.defined() ? x.held.contiguous() : with_room(x.held.contiguous());
+  const Tensor dx = dy.empty_like(dtype);
+  const Tensor dweight = norm.weight.defined() ? empty({dy.C}, grad, at::kFloat) : Tensor();
+  const Tensor dbias = norm.bias.defined() ? empty({dy.C}, grad, at::kFloat) : Tensor();
+  if (dx.numel() == 0) {
+    if (dweight.defined()) dweight.zero_();
+    if (dbias.defined()) dbias.zero_();
+  } else {
+    const int code = code_of(dtype);
+    const int64_t bytes = actnn_group_norm_workspace_bytes(dy.N, dy.C, dy.count, groups, code, 1);
+    const Tensor workspace = empty({bytes > 0 ? bytes : 0}, grad, at::kByte);
+    launch("group_norm_backward", [&] {
+      return actnn_group_norm_backward(ptr(grad), codes.defined() ? static_cast<int8_t*>(ptr(kept)) : nullptr, f32(scale),
+                                       codes.defined() ? nullptr : ptr(kept), f32(norm.weight), f32(norm.bias), f32(mean), f32(rstd),
+                                       ptr(dx), f32(dweight), f32(dbias), dy.N, dy.C, dy.count, groups, norm.activation, code,
+                                       ptr(workspace), bytes, stream_of(grad));
+    });
+  }
+  return tuple_of(Pixels::channels_first(dx), dweight, dbias);
+}
+
 template <PyObject* (*F)(PyObject* const*, Py_ssize_t)>
 PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -796,7 +931,7 @@ PyMethodDef methods[] = {
     ACTNN_CALL(batch_norm_geometry), ACTNN_CALL(batch_norm_forward_quantize), ACTNN_CALL(batch_norm_forward), ACTNN_CALL(batch_norm_backward),
     ACTNN_CALL(batch_norm_backward_packed), ACTNN_CALL(max_pool2d_forward), ACTNN_CALL(max_pool2d_backward),
     ACTNN_CALL(quantize_tokens), ACTNN_CALL(dequantize_tokens), ACTNN_CALL(matmul_tokens), ACTNN_CALL(linear_tokens),
-    ACTNN_CALL(linear_tokens_grad_weight), {nullptr, nullptr, 0, nullptr}};
+    ACTNN_CALL(linear_tokens_grad_weight), ACTNN_CALL(group_norm_forward), ACTNN_CALL(group_norm_backward), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods};
 
 }  // namespace

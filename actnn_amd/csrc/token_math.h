@@ -33,11 +33,13 @@ ACTNN_DEV TokenScale token_scale(float top) {
 // (an int conversion of a value that no int holds is one instruction that clamps, and `keep` drops what it gave)
 template <typename T> struct Coder {
   float factor;
+  Coder() = default;
   ACTNN_DEV explicit Coder(float top) : factor((127.0f / top) * (1.0f + 0x1p-21f)) {}
   ACTNN_DEV int code(float x) const { return (int)__builtin_fmaf(x, factor, __builtin_copysignf(0.5f, x)); }
 };
 template <> struct Coder<float> {
   double factor;
+  Coder() = default;
   ACTNN_DEV explicit Coder(float top) : factor((127.0 / (double)top) * (1.0 + 0x1p-45)) {}
   ACTNN_DEV int code(float x) const { return (int)__builtin_fma((double)x, factor, __builtin_copysign(0.5, (double)x)); }
 };

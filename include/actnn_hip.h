@@ -537,6 +537,25 @@ int actnn_tokens_grad_weight(const void* grad_out, int64_t ldg, const int8_t* co
                              void* grad_w, int64_t M, int64_t O, int64_t I, int go_dtype, int out_dtype, void* workspace,
                              int64_t workspace_bytes, void* stream);
 
+/* ---------------------------------------------------------------------------------
+ * Group norm with its activation (no reference counterpart), channels last: x, y, gradients and codes are dense
+ * [N, pixels, C] in memory, at any element address (a tensor below 16 bytes has room for 16).  Statistics over the pixels
+ * and the C / groups channels of a group of each sample, in fp32; weight and bias fp32 [C] or null.
+ *   forward:   z = (x - mean) * rstd * weight + bias, y = z (activation 0) or z * sigmoid(z) (1); mean, rstd [N, groups].
+ *              codes (null: not kept): x as int8 with one scale for each sample and group, scale [N, groups], the
+ *              rounding of the 8-bit tokens.
+ *   backward:  from codes and scale, or codes null and x itself; dx (null: not wanted) in dtype, dweight, dbias fp32 [C]
+ *              or null.  N and pixels are not 0.
+ * ------------------------------------------------------------------------------- */
+int64_t actnn_group_norm_workspace_bytes(int64_t N, int64_t C, int64_t pixels, int64_t groups, int dtype, int backward);
+int actnn_group_norm_forward(const void* x, const float* weight, const float* bias, void* y, float* mean, float* rstd,
+                             int8_t* codes, float* scale, int64_t N, int64_t C, int64_t pixels, int64_t groups, double eps,
+                             int activation, int dtype, void* workspace, int64_t workspace_bytes, void* stream);
+int actnn_group_norm_backward(const void* dy, const int8_t* codes, const float* scale, const void* x, const float* weight,
+                              const float* bias, const float* mean, const float* rstd, void* dx, float* dweight,
+                              float* dbias, int64_t N, int64_t C, int64_t pixels, int64_t groups, int activation, int dtype,
+                              void* workspace, int64_t workspace_bytes, void* stream);
+
 /* Plain device-to-device streaming copy of `bytes` bytes (16-byte aligned pointers and
  * size); used by the benchmark to calibrate bandwidth counters.  No reference counterpart. */
 int actnn_stream_copy(const void* src, void* dst, int64_t bytes, void* stream);

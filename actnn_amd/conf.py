@@ -53,6 +53,10 @@ class QuantizationConfig:
         # before the library multiplies them: 6-10 % less time for the layer, at one more tensor of the output
         # gradient's size (at most 128 MB) while the product runs.  False keeps the backward's peak where it is without
         self.linear_factors_by_sample = True
+        # layers that QModule puts in only where asked: linear layers that multiply in 8-bit integers and keep what they
+        # multiplied (QInt8Linear), and group norms that keep their input in 8 bits (QGroupNorm)
+        self.enable_int8_linear = False
+        self.enable_quantized_gn = False
         self.pool_index_nibbles = True                 # max-pool keeps its arg-max indices two per byte
         # memory management (conf.py:54-58)
         self.empty_cache_threshold = None

@@ -14,13 +14,16 @@ from torch.nn.modules.pooling import _AvgPoolNd, _MaxPoolNd
 from torch.nn.modules.utils import _pair, _single, _triple
 
 from .conf import config
+from .cpp_extension import backward_func as ext_backward_func
 from .cpp_extension import quantization as ext_quantization
+from .cpp_extension import tokens as ext_tokens
 from .ops import (SkipGradient, batch_norm, batch_norm_add_relu, batch_norm_relu, batch_norm_relu_geometry, conv1d,
-                  conv2d, conv3d, conv_transpose1d, conv_transpose2d, conv_transpose3d, linear)
+                  conv2d, conv3d, conv_transpose1d, conv_transpose2d, conv_transpose3d, group_norm,
+                  int8_linear, linear)
 from .ops import skip_connection as ops_skip_connection
 from .qbnscheme import QBNScheme
 from .qscheme import QScheme
-from .utils import channels_last_format, logical_order, memory_order
+from .utils import channels_last_format, logical_order, memory_order, to_channels_last
 
 
 def _autocast_apply(fn, *args):
@@ -190,6 +193,74 @@ class QLinear(nn.Linear):
         if not config.training:
             return super().forward(input)
         return _autocast_apply(linear, input, self.weight, self.bias, self.scheme)
+
+
+def _wants_grad(*tensors):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+class QInt8Linear(nn.Linear):
+    """A linear layer that multiplies in 8-bit integers - one scale for each token (row of the input) and each output channel -
+    and keeps, of its input, the codes it multiplied: a byte a value.  In training the weight is rounded anew in every forward
+    pass and its gradient is that of the kept values.
+
+    A layer that only answers rounds its weight once: `hold_weight()`, to be called again after the weight has been replaced
+    (changes in place, load_state_dict, .to() and train() are noticed and end the hold)."""
+
+    _held = None
+
+    def hold_weight(self):
+        with torch.no_grad():
+            self._held = (self.weight, self.weight._version, *ext_tokens.quantize_tokens(self.weight))
+        return self
+
+    def _weight_tokens(self):
+        held = self._held
+        if held is not None and held[0] is self.weight and held[1] == self.weight._version:
+            return held[2:]
+        self._held = None
+        return ext_tokens.quantize_tokens(self.weight)
+
+    def _apply(self, fn, recurse=True):
+        self._held = None
+        return super()._apply(fn, recurse)
+
+    def train(self, mode=True):
+        if mode:
+            self._held = None
+        return super().train(mode)
+
+    def __getstate__(self):
+        return {k: v for k, v in self.__dict__.items() if k != "_held"}
+
+    def forward(self, input):
+        if _wants_grad(input, self.weight, self.bias):
+            return _autocast_apply(int8_linear, input, self.weight, self.bias)
+        if torch.is_autocast_enabled("cuda"):
+            input = input.to(torch.get_autocast_dtype("cuda"))
+        return ext_tokens.linear_tokens(input, *self._weight_tokens(), self.bias)
+
+
+class QGroupNorm(nn.GroupNorm):
+    """Group norm over the channels-last layout that keeps its input in 8 bits, one scale for each sample and group.  An input
+    laid out otherwise is copied, the output is channels last.  As with batch norm the statistics and parameters stay
+    fp32 under autocast and the input is taken in its own type."""
+
+    def forward(self, input, silu=False):
+        """`silu`: the SiLU that follows this layer, in the same pass (gn_silu)."""
+        input = to_channels_last(input)
+        activation = "silu" if silu else None
+        if _wants_grad(input, self.weight, self.bias):
+            return group_norm.apply(input, self.num_groups, self.weight, self.bias, self.eps, activation)
+        return ext_backward_func.hip_group_norm_forward(input, self.num_groups, self.weight, self.bias, self.eps, activation)[0]
+
+
+def gn_silu(gn, silu, input):
+    """silu(gn(input)) for a model that knows the two layers follow each other: a converted group norm applies the SiLU in
+    its own pass, everything else is the two calls."""
+    if isinstance(gn, QGroupNorm) and type(silu) is nn.SiLU:
+        return gn(input, silu=True)
+    return silu(gn(input))
 
 
 class _QBatchNormMixin:

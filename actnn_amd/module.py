@@ -7,11 +7,12 @@ import torch.nn as nn
 
 from .conf import config
 from .layers import (AddReLU, QAddReLU, QAvgPool2d, QBatchNorm1d, QBatchNorm2d, QBatchNorm3d, QConv1d, QConv2d, QConv3d,
-                     QConvTranspose1d, QConvTranspose2d, QConvTranspose3d, QDropout, QLinear, QMaxPool2d,
-                     QReLU, QSyncBatchNorm)
+                     QConvTranspose1d, QConvTranspose2d, QConvTranspose3d, QDropout, QGroupNorm, QInt8Linear, QLinear,
+                     QMaxPool2d, QReLU, QSyncBatchNorm)
 
 _Q_TYPES = (QConv1d, QConv2d, QConv3d, QConvTranspose1d, QConvTranspose2d, QConvTranspose3d, QBatchNorm1d,
-            QBatchNorm2d, QBatchNorm3d, QSyncBatchNorm, QReLU, QAddReLU, QDropout, QLinear, QMaxPool2d, QAvgPool2d)
+            QBatchNorm2d, QBatchNorm3d, QSyncBatchNorm, QReLU, QAddReLU, QDropout, QLinear, QInt8Linear, QMaxPool2d, QAvgPool2d,
+            QGroupNorm)
 
 
 def _convert(child):
@@ -34,6 +35,10 @@ def _convert(child):
             if isinstance(child, bn):
                 return qbn(child.num_features, child.eps, child.momentum, child.affine,
                            child.track_running_stats)
+    if config.enable_quantized_gn and isinstance(child, nn.GroupNorm):
+        return QGroupNorm(child.num_groups, child.num_channels, child.eps, child.affine)
+    if config.enable_int8_linear and isinstance(child, nn.Linear):
+        return QInt8Linear(child.in_features, child.out_features, child.bias is not None)
     if isinstance(child, nn.Linear):
         return QLinear(child.in_features, child.out_features, child.bias is not None)
     if isinstance(child, nn.ReLU):

@@ -14,6 +14,7 @@ from .conf import config
 from .cpp_extension import backward_func as ext_backward_func
 from .cpp_extension import minimax as ext_minimax
 from .cpp_extension import quantization as ext_quantization
+from .cpp_extension import tokens as ext_tokens
 from .utils import (channels_last_format, compute_tensor_bytes, empty_cache, get_memory_usage,
                     logical_order, memory_order, swap_to_cpu, swap_to_device)
 
@@ -544,6 +545,39 @@ class linear(Function):
         return grad_input, grad_weight, grad_bias, None
 
 
+class int8_linear(Function):
+    """Linear layer multiplied in 8-bit integers: the input one scale a token, the weight one an output channel.  The tokens as
+    they were multiplied are all that is kept of the input, and the weight's gradient is that of the values they stand for.  To the
+    gradients the rounding of either factor is the identity: grad_input = grad_output @ weight."""
+
+    @staticmethod
+    def forward(ctx, input, weight, bias=None):
+        weight_codes, weight_scale = ext_tokens.quantize_tokens(weight)
+        output, codes, scale = ext_tokens.linear_tokens(input, weight_codes, weight_scale, bias, keep=True)
+        empty_cache(config.empty_cache_threshold)
+        ctx.save_for_backward(codes, scale, weight)
+        ctx.bias_dtype = None if bias is None else bias.dtype
+        return output
+
+    @staticmethod
+    def backward(ctx, grad_output):
+        codes, scale, weight = ctx.saved_tensors
+        go = grad_output.reshape(-1, grad_output.shape[-1])
+        grad_input = grad_weight = grad_bias = None
+        if ctx.needs_input_grad[1]:
+            if go.dtype == torch.float32:
+                values = ext_tokens.dequantize_tokens(codes, scale).reshape(-1, codes.shape[-1])
+                grad_weight = go.t().mm(values).to(weight.dtype)
+            else:
+                grad_weight = ext_tokens.linear_tokens_grad_weight(
+                    grad_output, codes, scale, torch.float32 if weight.dtype == torch.float32 else None).to(weight.dtype)
+        if ctx.needs_input_grad[0]:
+            grad_input = go.mm(weight.to(go.dtype)).view(codes.shape)
+        if ctx.bias_dtype is not None and ctx.needs_input_grad[2]:
+            grad_bias = go.sum(0, dtype=torch.float32).to(ctx.bias_dtype)
+        return grad_input, grad_weight, grad_bias
+
+
 # ------------------------------------------------------------------------------------------
 # batch norm (ops.py:436-502)
 # ------------------------------------------------------------------------------------------
@@ -851,6 +885,30 @@ class batch_norm_add_relu(Function):
         masked = [] if ctx.needs_input_grad[1] else None
         grads = _batch_norm_backward(ctx, grad_output, relu_mask=mask, keep_masked=masked)
         return (grads[0], masked[0] if masked else None) + grads[1:] + (None, None)
+
+
+class group_norm(Function):
+    """Group norm with its activation (None or "silu") of a channels-last input, of which 8-bit codes with one scale for each
+    sample and group are kept (config.compress_activation off: the input itself).  The gradients are those at the kept
+    values, with the statistics of the input."""
+
+    @staticmethod
+    def forward(ctx, input, num_groups, weight, bias, eps, activation=None):
+        keep = config.compress_activation
+        output, mean, rstd, codes, scale = ext_backward_func.hip_group_norm_forward(
+            input, num_groups, weight, bias, eps, activation, keep)
+        empty_cache(config.empty_cache_threshold)
+        ctx.save_for_backward(codes, scale, None if keep else input, weight, bias, mean, rstd)
+        ctx.num_groups, ctx.activation = num_groups, activation
+        return output
+
+    @staticmethod
+    def backward(ctx, grad_output):
+        codes, scale, input, weight, bias, mean, rstd = ctx.saved_tensors
+        grad_input, grad_weight, grad_bias = ext_backward_func.hip_group_norm_backward(
+            grad_output, codes, scale, ctx.num_groups, weight, bias, mean, rstd, ctx.activation, input)
+        return (grad_input, None, None if weight is None else grad_weight.to(weight.dtype),
+                None if bias is None else grad_bias.to(bias.dtype), None, None)
 
 
 class SkipGradient:

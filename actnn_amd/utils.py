@@ -121,6 +121,14 @@ def logical_order(t_mem, memory_format):
     return t_mem.permute(0, t_mem.dim() - 1, *range(1, t_mem.dim() - 1))
 
 
+def to_channels_last(t):
+    """`t` [N, C, ...] with the channels of a pixel side by side in memory: itself where it lies like that, else a copy."""
+    if t.dim() < 3:
+        return t.contiguous()
+    rows = t.permute(0, *range(2, t.dim()), 1)
+    return t if rows.is_contiguous() else rows.contiguous().permute(0, t.dim() - 1, *range(1, t.dim() - 1))
+
+
 def get_memory_usage(print_info=False):
     """Bytes currently allocated by torch's caching allocator on device 0 - the reference's
     memory metric (utils.py:16-23; explicitly not the driver's view)."""

@@ -46,6 +46,16 @@ ACTNN_DEV u32x4 lds_load16(uint32_t address) {
   return *reinterpret_cast<const __attribute__((address_space(3))) u32x4*>((lds_ptr_t)(uintptr_t)address);
 }
 
+ACTNN_DEV void lds_store16(uint32_t address, u32x4 v) {
+  *reinterpret_cast<__attribute__((address_space(3))) u32x4*>((lds_ptr_t)(uintptr_t)address) = v;
+}
+// between writes and reads of the same wave: LDS operations of a wave complete in order
+ACTNN_DEV void wave_lds_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // the first `valid` of 16 bytes, the others 0
 ACTNN_DEV u32x4 first_bytes(u32x4 v, int valid) {
   uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -90,6 +100,25 @@ template <> ACTNN_DEV void put4<int>(const Product& p, int64_t token, int channe
 #pragma unroll
   for (int i = 0; i < 4; ++i)
     if (channel + i < p.O) to[i] = sum[i];
+}
+
+// the integer sums of 16 bytes' worth of channels of a token, of which `valid` exist
+template <typename TY, int V>
+ACTNN_DEV void put_row(const Product& p, int64_t token, int channel, int valid, const int (&sum)[V], const float (&ws)[V],
+                       const float (&bias)[V]) {
+  TY* to = static_cast<TY*>(p.y) + token * p.O + channel;
+  if constexpr (std::is_same<TY, int>::value) {
+    store16_part<false>(reinterpret_cast<float*>(to), (u32x4){(uint32_t)sum[0], (uint32_t)sum[1], (uint32_t)sum[2], (uint32_t)sum[3]}, valid);
+  } else {
+    float v[V];
+    const float xs = p.xs[token];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      v[i] = (float)sum[i] * xs * ws[i];
+      if (p.bias) v[i] += bias[i];
+    }
+    store16_part<false>(to, narrow(static_cast<const TY*>(nullptr), v), valid);
+  }
 }
 
 // ------------------------------------------------------------------------------------------
@@ -226,19 +255,51 @@ __global__ __launch_bounds__(kThreads, 1) void tokens_tile_kernel(Product p, int
   }
   for_each<kGroup>([&](auto G) { mma(Const<3>{}, decltype(G)::value / NA, decltype(G)::value % NA); });
 
-  // accumulator register c of a lane: channel 8 (c / 4) + 4 (lane / 32) + c % 4 of the fragment, token lane % 32
+  // Accumulator register c of a lane: channel 8 (c / 4) + 4 (lane / 32) + c % 4 of the fragment, token lane % 32.  Stored
+  // from there a wave would write 8 bytes each into 32 rows.  The sums go through LDS instead (all of it is free: the last
+  // fragments were read before the last barrier), 32 tokens of the wave's channels at a time, and come back with a lane's
+  // channels side by side: whole lines, and a lane's scales and biases are the same for all its tokens.
+  constexpr int kChannels = 32 * NA, kPitch = 4 * kChannels + 16;     // bytes a token; the 16 keep rows off the same banks
+  constexpr int V = sizeof(TY) == 2 ? 8 : 4;                          // channels of a 16-byte store
+  constexpr int kAcross = kChannels / V, kDown = 64 / kAcross;        // lanes to a token, tokens to an instruction
+  static_assert(4 * 32 * kPitch <= 2 * kBuffer, "the sums of 32 tokens of four waves fit where the tiles were");
+  const uint32_t slab = lds0 + (uint32_t)(wave * 32 * kPitch);
+  const int channel = o0 + wr * kChannels + lane % kAcross * V;
+  const int valid = p.O - channel;
+  float ws[V], bias[V];
+  if constexpr (!std::is_same<TY, int>::value) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int c = channel + i < p.O ? channel + i : p.O - 1;
+      ws[i] = p.ws[c];
+      bias[i] = p.bias ? p.bias[c] : 0.0f;
+    }
+  }
 #pragma unroll
   for (int e = 0; e < NE; ++e) {
-    const int64_t token = t0 + wn * 32 * NE + 32 * e + (lane & 31);
 #pragma unroll
-    for (int a = 0; a < NA; ++a) {
+    for (int a = 0; a < NA; ++a)
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int channel = o0 + wr * 32 * NA + 32 * a + 8 * q + 4 * (lane >> 5);
-        const int sum[4] = {acc[e][a][4 * q], acc[e][a][4 * q + 1], acc[e][a][4 * q + 2], acc[e][a][4 * q + 3]};
-        if (channel < p.O) put4<TY>(p, token, channel, sum);
+      for (int q = 0; q < 4; ++q)
+        lds_store16(slab + (uint32_t)((lane & 31) * kPitch + 4 * (32 * a + 8 * q + 4 * (lane >> 5))),
+                    (u32x4){(uint32_t)acc[e][a][4 * q], (uint32_t)acc[e][a][4 * q + 1], (uint32_t)acc[e][a][4 * q + 2],
+                            (uint32_t)acc[e][a][4 * q + 3]});
+    wave_lds_fence();
+    const int64_t first_token = t0 + wn * 32 * NE + 32 * e;
+#pragma unroll
+    for (int j = 0; j < 32 / kDown; ++j) {
+      const int in = j * kDown + lane / kAcross;
+      const int64_t token = first_token + in;
+      const uint32_t at = slab + (uint32_t)(in * kPitch + lane % kAcross * V * 4);
+      int sum[V];
+#pragma unroll
+      for (int i = 0; i < V; i += 4) {
+        const u32x4 v = lds_load16(at + 4 * i);
+        sum[i] = (int)v.x; sum[i + 1] = (int)v.y; sum[i + 2] = (int)v.z; sum[i + 3] = (int)v.w;
       }
+      if (token < p.M && valid > 0) put_row<TY>(p, token, channel, valid, sum, ws, bias);
     }
+    wave_lds_fence();
   }
 }
 

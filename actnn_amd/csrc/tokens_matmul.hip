@@ -10,9 +10,9 @@
 //   * few tokens: bound by reading the weight once.  No tiles: a wave's lanes load their 16 bytes of 16 channels' rows
 //     straight into the operand registers of v_mfma_i32_16x16x64_i8, the waves of a block share the features of the same
 //     channels and add their sums in LDS.
-//   * tiles of 64, 128 or 256 channels by as many tokens, for everything else: v_mfma_i32_32x32x32_i8 out of LDS.  Two buffers of
-//     128 features; both operands go from global memory straight into LDS (global_load_lds, 16 bytes a lane), rows as they lie in
-//     memory, their eight 16-byte chunks at chunk ^ (row / 2) % 8: 16 rows of two banks' widths meet every bank once.
+//   * tiles of 64, 128 or 256 channels by as many tokens, for everything else: v_mfma_i32_32x32x32_i8 out of LDS.  Four buffers of
+//     64 features; both operands go from global memory straight into LDS (global_load_lds, 16 bytes a lane), rows as they lie in
+//     memory, their four 16-byte chunks at chunk ^ (row / 4) % 4: 16 rows that are read together meet every bank once.
 //   * tiles that do not fill the chip take slices of the features; a second kernel adds the slices.
 // Rows and channels past the end are read from the last one and not stored; features past the end are read from the
 // step's first chunk and masked out of the weight's operand.
@@ -49,6 +49,8 @@ ACTNN_DEV u32x4 lds_load16(uint32_t address) {
 ACTNN_DEV void lds_store16(uint32_t address, u32x4 v) {
   *reinterpret_cast<__attribute__((address_space(3))) u32x4*>((lds_ptr_t)(uintptr_t)address) = v;
 }
+// what s_waitcnt takes to wait for LDS and for all but the last n loads
+constexpr int waitcnt_all_but(int n) { return (n & 15) | 7 << 4 | (n >> 4) << 14; }
 // between writes and reads of the same wave: LDS operations of a wave complete in order
 ACTNN_DEV void wave_lds_fence() {
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -126,40 +128,46 @@ ACTNN_DEV void put_row(const Product& p, int64_t token, int channel, int valid, 
 // ------------------------------------------------------------------------------------------
 template <typename TY, int NA, int NE>
 __global__ __launch_bounds__(kThreads, 1) void tokens_tile_kernel(Product p, int slices, int steps_per_slice) {
-  constexpr int BO = 64 * NA, BT = 64 * NE, BK = 128;
+  constexpr int BO = 64 * NA, BT = 64 * NE, BK = 64, kBuffers = 4;
   constexpr int kBuffer = (BO + BT) * BK;
-  constexpr int kGroup = NA * NE, kSlots = 4 * kGroup, kFragments = NA + NE;
+  constexpr int kGroup = NA * NE, kSlots = 2 * kGroup, kFragments = NA + NE;
   constexpr int kReads = (kFragments + kGroup - 1) / kGroup;          // fragment reads beside an MFMA
-  constexpr int kPieces = kBuffer / (kThreads * 16);                  // direct loads of a wave and step
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[2 * kBuffer];
+  constexpr int kPieces = NA + NE;                                    // direct loads of a wave and step: 16 rows each
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[kBuffers * kBuffer];
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wr = wave & 1, wn = wave >> 1;
   const int tiles_o = (p.O + BO - 1) / BO, tiles_t = (p.M + BT - 1) / BT;
   const int slice = slices > 1 ? blockIdx.x / (tiles_o * tiles_t) : 0;
-  int tile = slices > 1 ? blockIdx.x % (tiles_o * tiles_t) : blockIdx.x;
+  const int tile = slices > 1 ? blockIdx.x % (tiles_o * tiles_t) : blockIdx.x;
+  int tile_t = tile / tiles_o, tile_o = tile % tiles_o;
   if (slices == 1 && tiles_t % 8 == 0) {
-    // blocks are dealt round-robin to the 8 XCDs: each gets whole panels of tokens, which stay in its L2
-    const int xcd = blockIdx.x & 7, i = blockIdx.x >> 3;
-    tile = (xcd * (tiles_t / 8) + i / tiles_o) * tiles_o + i % tiles_o;
+    // Blocks are dealt round-robin to the 8 XCDs: each gets panels of tokens of its own, and takes them by 8 tiles of
+    // channels, so that the tiles at work at one time share their operands in its L2.
+    const int xcd = blockIdx.x & 7, i = blockIdx.x >> 3, panels = tiles_t / 8;
+    const int strip = i / (panels * 8), in = i - strip * panels * 8;
+    const int wide = tiles_o - strip * 8 < 8 ? tiles_o - strip * 8 : 8;
+    tile_t = xcd * panels + in / wide;
+    tile_o = strip * 8 + in % wide;
   }
-  const int t0 = tile / tiles_o * BT, o0 = tile % tiles_o * BO;
+  const int t0 = tile_t * BT, o0 = tile_o * BO;
   const int all_steps = (p.K + BK - 1) / BK;
   const int first = slice * steps_per_slice;
   int steps = all_steps - first;
   if (slices > 1 && steps > steps_per_slice) steps = steps_per_slice;
   if (slices > 1) p.y = static_cast<int*>(p.y) + (int64_t)slice * p.M * p.O;
   const int chunks = (p.K + 15) / 16;
+  const int features = (p.K < (first + steps) * BK ? p.K : (first + steps) * BK) - first * BK;     // of this block
 
-  // ---- direct loads: piece j is 8 rows of the weight's tile or, behind those, of the tokens'
-  const int row_in = lane >> 3;
-  const int chunk = (lane & 7) ^ (((wave & 1) << 2) | (row_in >> 1));
+  // ---- direct loads: piece j is 16 rows of the weight's tile or, behind those, of the tokens'
+  const int row_in = lane >> 2;
+  const int chunk = (lane & 3) ^ ((lane >> 4) & 3);
   uint32_t off[kPieces];
 #pragma unroll
   for (int i = 0; i < kPieces; ++i) {
-    const int row = 8 * (wave + 4 * i) + row_in;
-    if (i < BO / 32) {
+    const int row = 16 * (wave + 4 * i) + row_in;
+    if (i < NA) {
       const int at = o0 + row < p.O ? row : p.O - 1 - o0;
       off[i] = (uint32_t)at * (uint32_t)p.ldw + (uint32_t)chunk * 16u;
     } else {
@@ -169,19 +177,22 @@ __global__ __launch_bounds__(kThreads, 1) void tokens_tile_kernel(Product p, int
   }
   const int8_t* wp = p.w + (int64_t)o0 * p.ldw;
   const int8_t* xp = p.x + (int64_t)t0 * p.ldx;
-  auto load_piece = [&](int buffer, int step, auto I) {
+  // (a step past the block's last loads that one again: nobody reads it)
+  auto load_piece = [&](auto BUF, int t, auto I) {
     constexpr int i = decltype(I)::value;
+    const int step = first + (t < steps ? t : steps - 1);
     uint32_t at = off[i];
-    if (step * 8 + chunk >= chunks) at -= (uint32_t)chunk * 16u;       // past the row's end: the step's first chunk
-    const int8_t* base = (i < BO / 32 ? wp : xp) + (int64_t)step * BK;
-    load_to_lds16_base(base, at, smem + buffer * kBuffer + (wave + 4 * i) * 1024);
+    if (step * 4 + chunk >= chunks) at -= (uint32_t)chunk * 16u;       // past the row's end: the step's first chunk
+    const int8_t* base = (i < NA ? wp : xp) + (int64_t)step * BK;
+    load_to_lds16_base(base, at, smem + decltype(BUF)::value * kBuffer + (wave + 4 * i) * 1024);
   };
 
   // ---- fragments: lane -> row lane % 32, features 32 kb + 16 (lane / 32) ..
   const uint32_t lds0 = lds_address(smem);
-  const uint32_t in_row = (uint32_t)(lane & 31) * BK + (uint32_t)((((lane >> 5) ^ (lane >> 1)) & 7) << 4);
+  const uint32_t in_row = (uint32_t)(lane & 31) * BK + (uint32_t)(((lane >> 5) ^ ((lane >> 2) & 3)) << 4);
   const uint32_t at_w = lds0 + (uint32_t)(wr * 32 * NA) * BK + in_row;
   const uint32_t at_x = lds0 + (uint32_t)(BO + wn * 32 * NE) * BK + in_row;
+  const uint32_t at_w2 = at_w ^ 32u, at_x2 = at_x ^ 32u;              // the second k-block
 
   i32x16 acc[NE][NA];
 #pragma unroll
@@ -198,62 +209,69 @@ __global__ __launch_bounds__(kThreads, 1) void tokens_tile_kernel(Product p, int
 #pragma unroll
     for (int e = 0; e < NE; ++e) fx[h][e] = (u32x4){0u, 0u, 0u, 0u};
   }
-  // valid: bytes of the weight's fragment that exist (16 but in the last step)
-  auto read_fragment = [&](auto BUF, auto KB, auto F, auto TAIL, int step) {
+  auto read_fragment = [&](auto BUF, auto KB, auto F, auto TAIL, int t) {
     constexpr int kb = decltype(KB)::value, f = decltype(F)::value;
     constexpr uint32_t buf = decltype(BUF)::value * kBuffer;
     if constexpr (f < NA) {
-      u32x4 v = lds_load16((at_w ^ (kb << 5)) + buf + f * 32 * BK);
-      if constexpr (decltype(TAIL)::value != 0) v = first_bytes(v, p.K - (step * BK + kb * 32 + (lane >> 5) * 16));
-      fw[kb & 1][f] = v;
+      u32x4 v = lds_load16((kb ? at_w2 : at_w) + buf + f * 32 * BK);
+      if constexpr (decltype(TAIL)::value != 0) v = first_bytes(v, features - (t * BK + kb * 32 + (lane >> 5) * 16));
+      fw[kb][f] = v;
     } else {
-      fx[kb & 1][f - NA] = lds_load16((at_x ^ (kb << 5)) + buf + (f - NA) * 32 * BK);
+      fx[kb][f - NA] = lds_load16((kb ? at_x2 : at_x) + buf + (f - NA) * 32 * BK);
     }
   };
   auto mma = [&](auto KB, int e, int a) {
-    constexpr int h = decltype(KB)::value & 1;
+    constexpr int h = decltype(KB)::value;
     acc[e][a] = __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(i32x4, fw[h][a]), __builtin_bit_cast(i32x4, fx[h][e]),
                                                       acc[e][a], 0, 0, 0);
   };
 
-  // Between two barriers: the MFMAs of the last k-block of the step before (its fragments are in registers) and of the
-  // first three of this step, the fragments of each k-block read beside the MFMAs of the one before, and the direct loads of
-  // the next step into the other buffer.
-  auto step = [&](auto BUF, auto TAIL, int t) {
+  // Step t is multiplied out of buffer t % 4.  Between two barriers: the MFMAs of the second k-block of the step before (its
+  // fragments are in registers) and of the first of this one, the fragments of each k-block read beside the MFMAs of the
+  // one before, and the direct loads of step t + 3 into the buffer whose last readers passed the barrier before.  The step
+  // ends when the loads of step t + 1 have landed: those of two steps may be on their way.
+  constexpr int kLandedOne = waitcnt_all_but(2 * kPieces);
+  // (no branches in a body: the compiler's own waits for LDS then stay exact)
+  auto step = [&](auto BUF, auto TAIL, auto AHEAD, int t) {
     constexpr int buf = decltype(BUF)::value;
+    constexpr bool ahead = decltype(AHEAD)::value != 0;
     for_each<kSlots>([&](auto S) {
       constexpr int slot = decltype(S)::value, in = slot % kGroup;
-      mma(Const<(slot / kGroup + 3) % 4>{}, in / NA, in % NA);
+      mma(Const<1 - slot / kGroup>{}, in / NA, in % NA);
       for_each<kReads>([&](auto R) {
         constexpr int f = in * kReads + decltype(R)::value;
-        if constexpr (f < kFragments) read_fragment(Const<buf>{}, Const<slot / kGroup>{}, Const<f>{}, TAIL, first + t);
+        if constexpr (f < kFragments) read_fragment(Const<buf>{}, Const<slot / kGroup>{}, Const<f>{}, TAIL, t);
       });
-      if constexpr (slot < kPieces) {
-        if (t + 1 < steps) load_piece(1 - buf, first + t + 1, Const<slot>{});
-      }
+      for_each<(kPieces + kSlots - 1) / kSlots>([&](auto R) {
+        constexpr int i = slot * ((kPieces + kSlots - 1) / kSlots) + decltype(R)::value;
+        if constexpr (i < kPieces && ahead) {
+          load_piece(Const<(buf + 3) % kBuffers>{}, t + 3, Const<i>{});
+        }
+      });
       __builtin_amdgcn_sched_barrier(0);
     });
-    __builtin_amdgcn_s_waitcnt(0);
+    __builtin_amdgcn_s_waitcnt(ahead ? kLandedOne : 0);
     __syncthreads();
   };
-  static_assert(kPieces <= kSlots, "a direct load beside each of the first MFMAs");
-  for_each<kPieces>([&](auto I) { load_piece(0, first, I); });
-  __builtin_amdgcn_s_waitcnt(0);
+  for_each<kPieces>([&](auto I) { load_piece(Const<0>{}, 0, I); });
+  for_each<kPieces>([&](auto I) { load_piece(Const<1>{}, 1, I); });
+  for_each<kPieces>([&](auto I) { load_piece(Const<2>{}, 2, I); });
+  __builtin_amdgcn_s_waitcnt(kLandedOne);
   __syncthreads();
-  const int whole = p.K % BK == 0 || first + steps < all_steps ? steps : steps - 1;   // steps without a tail
+  // The last one to four steps, masked, stand behind the loop once, and the steps that are missing there add zeros: with
+  // bodies under conditions the accumulators were copied and spilled where their paths met.
   int t = 0;
-  for (; t + 2 <= whole; t += 2) {
-    step(Const<0>{}, Const<0>{}, t);
-    step(Const<1>{}, Const<0>{}, t + 1);
+  for (; t + 4 < steps; t += 4) {
+    step(Const<0>{}, Const<0>{}, Const<1>{}, t);
+    step(Const<1>{}, Const<0>{}, Const<1>{}, t + 1);
+    step(Const<2>{}, Const<0>{}, Const<1>{}, t + 2);
+    step(Const<3>{}, Const<0>{}, Const<1>{}, t + 3);
   }
-  if (t < whole) {
-    step(Const<0>{}, Const<0>{}, t);
-    ++t;
-    if (t < steps) step(Const<1>{}, Const<1>{}, t);
-  } else if (t < steps) {
-    step(Const<0>{}, Const<1>{}, t);
-  }
-  for_each<kGroup>([&](auto G) { mma(Const<3>{}, decltype(G)::value / NA, decltype(G)::value % NA); });
+  step(Const<0>{}, Const<1>{}, Const<1>{}, t);
+  step(Const<1>{}, Const<1>{}, Const<0>{}, t + 1);
+  step(Const<2>{}, Const<1>{}, Const<0>{}, t + 2);
+  step(Const<3>{}, Const<1>{}, Const<0>{}, t + 3);
+  for_each<kGroup>([&](auto G) { mma(Const<1>{}, decltype(G)::value / NA, decltype(G)::value % NA); });
 
   // Accumulator register c of a lane: channel 8 (c / 4) + 4 (lane / 32) + c % 4 of the fragment, token lane % 32.  Stored
   // from there a wave would write 8 bytes each into 32 rows.  The sums go through LDS instead (all of it is free: the last
@@ -262,7 +280,7 @@ __global__ __launch_bounds__(kThreads, 1) void tokens_tile_kernel(Product p, int
   constexpr int kChannels = 32 * NA, kPitch = 4 * kChannels + 16;     // bytes a token; the 16 keep rows off the same banks
   constexpr int V = sizeof(TY) == 2 ? 8 : 4;                          // channels of a 16-byte store
   constexpr int kAcross = kChannels / V, kDown = 64 / kAcross;        // lanes to a token, tokens to an instruction
-  static_assert(4 * 32 * kPitch <= 2 * kBuffer, "the sums of 32 tokens of four waves fit where the tiles were");
+  static_assert(4 * 32 * kPitch <= kBuffers * kBuffer, "the sums of 32 tokens of four waves fit where the tiles were");
   const uint32_t slab = lds0 + (uint32_t)(wave * 32 * kPitch);
   const int channel = o0 + wr * kChannels + lane % kAcross * V;
   const int valid = p.O - channel;
@@ -376,13 +394,13 @@ struct Plan { int edge, slices, steps_per_slice; };
 Plan plan_of(int64_t M, int64_t K, int64_t O) {
   if (M <= 64) return Plan{0, 1, 0};
   constexpr int64_t kCUs = 256;
-  const int64_t steps = (K + 127) / 128;
+  const int64_t steps = (K + 63) / 64;
   auto tiles = [&](int64_t edge) { return ((M + edge - 1) / edge) * ((O + edge - 1) / edge); };
   const int edge = tiles(256) >= kCUs ? 256 : tiles(128) >= kCUs ? 128 : 64;
   int64_t slices = 1;
   if (tiles(edge) < kCUs) {
     slices = kCUs / tiles(edge);
-    if (slices > steps / 4) slices = steps / 4;                        // four steps at least
+    if (slices > steps / 8) slices = steps / 8;                        // eight steps at least
     if (slices < 1) slices = 1;
   }
   const int64_t per = (steps + slices - 1) / slices;

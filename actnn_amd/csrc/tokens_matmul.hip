@@ -51,6 +51,13 @@ ACTNN_DEV void lds_store16(uint32_t address, u32x4 v) {
 }
 // what s_waitcnt takes to wait for LDS and for all but the last n loads
 constexpr int waitcnt_all_but(int n) { return (n & 15) | 7 << 4 | (n >> 4) << 14; }
+// 16 bytes a lane from a base that the wave shares, plus the lane's offset, to LDS: lane l's at lds + 16 l (asynchronous)
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+ACTNN_DEV void load_rows(const int8_t* base, uint32_t lane_bytes, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(lds), "v"(lane_bytes), "s"(base) : "memory", "m0");
+}
+#pragma clang diagnostic pop
 // between writes and reads of the same wave: LDS operations of a wave complete in order
 ACTNN_DEV void wave_lds_fence() {
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -80,6 +87,8 @@ struct Product {
   int M, K, O;
 };
 
+ACTNN_DEV float scaled(int sum, float xs, float ws, float bias) { return __builtin_fmaf((float)sum * xs, ws, bias); }
+
 // four consecutive channels of a token, from their integer sums
 template <typename TY> ACTNN_DEV void put4(const Product& p, int64_t token, int channel, const int (&sum)[4]) {
   if (token >= p.M) return;
@@ -89,8 +98,7 @@ template <typename TY> ACTNN_DEV void put4(const Product& p, int64_t token, int 
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int c = channel + i < p.O ? channel + i : p.O - 1;
-    v[i] = (float)sum[i] * xs * p.ws[c];
-    if (p.bias) v[i] += p.bias[c];
+    v[i] = scaled(sum[i], xs, p.ws[c], p.bias ? p.bias[c] : 0.0f);
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i)
@@ -106,19 +114,15 @@ template <> ACTNN_DEV void put4<int>(const Product& p, int64_t token, int channe
 
 // the integer sums of 16 bytes' worth of channels of a token, of which `valid` exist
 template <typename TY, int V>
-ACTNN_DEV void put_row(const Product& p, int64_t token, int channel, int valid, const int (&sum)[V], const float (&ws)[V],
-                       const float (&bias)[V]) {
-  TY* to = static_cast<TY*>(p.y) + token * p.O + channel;
+ACTNN_DEV void put_row(TY* to, int valid, const int (&sum)[V], float xs, const float (&ws)[V], const float (&bias)[V]) {
+  u32x4 out;
   if constexpr (std::is_same<TY, int>::value) {
-    store16_part<false>(reinterpret_cast<float*>(to), (u32x4){(uint32_t)sum[0], (uint32_t)sum[1], (uint32_t)sum[2], (uint32_t)sum[3]}, valid);
+    out = (u32x4){(uint32_t)sum[0], (uint32_t)sum[1], (uint32_t)sum[2], (uint32_t)sum[3]};
+    store16_part<false>(reinterpret_cast<float*>(to), out, valid);
   } else {
     float v[V];
-    const float xs = p.xs[token];
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      v[i] = (float)sum[i] * xs * ws[i];
-      if (p.bias) v[i] += bias[i];
-    }
+    for (int i = 0; i < V; ++i) v[i] = scaled(sum[i], xs, ws[i], bias[i]);
     store16_part<false>(to, narrow(static_cast<const TY*>(nullptr), v), valid);
   }
 }
@@ -126,7 +130,8 @@ ACTNN_DEV void put_row(const Product& p, int64_t token, int channel, int valid, 
 // ------------------------------------------------------------------------------------------
 // Tiles.  Four waves, two by two; a wave has NA x NE fragments of 32 channels x 32 tokens.
 // ------------------------------------------------------------------------------------------
-template <typename TY, int NA, int NE>
+// WHOLE: the features are whole steps.
+template <typename TY, int NA, int NE, bool WHOLE>
 __global__ __launch_bounds__(kThreads, 1) void tokens_tile_kernel(Product p, int slices, int steps_per_slice) {
   constexpr int BO = 64 * NA, BT = 64 * NE, BK = 64, kBuffers = 4;
   constexpr int kBuffer = (BO + BT) * BK;
@@ -160,6 +165,9 @@ __global__ __launch_bounds__(kThreads, 1) void tokens_tile_kernel(Product p, int
   const int chunks = (p.K + 15) / 16;
   const int features = (p.K < (first + steps) * BK ? p.K : (first + steps) * BK) - first * BK;     // of this block
 
+  const uint32_t lds0 = lds_address(smem);
+  const uint32_t lds_wave = __builtin_amdgcn_readfirstlane(lds0 + wave * 1024);
+
   // ---- direct loads: piece j is 16 rows of the weight's tile or, behind those, of the tokens'
   const int row_in = lane >> 2;
   const int chunk = (lane & 3) ^ ((lane >> 4) & 3);
@@ -182,13 +190,14 @@ __global__ __launch_bounds__(kThreads, 1) void tokens_tile_kernel(Product p, int
     constexpr int i = decltype(I)::value;
     const int step = first + (t < steps ? t : steps - 1);
     uint32_t at = off[i];
-    if (step * 4 + chunk >= chunks) at -= (uint32_t)chunk * 16u;       // past the row's end: the step's first chunk
+    if constexpr (!WHOLE) {
+      if (step * 4 + chunk >= chunks) at -= (uint32_t)chunk * 16u;     // past the row's end: the step's first chunk
+    }
     const int8_t* base = (i < NA ? wp : xp) + (int64_t)step * BK;
-    load_to_lds16_base(base, at, smem + decltype(BUF)::value * kBuffer + (wave + 4 * i) * 1024);
+    load_rows(base, at, lds_wave + decltype(BUF)::value * kBuffer + i * 4096);
   };
 
   // ---- fragments: lane -> row lane % 32, features 32 kb + 16 (lane / 32) ..
-  const uint32_t lds0 = lds_address(smem);
   const uint32_t in_row = (uint32_t)(lane & 31) * BK + (uint32_t)(((lane >> 5) ^ ((lane >> 2) & 3)) << 4);
   const uint32_t at_w = lds0 + (uint32_t)(wr * 32 * NA) * BK + in_row;
   const uint32_t at_x = lds0 + (uint32_t)(BO + wn * 32 * NE) * BK + in_row;
@@ -230,6 +239,13 @@ __global__ __launch_bounds__(kThreads, 1) void tokens_tile_kernel(Product p, int
   // fragments are in registers) and of the first of this one, the fragments of each k-block read beside the MFMAs of the
   // one before, and the direct loads of step t + 3 into the buffer whose last readers passed the barrier before.  The step
   // ends when the loads of step t + 1 have landed: those of two steps may be on their way.
+  // (a direct load and what it takes stand beside MFMAs without fragment reads where there are any, half of them in either
+  // group: about six instructions fit beside one)
+  constexpr bool kRoom = kGroup >= kFragments + kPieces;
+  constexpr auto load_slot = [](int i) {
+    return !kRoom ? i * (kSlots / kPieces) : i < kPieces / 2 ? kFragments + 2 * i : kGroup + kFragments + 2 * (i - kPieces / 2);
+  };
+  static_assert(load_slot(kPieces - 1) < kSlots, "every load has its place");
   constexpr int kLandedOne = waitcnt_all_but(2 * kPieces);
   // (no branches in a body: the compiler's own waits for LDS then stay exact)
   auto step = [&](auto BUF, auto TAIL, auto AHEAD, int t) {
@@ -242,11 +258,9 @@ __global__ __launch_bounds__(kThreads, 1) void tokens_tile_kernel(Product p, int
         constexpr int f = in * kReads + decltype(R)::value;
         if constexpr (f < kFragments) read_fragment(Const<buf>{}, Const<slot / kGroup>{}, Const<f>{}, TAIL, t);
       });
-      for_each<(kPieces + kSlots - 1) / kSlots>([&](auto R) {
-        constexpr int i = slot * ((kPieces + kSlots - 1) / kSlots) + decltype(R)::value;
-        if constexpr (i < kPieces && ahead) {
-          load_piece(Const<(buf + 3) % kBuffers>{}, t + 3, Const<i>{});
-        }
+      for_each<kPieces>([&](auto I) {
+        constexpr int i = decltype(I)::value;
+        if constexpr (ahead && slot == load_slot(i)) load_piece(Const<(buf + 3) % kBuffers>{}, t + 3, Const<i>{});
       });
       __builtin_amdgcn_sched_barrier(0);
     });
@@ -293,8 +307,13 @@ __global__ __launch_bounds__(kThreads, 1) void tokens_tile_kernel(Product p, int
       bias[i] = p.bias ? p.bias[c] : 0.0f;
     }
   }
+  TY* const out = static_cast<TY*>(p.y) + channel;
 #pragma unroll
   for (int e = 0; e < NE; ++e) {
+    const int first_token = t0 + wn * 32 * NE + 32 * e + lane / kAcross;
+    float xs[32 / kDown];
+#pragma unroll
+    for (int j = 0; j < 32 / kDown; ++j) xs[j] = p.xs[first_token + j * kDown < p.M ? first_token + j * kDown : p.M - 1];
 #pragma unroll
     for (int a = 0; a < NA; ++a)
 #pragma unroll
@@ -303,19 +322,17 @@ __global__ __launch_bounds__(kThreads, 1) void tokens_tile_kernel(Product p, int
                     (u32x4){(uint32_t)acc[e][a][4 * q], (uint32_t)acc[e][a][4 * q + 1], (uint32_t)acc[e][a][4 * q + 2],
                             (uint32_t)acc[e][a][4 * q + 3]});
     wave_lds_fence();
-    const int64_t first_token = t0 + wn * 32 * NE + 32 * e;
 #pragma unroll
     for (int j = 0; j < 32 / kDown; ++j) {
-      const int in = j * kDown + lane / kAcross;
-      const int64_t token = first_token + in;
-      const uint32_t at = slab + (uint32_t)(in * kPitch + lane % kAcross * V * 4);
+      const int64_t token = first_token + j * kDown;
+      const uint32_t at = slab + (uint32_t)((j * kDown + lane / kAcross) * kPitch + lane % kAcross * V * 4);
       int sum[V];
 #pragma unroll
       for (int i = 0; i < V; i += 4) {
         const u32x4 v = lds_load16(at + 4 * i);
         sum[i] = (int)v.x; sum[i + 1] = (int)v.y; sum[i + 2] = (int)v.z; sum[i + 3] = (int)v.w;
       }
-      if (token < p.M && valid > 0) put_row<TY>(p, token, channel, valid, sum, ws, bias);
+      put_row<TY>(out + token * p.O, token < p.M ? valid : 0, sum, xs[j], ws, bias);
     }
     wave_lds_fence();
   }
@@ -383,9 +400,7 @@ __global__ __launch_bounds__(kThreads) void tokens_sum_slices_kernel(Product p, 
     for (int s = 0; s < slices; ++s) sum += part[s * n + i];
     const int64_t token = i / p.O;
     const int channel = (int)(i - token * p.O);
-    float v = (float)sum * p.xs[token] * p.ws[channel];
-    if (p.bias) v += p.bias[channel];
-    Conv<TY>::store(static_cast<TY*>(p.y), i, v);
+    Conv<TY>::store(static_cast<TY*>(p.y), i, scaled(sum, p.xs[token], p.ws[channel], p.bias ? p.bias[channel] : 0.0f));
   }
 }
 
@@ -408,7 +423,9 @@ Plan plan_of(int64_t M, int64_t K, int64_t O) {
 }
 
 template <typename TY, int N> void launch_tiles(const Product& p, const Plan& plan, int64_t blocks, hipStream_t s) {
-  tokens_tile_kernel<TY, N, N><<<dim3((unsigned)blocks), dim3(kThreads), 0, s>>>(p, plan.slices, plan.steps_per_slice);
+  const dim3 grid((unsigned)blocks), blk(kThreads);
+  if (p.K % 64 == 0) tokens_tile_kernel<TY, N, N, true><<<grid, blk, 0, s>>>(p, plan.slices, plan.steps_per_slice);
+  else tokens_tile_kernel<TY, N, N, false><<<grid, blk, 0, s>>>(p, plan.slices, plan.steps_per_slice);
 }
 template <typename TY> void launch_edge(const Product& p, const Plan& plan, int64_t blocks, hipStream_t s) {
   if (plan.edge == 256) launch_tiles<TY, 4>(p, plan, blocks, s);

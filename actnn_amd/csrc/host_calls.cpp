@@ -761,26 +761,39 @@ PyObject* linear_tokens_grad_weight(PyObject* const* a, Py_ssize_t n) {
               "grad_output ", grad.sizes(), " and codes ", codes.sizes(), " are not of the same tokens");
   const c10::DeviceGuard guard(grad.device());
   const Tensor scale = row_scales(given, x.M, codes, "scale");
-  const int64_t O = grad.size(-1);
-  const Tensor out = empty({O, x.K}, grad, dtype);
-  if (O == 0) return wrap(out);
-  if (x.M == 0) return wrap(out.zero_());
+  const int64_t outputs = grad.size(-1);
+  int64_t O = outputs;
+  if (O == 0 || x.M == 0) {
+    const Tensor out = empty({O, x.K}, grad, dtype);
+    return wrap(out.zero_());
+  }
   Tensor rows = grad.detach().reshape({x.M, O});
   if (O > 1 && rows.stride(1) != 1) rows = rows.contiguous();
   int64_t ld = x.M > 1 ? rows.stride(0) : O;
-  if ((x.M - 1) * ld + O < 8) {                          // the kernel reads 16 bytes at least
-    const Tensor room = at::zeros({x.M, 8}, rows.options());
-    room.narrow(1, 0, O).copy_(rows);
+  auto pad = [&](int64_t width) {                        // rows of `width`, zeros behind the outputs
+    const Tensor room = empty({x.M, width}, grad, type);
+    room.narrow(1, 0, outputs).copy_(rows);
+    if (width > outputs) room.narrow(1, outputs, width - outputs).zero_();
     rows = room;
-    ld = 8;
+    ld = width;
+  };
+  if (actnn_tokens_grad_weight_wants_chunks(x.M, O, x.K)) {
+    // (two passes over the gradient, where the product would take twice as long; the outputs added are cut off below)
+    if (O % 8 != 0 || ld % 8 != 0 || reinterpret_cast<uintptr_t>(rows.data_ptr()) % 16 != 0) {
+      pad((O + 7) / 8 * 8);
+      O = ld;
+    }
+  } else if ((x.M - 1) * ld + O < 8) {                   // the kernel reads 16 bytes at least
+    pad(8);
   }
+  const Tensor out = empty({O, x.K}, grad, dtype);
   const int64_t bytes = actnn_tokens_grad_weight_workspace_bytes(x.M, O, x.K);
   const Tensor workspace = bytes > 0 ? empty({bytes}, grad, at::kByte) : Tensor();
   launch("linear_tokens_grad_weight", [&] {
     return actnn_tokens_grad_weight(ptr(rows), ld, x.data(), x.ld, f32(scale), ptr(out), x.M, O, x.K, code_of(type),
                                     code_of(dtype), ptr(workspace), bytes, stream_of(grad));
   });
-  return wrap(out);
+  return wrap(O == outputs ? out : out.narrow(0, 0, outputs));
 }
 
 // ---------------------------------------------------------------------------- group norm

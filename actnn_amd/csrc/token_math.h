@@ -47,11 +47,8 @@ ACTNN_DEV uint32_t pack_codes(int a, int b, int c, int d) {
   return __builtin_amdgcn_perm((uint32_t)b, (uint32_t)a, 0x0c0c0400u) |
          __builtin_amdgcn_perm((uint32_t)d, (uint32_t)c, 0x04000c0cu);
 }
-// byte I of a word of codes, as a number (the codes' offset form - sign bits flipped - converts in one instruction)
-ACTNN_DEV uint32_t offset_codes(uint32_t w) { return w ^ 0x80808080u; }
-template <int I> ACTNN_DEV float code_value(uint32_t offset_word) {
-  return (float)((offset_word >> (8 * I)) & 0xffu) - 128.0f;
-}
+// byte I of a word of codes, as a number (one instruction)
+template <int I> ACTNN_DEV float code_value(uint32_t word) { return (float)(int8_t)(word >> (8 * I)); }
 
 // Largest magnitudes as the values' bits without the sign: as whole numbers they order like the magnitudes, with
 // infinity and then NaN on top, and 16-bit types go two at a time.
@@ -129,13 +126,29 @@ template <typename T> ACTNN_DEV typename CodeWords<T>::type codes_of(const Coder
 }
 // and back: the codes as numbers
 ACTNN_DEV void code_values(uint32_t w, float (&f)[4]) {
-  w = offset_codes(w);
   f[0] = code_value<0>(w); f[1] = code_value<1>(w); f[2] = code_value<2>(w); f[3] = code_value<3>(w);
 }
 ACTNN_DEV void code_values(u32x2 v, float (&f)[8]) {
-  const uint32_t a = offset_codes(v.x), b = offset_codes(v.y);
+  const uint32_t a = v.x, b = v.y;
   f[0] = code_value<0>(a); f[1] = code_value<1>(a); f[2] = code_value<2>(a); f[3] = code_value<3>(a);
   f[4] = code_value<0>(b); f[5] = code_value<1>(b); f[6] = code_value<2>(b); f[7] = code_value<3>(b);
 }
+
+// Codes 2 J and 2 J + 1 of a word times a scale, in 16 bits: one rounding for fp16 (the codes are made halves by putting them
+// behind the exponent of 1024, and a mixed multiply-add rounds their product with the fp32 scale), two for bf16 (to 32 bits
+// first).  Two and two and a half instructions a value.
+template <typename T, int J> ACTNN_DEV uint32_t code_pair(uint32_t word, float scale);
+template <> ACTNN_DEV uint32_t code_pair<bf16_t, 0>(uint32_t w, float s) { return pack_bf16x2(code_value<0>(w) * s, code_value<1>(w) * s); }
+template <> ACTNN_DEV uint32_t code_pair<bf16_t, 1>(uint32_t w, float s) { return pack_bf16x2(code_value<2>(w) * s, code_value<3>(w) * s); }
+typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+template <int J> ACTNN_DEV uint32_t half_code_pair(uint32_t w, float s) {
+  const f16x2_t off = {(_Float16)-1152.0f, (_Float16)-1152.0f};
+  const uint32_t raised = __builtin_amdgcn_perm(w ^ 0x80808080u, 0x64646464u, J == 0 ? 0x00050004u : 0x00070006u);
+  const f16x2_t q = __builtin_bit_cast(f16x2_t, raised) + off;
+  const f16x2_t v = {(_Float16)__builtin_fmaf((float)q.x, s, 0.0f), (_Float16)__builtin_fmaf((float)q.y, s, 0.0f)};
+  return __builtin_bit_cast(uint32_t, v);
+}
+template <> ACTNN_DEV uint32_t code_pair<__half, 0>(uint32_t w, float s) { return half_code_pair<0>(w, s); }
+template <> ACTNN_DEV uint32_t code_pair<__half, 1>(uint32_t w, float s) { return half_code_pair<1>(w, s); }
 
 }  // namespace actnn

@@ -44,6 +44,12 @@ ACTNN_DEV u32x2 read_transposed(uint32_t at) {
   return __builtin_bit_cast(u32x2, v);
 }
 
+// eight codes of a token as values
+template <typename T> ACTNN_DEV u32x4 values_of(u32x2 codes, float scale) {
+  const uint32_t a = codes.x, b = codes.y;
+  return (u32x4){code_pair<T, 0>(a, scale), code_pair<T, 1>(a, scale), code_pair<T, 0>(b, scale), code_pair<T, 1>(b, scale)};
+}
+
 struct Grad {
   const void* g;                         // [M, O], rows `ldg` elements apart
   const int8_t* x;                       // [M, I], rows `ldx` bytes apart
@@ -92,12 +98,7 @@ __global__ __launch_bounds__(kThreads, 2) void tokens_grad_kernel(Grad p, int sp
       const int row = row0 + 16 * j;
       const int at = row * kRow + ((ch ^ ((row & 3) << 2)) << 4);
       *reinterpret_cast<u32x4*>(tg + at) = row_vector_ends<T>(rg[j]);
-      float f[8];
-      code_values(rx[j], f);
-      const bool valid = m + row < m1;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) f[e] = valid ? f[e] * rs[j] : 0.0f;
-      *reinterpret_cast<u32x4*>(tg + kTile + at) = words_of8(static_cast<const T*>(nullptr), f);
+      *reinterpret_cast<u32x4*>(tg + kTile + at) = values_of<T>(rx[j], m + row < m1 ? rs[j] : 0.0f);
     }
   };
 
@@ -171,6 +172,276 @@ __global__ __launch_bounds__(kThreads, 2) void tokens_grad_kernel(Grad p, int sp
   }
 }
 
+// ------------------------------------------------------------------------------------------
+// Large products: 256 outputs x 256 features a block, four waves of 128 x 128, 32 tokens a step.
+//
+// grad_out's rows go straight into LDS (global_load_lds; rows of whole 16-byte chunks), four buffers, loads three steps ahead.
+// The codes go into LDS as they are too, four steps ahead, each wave those of its eight tokens of a step with their scales; one
+// step ahead the wave turns them into values in the tile that the transposing reads take (two buffers).  So every load is one
+// whose arrival the kernel counts itself, and the step only waits for those of two steps before.  A row of a tile is 512 bytes, its
+// 32 chunks at chunk ^ 4 (row % 8).  Everything but the MFMAs stands beside one of them, about six instructions at most: fragment
+// reads and loads in the first eight of a group of sixteen, the values two at a time in the other eight.
+//
+// The first tokens, up to a multiple of 128, go through registers, masked: behind the last token there is nothing that may be
+// multiplied, an infinite gradient times a zero would be a NaN.
+// ------------------------------------------------------------------------------------------
+template <int N> struct Const { static constexpr int value = N; };
+template <int N, typename F> ACTNN_DEV void for_each(F&& f) {
+  if constexpr (N > 0) {
+    for_each<N - 1>(f);
+    f(Const<N - 1>{});
+  }
+}
+template <typename V> ACTNN_DEV V lds_load(uint32_t address) {
+  return *reinterpret_cast<const __attribute__((address_space(3))) V*>((lds_ptr_t)(uintptr_t)address);
+}
+template <typename V> ACTNN_DEV void lds_store(uint32_t address, V v) {
+  *reinterpret_cast<__attribute__((address_space(3))) V*>((lds_ptr_t)(uintptr_t)address) = v;
+}
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+// 16 (4) bytes a lane from a base that the wave shares, plus the lane's offset, to LDS: lane l's at lds + 16 l (4 l); asynchronous
+ACTNN_DEV void load_rows(const void* base, uint32_t lane_bytes, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(lds), "v"(lane_bytes), "s"(base) : "memory", "m0");
+}
+ACTNN_DEV void load_words(const void* base, uint32_t lane_bytes, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" : : "s"(lds), "v"(lane_bytes), "s"(base) : "memory", "m0");
+}
+#pragma clang diagnostic pop
+constexpr int waitcnt_all_but(int n) { return (n & 15) | 7 << 4 | (n >> 4) << 14; }     // (and for LDS)
+ACTNN_DEV void wave_lds_fence() {                       // between writes and reads of the same wave
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+template <typename T, typename TY>
+__global__ __launch_bounds__(kThreads, 1) void tokens_grad_large_kernel(Grad p, int splits, int tokens_per_split) {
+  constexpr int BO = 256, BI = 256, BK = 32, kRow = 512, kTile = BK * kRow, NA = 4, NE = 4;
+  constexpr int kRawWave = 8 * 256 + 256, kRaw = 4 * kRawWave;        // codes and scales of a step
+  constexpr int kX = 4 * kTile, kCodes = kX + 2 * kTile;              // where they begin
+  constexpr int kGroup = NA * NE, kSlots = 2 * kGroup;
+  constexpr int kLoads = 4 + 2 + 1;                                   // of a wave and step
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[kCodes + 4 * kRaw];
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wr = wave & 1, wn = wave >> 1;
+  const int tiles_i = (p.I + BI - 1) / BI, tiles_o = (p.O + BO - 1) / BO, tiles = tiles_o * tiles_i;
+  const int split = splits > 1 ? blockIdx.x / tiles : 0;
+  const int tile = splits > 1 ? blockIdx.x % tiles : blockIdx.x;
+  int tile_o = tile / tiles_i, tile_i = tile % tiles_i;
+  if (splits == 1 && tiles_o % 8 == 0) {
+    // each XCD gets panels of outputs of its own, and takes them by 8 tiles of features
+    const int xcd = blockIdx.x & 7, i = blockIdx.x >> 3, panels = tiles_o / 8;
+    const int strip = i / (panels * 8), in = i - strip * panels * 8;
+    const int wide = tiles_i - strip * 8 < 8 ? tiles_i - strip * 8 : 8;
+    tile_o = xcd * panels + in / wide;
+    tile_i = strip * 8 + in % wide;
+  }
+  const int o0 = tile_o * BO, i0 = tile_i * BI;
+  const int m_first = split * tokens_per_split;
+  const int count = p.M - m_first < tokens_per_split ? p.M - m_first : tokens_per_split;
+  const int masked = count % (4 * BK), steps = count / BK - masked / BK;     // steps: a multiple of four
+  const T* g = static_cast<const T*>(p.g) + o0;
+  const int8_t* x = p.x + i0;
+  const uint32_t lds0 = lds_address(smem);
+
+  // ---- fragments: lane -> column n0 + lane % 32, tokens 16 kb + 8 (lane / 32) ..
+  const int blk = lane >> 4, r = lane & 15;
+  const int f_row = 8 * (blk >> 1) + (r >> 2);
+  auto fragment_at = [&](int n0) {
+    const int ch = n0 / 8 + 2 * (blk & 1) + ((r & 3) >> 1);
+    return (uint32_t)(f_row * kRow + ((ch ^ ((f_row & 7) << 2)) << 4) + (r & 1) * 8);
+  };
+  // (the second read of a fragment, four rows on, lies in the other half of the row)
+  uint32_t ag[NA], ax[NE], ag2[NA], ax2[NE];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    ag[i] = lds0 + fragment_at(wr * 128 + 32 * i);
+    ax[i] = lds0 + kX + fragment_at(wn * 128 + 32 * i);
+    ag2[i] = ag[i] ^ 256u;
+    ax2[i] = ax[i] ^ 256u;
+  }
+  f32x16 acc[NE][NA];
+#pragma unroll
+  for (int e = 0; e < NE; ++e)
+#pragma unroll
+    for (int a = 0; a < NA; ++a)
+#pragma unroll
+      for (int c = 0; c < 16; ++c) acc[e][a][c] = 0.0f;
+  u32x4 fg[2][NA], fx[2][NE];
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) fg[h][i] = fx[h][i] = (u32x4){0u, 0u, 0u, 0u};
+  auto read_fragment = [&](auto BUF, auto KB, auto F) {
+    constexpr int buf = decltype(BUF)::value, kb = decltype(KB)::value, f = decltype(F)::value;
+    constexpr bool is_g = f < NA;
+    constexpr uint32_t at = (is_g ? buf : buf & 1) * kTile + kb * 16 * kRow;
+    const u32x2 lo = read_transposed((is_g ? ag[f % 4] : ax[f % 4]) + at), hi = read_transposed((is_g ? ag2[f % 4] : ax2[f % 4]) + at + 4 * kRow);
+    const u32x4 v = {lo.x, lo.y, hi.x, hi.y};
+    if constexpr (is_g) fg[kb][f] = v;
+    else fx[kb][f - NA] = v;
+  };
+  auto mma = [&](auto KB, int e, int a) {
+    constexpr int h = decltype(KB)::value;
+    acc[e][a] = mma16<T>(fx[h][e], fg[h][a], acc[e][a]);
+  };
+
+  // ---- the first tokens, through registers: thread -> chunk tid % 32 of rows tid / 32 + 8 j
+  for (int m = 0; m < masked; m += BK) {
+    const int ch = tid & 31;
+    const bool in_g = o0 + ch * 8 < p.O, in_x = i0 + ch * 8 < p.I;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int row = (tid >> 5) + 8 * j;
+      const bool valid = m + row < masked;
+      const int64_t at = m_first + (valid ? m + row : 0);
+      const u32x4 none = {0u, 0u, 0u, 0u};
+      const u32x4 v = valid && in_g ? load16(g + at * p.ldg + ch * 8) : none;
+      const u32x2 q = *reinterpret_cast<const u32x2*>(x + at * p.ldx + (in_x ? ch * 8 : 0));
+      const uint32_t to = lds0 + (uint32_t)(row * kRow + ((ch ^ ((row & 7) << 2)) << 4));
+      lds_store(to, v);
+      lds_store(to + kX, values_of<T>(q, valid ? p.scale[at] : 0.0f));
+    }
+    __syncthreads();
+    for_each<2>([&](auto KB) {
+      for_each<NA + NE>([&](auto F) { read_fragment(Const<0>{}, KB, F); });
+      for_each<kGroup>([&](auto G) { mma(KB, decltype(G)::value / NA, decltype(G)::value % NA); });
+    });
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) fg[1][i] = fx[1][i] = (u32x4){0u, 0u, 0u, 0u};     // (multiplied once more at the start)
+
+  if (steps > 0) {
+    __syncthreads();
+    const int m0 = m_first + masked;
+    // ---- direct loads.  grad_out: one instruction is rows 2 rp and 2 rp + 1, rp = wave + 4 jj, LDS chunk lane % 32
+    const int g_row = lane >> 5;
+    const int g_chunk = (lane & 31) ^ (((2 * wave + g_row) & 7) << 2);
+    const uint32_t g_lane = (uint32_t)g_row * (uint32_t)p.ldg * 2u + (o0 + g_chunk * 8 < p.O ? (uint32_t)g_chunk * 16u : 0u);
+    const char* g_wave = reinterpret_cast<const char*>(g + (int64_t)(m0 + 2 * wave) * p.ldg);
+    const int64_t g_step = (int64_t)BK * p.ldg * 2, g_piece = (int64_t)8 * p.ldg * 2;
+    // codes: one instruction is four of the wave's eight tokens, 16 bytes a lane; scales: the even tokens' and the odd ones'
+    const int c_row = lane >> 4;
+    const uint32_t c_lane = (uint32_t)c_row * (uint32_t)p.ldx + (i0 + (lane & 15) * 16 < p.I ? (uint32_t)(lane & 15) * 16u : 0u);
+    const int8_t* c_wave = x + (int64_t)(m0 + 8 * wave) * p.ldx;
+    const int64_t c_step = (int64_t)BK * p.ldx, c_piece = (int64_t)4 * p.ldx;
+    const uint32_t s_lane = (uint32_t)((lane & 3) * 2 + ((lane >> 2) & 1)) * 4u;
+    const float* s_wave = p.scale + m0 + 8 * wave;
+    const uint32_t lds_g = __builtin_amdgcn_readfirstlane(lds0 + wave * 1024);
+    const uint32_t lds_c = __builtin_amdgcn_readfirstlane(lds0 + kCodes + wave * kRawWave);
+    // (steps past the last load that one again: nobody reads it)
+    auto load_g = [&](auto BUF, int t, auto J) {
+      const int64_t at = t < steps ? t : steps - 1;
+      load_rows(g_wave + at * g_step + decltype(J)::value * g_piece, g_lane, lds_g + decltype(BUF)::value * kTile + decltype(J)::value * 4096);
+    };
+    auto load_codes = [&](auto BUF, int t, auto J) {
+      constexpr int j = decltype(J)::value;
+      const int64_t at = t < steps ? t : steps - 1;
+      const uint32_t to = lds_c + decltype(BUF)::value * kRaw;
+      if constexpr (j < 2) load_rows(c_wave + at * c_step + j * c_piece, c_lane, to + j * 1024);
+      else load_words(s_wave + at * BK, s_lane, to + 2048);
+    };
+    auto load_piece = [&](auto BUF, int t, auto I) {      // buffer of step t, which loads grad_out of t + 3 and codes of t + 4
+      constexpr int i = decltype(I)::value, buf = decltype(BUF)::value;
+      if constexpr (i < 4) load_g(Const<(buf + 3) % 4>{}, t + 3, Const<i>{});
+      else load_codes(Const<buf>{}, t + 4, Const<i - 4>{});
+    };
+
+    // ---- codes to values: lane -> eight codes (lane % 32) of tokens 2 i + lane / 32 of the wave's
+    const int v_row = lane >> 5;
+    const uint32_t raw_at = lds0 + kCodes + wave * kRawWave + lane * 8;
+    const uint32_t scale_at = lds0 + kCodes + wave * kRawWave + 2048 + v_row * 16;
+    const uint32_t value_at = lds0 + kX + (uint32_t)((8 * wave + v_row) * kRow + (((lane & 31) ^ (v_row << 2)) << 4));
+    u32x2 raw[4];
+    u32x4 scales;
+    uint32_t made[4];
+    auto read_raw = [&](auto BUF, auto I) {
+      constexpr int i = decltype(I)::value;
+      if constexpr (i < 4) raw[i] = lds_load<u32x2>(raw_at + decltype(BUF)::value * kRaw + i * 512);
+      else scales = lds_load<u32x4>(scale_at + decltype(BUF)::value * kRaw);
+    };
+    auto make_values = [&](auto BUF, auto I) {            // two of the lane's 32 codes; every fourth call stores 16 bytes
+      constexpr int i = decltype(I)::value / 4, w = decltype(I)::value % 4;
+      const u32x4 all = scales;
+      const uint32_t sc = i == 0 ? all.x : i == 1 ? all.y : i == 2 ? all.z : all.w;
+      const u32x2 two = raw[i];
+      const uint32_t word = w < 2 ? two.x : two.y;
+      made[w] = code_pair<T, w % 2>(word, as_float(sc));
+      if constexpr (w == 3)
+        lds_store((value_at ^ (i << 7)) + decltype(BUF)::value * kTile + i * 1024, (u32x4){made[0], made[1], made[2], made[3]});
+    };
+
+    auto step = [&](auto BUF, int t) {
+      constexpr int buf = decltype(BUF)::value;
+      for_each<kSlots>([&](auto S) {
+        constexpr int slot = decltype(S)::value, in = slot % kGroup;
+        mma(Const<1 - slot / kGroup>{}, in / NA, in % NA);
+        if constexpr (in < NA + NE) {
+          read_fragment(Const<buf>{}, Const<slot / kGroup>{}, Const<in>{});
+          if constexpr (slot < 5) read_raw(Const<(buf + 1) % 4>{}, Const<slot>{});
+          if constexpr (slot >= kGroup && in < kLoads) load_piece(Const<buf>{}, t, Const<in>{});
+        } else {
+          make_values(Const<(buf + 1) % 2>{}, Const<(slot / kGroup) * 8 + in - 8>{});
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      });
+      __builtin_amdgcn_s_waitcnt(waitcnt_all_but(2 * kLoads));
+      __syncthreads();
+    };
+    for_each<4>([&](auto B) { for_each<3>([&](auto J) { load_codes(B, decltype(B)::value, J); }); });
+    for_each<3>([&](auto B) { for_each<4>([&](auto J) { load_g(B, decltype(B)::value, J); }); });
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    for_each<5>([&](auto I) { read_raw(Const<0>{}, I); });
+    for_each<16>([&](auto I) { make_values(Const<0>{}, I); });
+    __syncthreads();
+    for (int t = 0; t < steps; t += 4) {
+      step(Const<0>{}, t);
+      step(Const<1>{}, t + 1);
+      step(Const<2>{}, t + 2);
+      step(Const<3>{}, t + 3);
+    }
+    for_each<kGroup>([&](auto G) { mma(Const<1>{}, decltype(G)::value / NA, decltype(G)::value % NA); });
+  }
+  __builtin_amdgcn_s_waitcnt(0);                         // (the last steps' loads write into LDS still)
+  __syncthreads();
+
+  // accumulator register c of a lane: feature 8 (c / 4) + 4 (lane / 32) + c % 4 of the fragment, output lane % 32: through
+  // LDS, 32 outputs of the wave's 128 features at a time, so that whole lines are stored
+  constexpr int kPitch = 4 * 128 + 16, V = 16 / sizeof(TY), kAcross = 128 / V, kDown = 64 / kAcross;
+  static_assert(4 * 32 * kPitch <= kCodes, "the sums of 32 outputs of four waves fit");
+  const uint32_t slab = lds0 + (uint32_t)(wave * 32 * kPitch);
+  const int feature = i0 + wn * 128 + lane % kAcross * V;
+  TY* const out = static_cast<TY*>(p.out) + (int64_t)split * p.O * p.I + feature;
+#pragma unroll
+  for (int a = 0; a < NA; ++a) {
+#pragma unroll
+    for (int e = 0; e < NE; ++e)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        lds_store(slab + (uint32_t)((lane & 31) * kPitch + 4 * (32 * e + 8 * q + 4 * (lane >> 5))),
+                  (u32x4){as_uint(acc[e][a][4 * q]), as_uint(acc[e][a][4 * q + 1]), as_uint(acc[e][a][4 * q + 2]), as_uint(acc[e][a][4 * q + 3])});
+    wave_lds_fence();
+#pragma unroll
+    for (int j = 0; j < 32 / kDown; ++j) {
+      const int o = o0 + wr * 128 + 32 * a + j * kDown + lane / kAcross;
+      const uint32_t at = slab + (uint32_t)((j * kDown + lane / kAcross) * kPitch + lane % kAcross * V * 4);
+      float v[V];
+#pragma unroll
+      for (int i = 0; i < V; i += 4) {
+        const u32x4 w = lds_load<u32x4>(at + 4 * i);
+        v[i] = as_float(w.x); v[i + 1] = as_float(w.y); v[i + 2] = as_float(w.z); v[i + 3] = as_float(w.w);
+      }
+      store16_part<false>(out + (int64_t)o * p.I, narrow(static_cast<const TY*>(nullptr), v), o < p.O ? p.I - feature : 0);
+    }
+    wave_lds_fence();
+  }
+}
+
 template <typename TY>
 __global__ __launch_bounds__(kThreads) void tokens_grad_sum_kernel(const float* __restrict__ part, TY* __restrict__ out,
                                                                    int64_t n, int splits) {
@@ -181,33 +452,42 @@ __global__ __launch_bounds__(kThreads) void tokens_grad_sum_kernel(const float* 
   Conv<TY>::store(out, i, v);
 }
 
-// Blocks that share the tokens of a tile: enough to fill the chip twice, with four steps each at least.
-struct Plan { int splits, tokens; };
-Plan plan_of(int64_t M, int64_t O, int64_t I) {
-  const int64_t tiles = ((O + 127) / 128) * ((I + 127) / 128), steps = (M + 63) / 64;
-  int64_t splits = tiles >= 256 ? 1 : 512 / tiles;
-  if (splits > steps / 4) splits = steps / 4;
-  if (splits < 1) splits = 1;
-  const int64_t per = (steps + splits - 1) / splits;
-  return Plan{(int)((steps + per - 1) / per), (int)(per * 64)};
+// Which kernel, and how many blocks share the tokens of a tile (`tokens` each).
+struct Plan { int edge, splits, tokens; };
+Plan plan_of(int64_t M, int64_t O, int64_t I, bool aligned) {
+  auto tiles = [&](int64_t edge) { return ((O + edge - 1) / edge) * ((I + edge - 1) / edge); };
+  auto cut = [&](int edge, int64_t unit, int64_t blocks, int64_t least) {   // about `blocks` of them, `least` units of tokens each
+    const int64_t units = (M + unit - 1) / unit;
+    int64_t splits = tiles(edge) >= blocks ? 1 : blocks / tiles(edge);
+    if (splits > units / least) splits = units / least;
+    if (splits < 1) splits = 1;
+    const int64_t per = (units + splits - 1) / splits;
+    return Plan{edge, (int)((units + per - 1) / per), (int)(per * unit)};
+  };
+  if (aligned && M >= 2048 && tiles(256) >= 64) return cut(256, 128, 256, 8);
+  return cut(128, 64, 512, 4);
 }
 
 template <typename T, typename TY>
-int launch_grad(Grad p, void* workspace, int64_t workspace_bytes, hipStream_t s) {
-  Plan plan = plan_of(p.M, p.O, p.I);
+int launch_grad(Grad p, bool aligned, void* workspace, int64_t workspace_bytes, hipStream_t s) {
+  Plan plan = plan_of(p.M, p.O, p.I, aligned);
   const int64_t n = (int64_t)p.O * p.I;
-  const int64_t whole = ((int64_t)p.M + 63) / 64 * 64;
-  if (plan.splits > 1 && (!workspace || workspace_bytes < 4 * n * plan.splits)) plan = Plan{1, (int)whole};
-  const int64_t blocks = ((p.O + 127LL) / 128) * ((p.I + 127LL) / 128) * plan.splits;
+  if (plan.splits > 1 && (!workspace || workspace_bytes < 4 * n * plan.splits)) plan = Plan{plan.edge, 1, p.M};
+  const int64_t edge = plan.edge, blocks = ((p.O + edge - 1) / edge) * ((p.I + edge - 1) / edge) * plan.splits;
   if (blocks > 0x7fffffffLL || (n + kThreads - 1) / kThreads > 0x7fffffffLL) return ACTNN_EINVAL;
   const dim3 grid((unsigned)blocks), blk(kThreads);
+  auto go = [&](auto* to) {
+    using TO = std::remove_pointer_t<decltype(to)>;
+    p.out = to;
+    if (edge == 256) tokens_grad_large_kernel<T, TO><<<grid, blk, 0, s>>>(p, plan.splits, plan.tokens);
+    else tokens_grad_kernel<T, TO><<<grid, blk, 0, s>>>(p, plan.splits, plan.tokens);
+  };
+  TY* out = static_cast<TY*>(p.out);
   if (plan.splits == 1) {
-    tokens_grad_kernel<T, TY><<<grid, blk, 0, s>>>(p, 1, plan.tokens);
+    go(out);
   } else {
     if (!aligned16(workspace)) return ACTNN_EALIGN;
-    TY* out = static_cast<TY*>(p.out);
-    p.out = workspace;
-    tokens_grad_kernel<T, float><<<grid, blk, 0, s>>>(p, plan.splits, plan.tokens);
+    go(static_cast<float*>(workspace));
     tokens_grad_sum_kernel<TY><<<dim3((unsigned)((n + kThreads - 1) / kThreads)), blk, 0, s>>>(
         static_cast<const float*>(workspace), out, n, plan.splits);
   }
@@ -215,8 +495,10 @@ int launch_grad(Grad p, void* workspace, int64_t workspace_bytes, hipStream_t s)
 }
 template <typename T>
 int launch_out(const Grad& p, int out_dtype, void* workspace, int64_t workspace_bytes, hipStream_t s) {
-  if (out_dtype == ACTNN_F32) return launch_grad<T, float>(p, workspace, workspace_bytes, s);
-  return launch_grad<T, T>(p, workspace, workspace_bytes, s);
+  // (offsets of rows inside a wave's load are 32-bit)
+  const bool aligned = aligned16(p.g) && p.ldg % 8 == 0 && p.O % 8 == 0 && p.ldg < (1 << 24) && p.ldx < (1 << 24);
+  if (out_dtype == ACTNN_F32) return launch_grad<T, float>(p, aligned, workspace, workspace_bytes, s);
+  return launch_grad<T, T>(p, aligned, workspace, workspace_bytes, s);
 }
 
 }  // namespace
@@ -225,8 +507,18 @@ int launch_out(const Grad& p, int out_dtype, void* workspace, int64_t workspace_
 extern "C" int64_t actnn_tokens_grad_weight_workspace_bytes(int64_t M, int64_t O, int64_t I) {
   using namespace actnn;
   if (M < 1 || O < 1 || I < 1 || M > 0x7fffff00LL || O > 0x7fffff00LL || I > 0x7fffff00LL) return 0;
-  const Plan plan = plan_of(M, O, I);
-  return plan.splits > 1 ? 4 * O * I * plan.splits : 0;
+  int64_t most = 0;
+  for (const bool aligned : {false, true}) {
+    const Plan plan = plan_of(M, O, I, aligned);
+    if (plan.splits > 1 && 4 * O * I * plan.splits > most) most = 4 * O * I * plan.splits;
+  }
+  return most;
+}
+
+extern "C" int actnn_tokens_grad_weight_wants_chunks(int64_t M, int64_t O, int64_t I) {
+  using namespace actnn;
+  if (M < 1 || O < 1 || I < 1 || M > 0x7fffff00LL || O > 0x7fffff00LL || I > 0x7fffff00LL) return 0;
+  return plan_of(M, O, I, true).edge == 256;
 }
 
 extern "C" int actnn_tokens_grad_weight(const void* grad_out, int64_t ldg, const int8_t* codes, int64_t ldc, const float* scale,

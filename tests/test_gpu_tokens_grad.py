@@ -1,5 +1,6 @@
 """The weight gradient from 8-bit tokens against the same sum in 64 bits over the values the kernel multiplies: the codes'
 values rounded to the gradient's type, so that what is left is the fp32 sum and the output's rounding."""
+import numpy as np
 import pytest
 import torch
 
@@ -18,8 +19,16 @@ def make(M, O, I, dtype, seed):
     return (g, *tokens.quantize_tokens(x))
 
 
+def kept_values(codes, scale, dtype):
+    """What the kernel multiplies: fp16 rounded once (numpy's conversion), bf16 by way of 32 bits."""
+    if dtype == torch.float16:
+        exact = codes.double() * scale.double()[..., None]
+        return torch.from_numpy(exact.cpu().numpy().astype(np.float16)).to(codes.device).double()
+    return (codes.float() * scale[..., None]).to(dtype).double()
+
+
 def check(gw, g, codes, scale, out):
-    values = (codes.float() * scale[..., None]).to(g.dtype).double().reshape(-1, codes.shape[-1])
+    values = kept_values(codes, scale, g.dtype).reshape(-1, codes.shape[-1])
     gd = g.double().reshape(-1, g.shape[-1])
     exact = gd.t() @ values
     size = gd.abs().t() @ values.abs()
@@ -35,7 +44,8 @@ def check(gw, g, codes, scale, out):
 
 
 SHAPES = [(1, 8, 16), (1, 1, 1), (2, 3, 5), (3, 7, 33), (63, 64, 128), (64, 128, 128), (65, 129, 130), (100, 100, 784), (1000, 100, 784),
-          (257, 1, 300), (300, 260, 1), (513, 250, 257), (2048, 40, 40), (130, 1000, 515), (512, 512, 512), (1030, 512, 768), (4096, 256, 256), (640, 2048, 1100)]
+          (257, 1, 300), (300, 260, 1), (513, 250, 257), (2048, 40, 40), (130, 1000, 515), (512, 512, 512), (1030, 512, 768), (4096, 256, 256), (640, 2048, 1100),
+          (2048, 2048, 2048), (2177, 2056, 2100), (4100, 2051, 2033), (5000, 1800, 2300)]        # the large tiles, with and without splits
 
 
 @pytest.mark.gpu
@@ -56,7 +66,7 @@ def test_gradient_is_the_formulas_difference():
     M, O, I = 40, 6, 20
     g, codes, scale = make(M, O, I, torch.float16, 3)
     gw = tokens.linear_tokens_grad_weight(g, codes, scale, torch.float32).double()
-    values = tokens.dequantize_tokens(codes, scale, torch.float16).double()
+    values = kept_values(codes, scale, torch.float16)
     w = torch.randn(O, I, device=DEV, dtype=torch.float64)
     loss = lambda w: (g.double() * (values @ w.t())).sum()  # noqa: E731
     for o, i in ((0, 0), (3, 7), (5, 19)):
@@ -85,8 +95,8 @@ def test_layouts_strides_and_leading_dimensions(M, dtype):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("M", [1, 65, 257, 1023])
-@pytest.mark.parametrize("O,I", [(16, 48), (264, 512)])
+@pytest.mark.parametrize("M", [1, 65, 257, 1023, 2175])
+@pytest.mark.parametrize("O,I", [(16, 48), (264, 512), (2000, 2048)])
 def test_infinite_gradients_stay_where_they_are(M, O, I):
     # an infinite gradient of the last token spoils its own output alone, and as an infinity
     g, codes, scale = make(M, O, I, torch.bfloat16, 4)
@@ -109,7 +119,7 @@ def test_no_tokens_and_no_outputs():
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("M,O,I", [(512, 64, 200), (700, 520, 512)])
+@pytest.mark.parametrize("M,O,I", [(512, 64, 200), (700, 520, 512), (2100, 2000, 2003)])
 def test_captured_and_replayed(M, O, I):
     g, codes, scale = make(M, O, I, torch.bfloat16, 1)
     side = torch.cuda.Stream()

@@ -5,12 +5,16 @@
 //   backward   n = (x' - mean) rstd from the codes' values x' = code * scale (or from x itself), z as above, dz = dy act'(z);
 //              db = sum dz,  dw = sum dz n,  u = dz w,  dx = rstd (u - mean(u) - n mean(u n))
 //
-// All four passes are bound by memory.  A pixel's channels are consecutive, a group's are not: blocks take whole groups side
+// Large tensors are bound by memory.  A pixel's channels are consecutive, a group's are not: blocks take whole groups side
 // by side (128 bytes of a pixel at least), a thread keeps the same 16 bytes of channels from pixel to pixel, so that
 // everything that goes by channel stays in its registers, and sums are made per channel first and per group at the end.
 // Each direction is two passes over the data with a table of partial results between them: a block of the second pass adds up
 // the entries of its own groups before it starts.  The second pass takes the samples in the opposite order: the first one's last
 // samples are still in the caches.
+//
+// Small tensors are bound by the instructions: a kernel's code comes from the L2 at about a microsecond a kilobyte when it is
+// run once.  So small planes take one kernel instead of two, a block to a plane's chunk that reads it twice; loops over
+// pixels are unrolled as far as loads need it and no further, and positions come from divisions prepared on the host.
 //
 // Sums and statistics are fp32.  The variance is summed about the mean, not as a difference of moments: a thread sums up to
 // 32 pixels about the first of them (which costs at most a factor of 32 of the last bit, however far the
@@ -21,6 +25,7 @@ namespace actnn {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kWide = 1024;              // of the kernel that adds up the parameters' gradients
 constexpr int kRun = 32;                 // pixels summed about the same value
 
 // How a tensor [N, pixels, C] in G groups is cut into blocks: `chunk` channels (`per` whole groups, or a part of one wider than
@@ -31,19 +36,19 @@ struct Cut {
   int per;                               // groups of a chunk; 0: `parts` chunks to a group
   int parts, chunk, chunks;              // chunks: over all channels
   int slices, slice;
+  int cols, rows;                        // vectors of a chunk's pixel, pixels of a round of the block's threads
+  FastDiv by_chunks, by_slices, by_parts, by_cols, by_rows, by_width;
   __host__ __device__ int slots() const { return slices * parts; }
+  int64_t blocks() const { return (int64_t)N * chunks * slices; }
 };
 
-template <typename T> bool whole_vectors(const Cut& c) {
-  constexpr int E = kVector<T>;
-  return c.C % E == 0 && c.chunk % E == 0 && (c.per || c.width % E == 0);
-}
+// vectors that are whole and lie at multiples of 16 bytes
+bool whole_vectors(const Cut& c, int E) { return c.C % E == 0 && c.chunk % E == 0 && (c.per || c.width % E == 0); }
 
 int gcd(int a, int b) { return b ? gcd(b, a % b) : a; }
 
-Cut cut_of(int64_t N, int64_t C, int64_t pixels, int64_t G, int E) {
-  Cut c;
-  c.N = (int)N; c.C = (int)C; c.G = (int)G; c.width = (int)(C / G); c.pixels = pixels;
+// A chunk of whole groups, ending with a vector where it can, of `least` vectors where there are as many channels.
+void cut_channels(Cut& c, int E, int least) {
   const int most = kThreads * E;
   if (c.width > most) {
     c.per = 0;
@@ -52,41 +57,80 @@ Cut cut_of(int64_t N, int64_t C, int64_t pixels, int64_t G, int E) {
     c.parts = (c.width + c.chunk - 1) / c.chunk;
     c.chunks = c.G * c.parts;
   } else {
-    // groups that end with a vector, 8 vectors at least
     int unit = E / gcd(c.width, E);
-    if ((int64_t)unit * c.width > most || C % E) unit = 1;
+    if ((int64_t)unit * c.width > most || c.C % E) unit = 1;
     int per = unit;
-    while (per < c.G && (int64_t)per * c.width < 8 * E && (int64_t)(per + unit) * c.width <= most) per += unit;
+    while (per < c.G && (int64_t)per * c.width < least * E && (int64_t)(per + unit) * c.width <= most) per += unit;
     if (per > c.G) per = c.G;
     c.per = per;
     c.parts = 1;
     c.chunk = per * c.width;
     c.chunks = (c.G + per - 1) / per;
   }
-  // slices: some thousand blocks, four rounds of pixels each at least
-  const int rows = kThreads / ((c.chunk + E - 1) / E);
-  int64_t slices = 2048 / ((int64_t)c.N * c.chunks);
-  const int64_t most_slices = (pixels + 4 * rows - 1) / (4 * rows);
-  if (slices > most_slices) slices = most_slices;
-  if (slices > 64) slices = 64;
-  if (slices < 1) slices = 1;
-  c.slice = (int)((pixels + slices - 1) / slices);
-  c.slices = (int)((pixels + c.slice - 1) / c.slice);
+  c.cols = (c.chunk + E - 1) / E;
+}
+void cut_pixels(Cut& c, int64_t slices) {
+  c.rows = kThreads / c.cols;
+  c.slice = (int)((c.pixels + slices - 1) / slices);
+  c.slices = (int)((c.pixels + c.slice - 1) / c.slice);
+  c.by_chunks = FastDiv((uint32_t)c.chunks);
+  c.by_slices = FastDiv((uint32_t)c.slices);
+  c.by_parts = FastDiv((uint32_t)c.parts);
+  c.by_cols = FastDiv((uint32_t)c.cols);
+  c.by_rows = FastDiv((uint32_t)c.rows);
+  c.by_width = FastDiv((uint32_t)c.width);
+}
+
+Cut cut_of(int64_t N, int64_t C, int64_t pixels, int64_t G, int E) {
+  Cut c;
+  c.N = (int)N; c.C = (int)C; c.G = (int)G; c.width = (int)(C / G); c.pixels = pixels;
+  // Chunks of 32 vectors (512 bytes of a pixel) while that leaves enough blocks, else of 16 or 8; slices for a thousand
+  // blocks, of eight rounds of pixels each at least ([128, 56 * 56, 256] bf16, both directions: 333 us; 2048 blocks 357, 4096
+  // 414, chunks of 8 vectors 351).
+  int64_t slices = 1;
+  for (int least = 32; least >= 8; least /= 2) {
+    cut_channels(c, E, least);
+    const int rows = kThreads / c.cols;
+    const int64_t most = (pixels + 8 * rows - 1) / (8 * rows);
+    slices = (1024 + (int64_t)c.N * c.chunks - 1) / ((int64_t)c.N * c.chunks);
+    if (slices > most) slices = most;
+    if (slices > 64) slices = 64;
+    if ((int64_t)c.N * c.chunks * slices >= 768) break;
+  }
+  const int64_t needed = (pixels * C >> 30) + 1;        // (offsets inside a slice are 32-bit)
+  if (slices < needed) slices = needed < pixels ? needed : pixels;
+  cut_pixels(c, slices);
   return c;
+}
+
+// One kernel: a block to a sample's chunk of 8 vectors at least, where a thread has few pixels ([4, 16 * 16, 320] fp16 both
+// directions 24.9 us, by two kernels each 27.4) or the blocks fill the chip anyway ([64, 28 * 28, 256] bf16 45.9, 67.9; 64 blocks
+// of 32 pixels a thread, [16, 32 * 32, 256]: 47.7, 34.0).  False: the plane is too large, or a group wider than a block.
+constexpr int kFewPixels = 16, kSomePixels = 64;
+bool cut_once(Cut& c, int E) {
+  Cut once = c;
+  cut_channels(once, E, 8);
+  if (!once.per || c.pixels * c.C >> 30) return false;
+  const int64_t mine = (c.pixels + kThreads / once.cols - 1) / (kThreads / once.cols);
+  if (mine > kFewPixels && (mine > kSomePixels || (int64_t)c.N * once.chunks < 256)) return false;
+  cut_pixels(once, 1);
+  c = once;
+  return true;
 }
 
 // The block's place: blocks run over the chunks first, then the slices, then the samples.
 struct Place {
-  int n, chunk, slice, part;
+  int n, slice, part;
   int c0, channels, g0, groups;          // first channel, number of them; first group, number of them
   int64_t p0;                            // first pixel, and how many
   int count;
-  int cols, rows, col, row;              // vectors of a pixel, pixels of a round; this thread's (row >= rows: none)
-  ACTNN_DEV Place(const Cut& c, uint32_t block, int E, bool backwards) {
-    chunk = block % c.chunks;
-    const uint32_t rest = block / c.chunks;
-    slice = rest % c.slices;
-    n = rest / c.slices;
+  int col, row;                          // this thread's vector, and its first pixel
+  int rounds, over;                      // pixels of every row of threads, and the rows that have one more
+  ACTNN_DEV Place(const Cut& c, int E, bool backwards) {
+    const uint32_t rest = c.by_chunks.div(blockIdx.x);
+    const int chunk = (int)(blockIdx.x - rest * c.chunks);
+    n = (int)c.by_slices.div(rest);
+    slice = (int)(rest - (uint32_t)n * c.slices);
     if (backwards) { n = c.N - 1 - n; slice = c.slices - 1 - slice; }
     if (c.per) {
       part = 0;
@@ -95,21 +139,23 @@ struct Place {
       c0 = g0 * c.width;
       channels = groups * c.width;
     } else {
-      part = chunk % c.parts;
-      g0 = chunk / c.parts;
+      g0 = (int)c.by_parts.div((uint32_t)chunk);
+      part = chunk - g0 * c.parts;
       groups = 1;
       c0 = g0 * c.width + part * c.chunk;
       channels = c.width - part * c.chunk < c.chunk ? c.width - part * c.chunk : c.chunk;
     }
     p0 = (int64_t)slice * c.slice;
     count = c.pixels - p0 < c.slice ? (int)(c.pixels - p0) : c.slice;
-    cols = (channels + E - 1) / E;
-    rows = kThreads / cols;
-    col = threadIdx.x % cols;
-    row = threadIdx.x / cols;
+    row = (int)c.by_cols.div(threadIdx.x);
+    col = (int)threadIdx.x - row * c.cols;
+    rounds = (int)c.by_rows.div((uint32_t)count);
+    over = count - rounds * c.rows;
+    at_end = col * E >= channels;                        // (the last chunk may have fewer vectors)
   }
-  ACTNN_DEV int mine() const { return row < rows && row < count ? (count - row + rows - 1) / rows : 0; }     // this thread's pixels
-  ACTNN_DEV int of_row(int r) const { return r < count ? (count - r + rows - 1) / rows : 0; }
+  bool at_end;
+  ACTNN_DEV int of_row(int r) const { return rounds + (r < over); }
+  ACTNN_DEV int mine(const Cut& c) const { return row < c.rows && !at_end ? of_row(row) : 0; }     // this thread's pixels
   ACTNN_DEV int valid(int E) const { return channels - col * E < E ? channels - col * E : E; }
 };
 
@@ -120,12 +166,12 @@ template <typename T, bool WHOLE> struct Source {
   int valid;
   ACTNN_DEV Source(const T* base, const Cut& c, const Place& b) {
     constexpr int E = kVector<T>;
-    at = base + ((int64_t)b.n * c.pixels + b.p0) * c.C + b.c0 + b.col * E;
+    at = base + ((int64_t)b.n * c.pixels + b.p0) * c.C + b.c0 + (b.at_end ? 0 : b.col * E);
     const int64_t all = (int64_t)c.N * c.pixels * c.C;
     last = base + (all > E ? all - E : 0);               // (a smaller tensor has room for 16 bytes)
     valid = b.valid(E);
   }
-  ACTNN_DEV u32x4 get(int64_t offset) const {
+  ACTNN_DEV u32x4 get(int offset) const {
     if constexpr (WHOLE) return load16(at + offset);
     else return row_vector_ends<T>(load16_row<T>(at + offset, valid, last));
   }
@@ -160,17 +206,50 @@ template <typename T, bool WHOLE> ACTNN_DEV typename CodeWords<T>::type get_code
   }
 }
 
+// A thread's pixels, AHEAD of them on their way while as many before them are worked on (two: four are 2 % faster for the largest
+// tensors and 5 to 8 % slower below, by their code): get(offset) loads one, use(vector,
+// offset, i) works on it.  No load is guarded, the waits would follow each of them: what does not exist is the thread's
+// first vector once more.
+template <typename RAW, int AHEAD> struct Walk {
+  RAW next[AHEAD];
+  int at, step, mine;
+  template <typename GET> ACTNN_DEV void begin(const Cut& c, const Place& b, GET get) {
+    step = c.rows * c.C;
+    at = b.row * c.C;
+    mine = b.mine(c);
+    ahead(mine, get);
+  }
+  template <typename GET> ACTNN_DEV void ahead(int left, GET get) {
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) next[j] = get(j < left ? at + j * step : 0);
+  }
+  template <typename GET, typename USE> ACTNN_DEV void run(GET get, USE use) {
+    for (int i = 0; i < mine; i += AHEAD) {
+      RAW raw[AHEAD];
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) raw[j] = next[j];
+      const int here = at;
+      at += AHEAD * step;
+      ahead(mine - i - AHEAD, get);
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j)
+        if (i + j < mine) use(raw[j], here + j * step, i + j);
+    }
+  }
+};
+
 // ------------------------------------------------------------------------------------------
 // Sums over a group by a team of lanes: 1 to 64 lanes of a wave, a power of two of them.
 // ------------------------------------------------------------------------------------------
 struct Team {
   int size, lane, first, step;           // lanes of a team, this one; the team's first group, and the distance to its next
   ACTNN_DEV explicit Team(int groups) {
-    size = 64;
-    while (size > 1 && size * groups > kThreads) size >>= 1;
+    int shift = 6;
+    while (shift > 0 && groups << shift > kThreads) --shift;
+    size = 1 << shift;
     lane = threadIdx.x & (size - 1);
-    first = threadIdx.x / size;
-    step = kThreads / size;
+    first = threadIdx.x >> shift;
+    step = kThreads >> shift;
   }
   ACTNN_DEV float sum(float v) const {
     for (int d = size >> 1; d > 0; d >>= 1) v += __shfl_xor(v, d);
@@ -185,82 +264,84 @@ struct Team {
   }
 };
 
+// The entries [rows][width] of a group by the lanes of a team: f(row, channel).
+template <typename F> ACTNN_DEV void each_entry(const Team& team, const Cut& c, int width, int rows, F f) {
+  // (a part of a wide group has a width of its own)
+  const bool usual = width == c.width;
+  int r = usual ? (int)c.by_width.div((uint32_t)team.lane) : team.lane / width, ch = team.lane - r * width;
+  const int down = usual ? (int)c.by_width.div((uint32_t)team.size) : team.size / width, across = team.size - down * width;
+  while (r < rows) {
+    f(r, ch);
+    r += down;
+    ch += across;
+    if (ch >= width) { ch -= width; ++r; }
+  }
+}
+
 struct Partial { float mean, squares, count, top; };     // top: bits of the largest magnitude, as a float's
 
 // ------------------------------------------------------------------------------------------
-// Forward, first pass: partial statistics [N][G][slots].
+// Statistics: a thread's, by channel, and from those the block's, by group.
 // ------------------------------------------------------------------------------------------
-template <typename T, bool WHOLE>
-__global__ __launch_bounds__(kThreads) void group_norm_stats_kernel(const T* __restrict__ x, Partial* __restrict__ table, Cut c) {
+template <typename T> struct ChannelStats {
+  static constexpr int E = kVector<T>;
+  float mean[E], squares[E];
+  uint32_t top[4];
+  float first[E], s1[E], s2[E];          // a run of pixels about its first one
+  ACTNN_DEV ChannelStats() {
+#pragma unroll
+    for (int e = 0; e < E; ++e) mean[e] = squares[e] = 0.0f;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) top[q] = 0u;
+  }
+  // the thread's pixel number i, the last one being number last
+  ACTNN_DEV void add(const u32x4& raw, int i, int last) {
+    float f[E];
+    widen(static_cast<const T*>(nullptr), raw, f);
+    if (i % kRun == 0) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        first[e] = f[e];
+        s1[e] = s2[e] = 0.0f;
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const float d = f[e] - first[e];
+      s1[e] += d;
+      s2[e] = __builtin_fmaf(d, d, s2[e]);
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) top[q] = Top<T>::larger(top[q], raw[q] & (sizeof(T) == 4 ? 0x7fffffffu : 0x7fff7fffu));
+    if (i % kRun == kRun - 1 || i == last) {
+      const float run = (float)(i % kRun + 1), done = (float)(i / kRun * kRun);
+      const float by_run = 1.0f / run, share = run / (done + run);
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const float m = s1[e] * by_run, q = s2[e] - s1[e] * m, d = first[e] + m - mean[e];
+        squares[e] += q + d * d * (done * share);
+        mean[e] += d * share;
+      }
+    }
+  }
+  ACTNN_DEV uint32_t top_of(int e) const {
+    return sizeof(T) == 4 ? top[e & 3] : (e & 1) ? top[(e >> 1) & 3] >> 16 : top[(e >> 1) & 3] & 0xffffu;
+  }
+};
+// emit(g, partial) by the first lane of each group's team
+template <typename T, typename F>
+ACTNN_DEV void block_stats(const ChannelStats<T>& mine, const Cut& c, const Place& b, F emit) {
   constexpr int E = kVector<T>;
   __shared__ float s_mean[kThreads * E], s_squares[kThreads * E];
   __shared__ uint32_t s_top[kThreads * E];
-  const Place b(c, blockIdx.x, E, false);
-  const int mine = b.mine();
-  const T* none = nullptr;
-  float mean[E], squares[E];
-  uint32_t top[4] = {0u, 0u, 0u, 0u};
-#pragma unroll
-  for (int e = 0; e < E; ++e) mean[e] = squares[e] = 0.0f;
-  if (mine > 0) {
-    const Source<T, WHOLE> src(x, c, b);
-    const int64_t step = (int64_t)b.rows * c.C;
-    int64_t at = (int64_t)b.row * c.C;
-    float done = 0.0f;
-    for (int i = 0; i < mine; i += kRun) {
-      const int run = mine - i < kRun ? mine - i : kRun;
-      float first[E], s1[E], s2[E];
-      auto add = [&](const u32x4& raw) {
-        float f[E];
-        widen(none, raw, f);
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const float d = f[e] - first[e];
-          s1[e] += d;
-          s2[e] = __builtin_fmaf(d, d, s2[e]);
-        }
-#pragma unroll
-        for (int k = 0; k < 4; ++k) top[k] = Top<T>::larger(top[k], raw[k] & (sizeof(T) == 4 ? 0x7fffffffu : 0x7fff7fffu));
-      };
-      {
-        const u32x4 raw = src.get(at);
-        widen(none, raw, first);
-#pragma unroll
-        for (int e = 0; e < E; ++e) s1[e] = s2[e] = 0.0f;
-        add(raw);
-        at += step;
-      }
-      int k = 1;
-      for (; k + 4 <= run; k += 4) {
-        u32x4 raw[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) raw[j] = src.get(at + j * step);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) add(raw[j]);
-        at += 4 * step;
-      }
-      for (; k < run; ++k) {
-        add(src.get(at));
-        at += step;
-      }
-      const float n = (float)run, total = done + n;
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const float m = s1[e] / n, q = s2[e] - s1[e] * m, d = first[e] + m - mean[e];
-        squares[e] += q + d * d * (done * n / total);
-        mean[e] += d * (n / total);
-      }
-      done = total;
-    }
-  }
-  // per channel and row of threads into LDS, then per group
-  if (b.row < b.rows) {
+  const int pitch = c.cols * E;
+  if (b.row < c.rows) {
+    const int at = b.row * pitch + b.col * E;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      const int at = (b.row * b.cols + b.col) * E + e;
-      s_mean[at] = mean[e];
-      s_squares[at] = squares[e];
-      s_top[at] = sizeof(T) == 4 ? top[e & 3] : (e & 1) ? top[(e >> 1) & 3] >> 16 : top[(e >> 1) & 3] & 0xffffu;
+      s_mean[at + e] = mine.mean[e];
+      s_squares[at + e] = mine.squares[e];
+      s_top[at + e] = mine.top_of(e);
     }
   }
   __syncthreads();
@@ -268,32 +349,47 @@ __global__ __launch_bounds__(kThreads) void group_norm_stats_kernel(const T* __r
   const int width = c.per ? c.width : b.channels;        // of a group, in this block
   const float count = (float)b.count * (float)width;
   for (int g = team.first; g < b.groups; g += team.step) {
-    const float about = s_mean[g * width];               // (means are summed about one of them, like values)
-    float sum = 0.0f;
+    const int at0 = g * width;
+    const float about = s_mean[at0];                     // (means are summed about one of them, like values)
+    float sum = 0.0f, m = about, q = 0.0f;
     uint32_t largest = 0;
-    for (int i = team.lane; i < b.rows * width; i += team.size) {
-      const int r = i / width, at = r * b.cols * E + g * width + i % width;
-      sum += (float)b.of_row(r) * (s_mean[at] - about);
-      largest = largest > s_top[at] ? largest : s_top[at];
-    }
-    // (rows of threads without a pixel have count 0, and mean 0)
-    const float m = about + team.sum(sum) / count;
-    largest = team.largest(largest);
-    float q = 0.0f;
-    for (int i = team.lane; i < b.rows * width; i += team.size) {
-      const int r = i / width, at = r * b.cols * E + g * width + i % width;
-      const float d = s_mean[at] - m;
-      q += s_squares[at] + (float)b.of_row(r) * d * d;
+    // twice: for the mean, and about it (rows of threads without a pixel count 0)
+    for (int pass = 0; pass < 2; ++pass) {
+      each_entry(team, c, width, c.rows, [&](int r, int ch) {
+        const int at = r * pitch + at0 + ch;
+        const float d = s_mean[at] - m, n = (float)b.of_row(r);
+        sum = __builtin_fmaf(n, d, sum);
+        q += __builtin_fmaf(n * d, d, s_squares[at]);
+        largest = largest > s_top[at] ? largest : s_top[at];
+      });
+      if (pass == 0) {
+        m = about + team.sum(sum) / count;
+        q = 0.0f;
+      }
     }
     q = team.sum(q);
-    if (team.lane == 0)
-      table[((int64_t)b.n * c.G + b.g0 + g) * c.slots() + b.slice * c.parts + b.part] = Partial{m, q, count, Top<T>::value(largest)};
+    largest = team.largest(largest);
+    if (team.lane == 0) emit(g, Partial{m, q, count, Top<T>::value(largest)});
   }
 }
 
-struct Moments { float mean, rstd, top; };
+// Forward, first pass: partial statistics [N][G][slots].
+template <typename T, bool WHOLE>
+__global__ __launch_bounds__(kThreads) void group_norm_stats_kernel(const T* __restrict__ x, Partial* __restrict__ table, Cut c) {
+  const Place b(c, kVector<T>, false);
+  const Source<T, WHOLE> src(x, c, b);
+  ChannelStats<T> stats;
+  Walk<u32x4, 2> walk;
+  auto get = [&](int offset) { return src.get(offset); };
+  walk.begin(c, b, get);
+  walk.run(get, [&](const u32x4& raw, int, int i) { stats.add(raw, i, walk.mine - 1); });
+  block_stats(stats, c, b, [&](int g, const Partial& v) {
+    table[((int64_t)b.n * c.G + b.g0 + g) * c.slots() + b.slice * c.parts + b.part] = v;
+  });
+}
+
 // a group's statistics from its partial ones, by a team; every lane has them
-ACTNN_DEV Moments join(const Team& team, const Partial* p, int slots, float eps) {
+ACTNN_DEV Partial join(const Team& team, const Partial* p, int slots) {
   const float about = p[0].mean;
   float n = 0.0f, sum = 0.0f;
   uint32_t top = 0;
@@ -313,14 +409,48 @@ ACTNN_DEV Moments join(const Team& team, const Partial* p, int slots, float eps)
     const float d = v.mean - mean;
     q += v.squares + v.count * d * d;
   }
-  q = team.sum(q);
-  return Moments{mean, 1.0f / __builtin_sqrtf(q / n + eps), as_float(top)};
+  return Partial{mean, team.sum(q), n, as_float(top)};
 }
 
 ACTNN_DEV float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.0f + __expf(-z)); }
 
+// A thread's vector of a parameter, `fallback` without one.
+template <int E, bool WHOLE> ACTNN_DEV void by_channel(const float* p, const Place& b, float fallback, float (&v)[E]) {
+#pragma unroll
+  for (int e = 0; e < E; ++e) v[e] = fallback;
+  if (!p) return;
+  const float* from = p + b.c0 + (b.at_end ? 0 : b.col * E);
+  if constexpr (WHOLE) {
+#pragma unroll
+    for (int i = 0; i < E; i += 4) {
+      const u32x4 w = load16(from + i);
+      v[i] = as_float(w.x); v[i + 1] = as_float(w.y); v[i + 2] = as_float(w.z); v[i + 3] = as_float(w.w);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = from[e < b.valid(E) && !b.at_end ? e : 0];
+  }
+}
+// f(e, group in the chunk) for the channels of a thread's vector
+template <int E, typename F> ACTNN_DEV void by_group(const Cut& c, const Place& b, F f) {
+  int g = 0, left = c.C;
+  if (c.per) {
+    const int ch = b.at_end ? 0 : b.col * E;
+    g = (int)c.by_width.div((uint32_t)ch);
+    left = (g + 1) * c.width - ch;
+  }
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    f(e, g);
+    if (--left == 0) {
+      left = c.width;
+      if (g + 1 < b.groups) ++g;                         // (behind the chunk's last channel: nobody uses it)
+    }
+  }
+}
+
 // ------------------------------------------------------------------------------------------
-// Forward, second pass.
+// Forward: from statistics to outputs and codes.
 // ------------------------------------------------------------------------------------------
 struct Forward {
   const Partial* table;
@@ -329,45 +459,43 @@ struct Forward {
   int8_t* codes;
   float eps;
 };
-template <typename T, bool WHOLE, bool SILU, bool KEEP>
-__global__ __launch_bounds__(kThreads) void group_norm_apply_kernel(const T* __restrict__ x, T* __restrict__ y, Forward f, Cut c) {
-  constexpr int E = kVector<T>;
-  __shared__ Moments s_group[kThreads * E];
-  const Place b(c, blockIdx.x, E, true);
-  const Team team(b.groups);
-  for (int g = team.first; g < b.groups; g += team.step) {
-    const int64_t at = (int64_t)b.n * c.G + b.g0 + g;
-    const Moments m = join(team, f.table + at * c.slots(), c.slots(), f.eps);
-    if (team.lane == 0) {
-      s_group[g] = m;
-      if (b.slice == 0 && b.part == 0) {
-        f.mean[at] = m.mean;
-        f.rstd[at] = m.rstd;
-        if constexpr (KEEP) f.scale[at] = token_scale(m.top).scale;
-      }
-    }
+template <typename T> struct Group {     // factor 0: every code is 0
+  float mean, rstd;
+  decltype(Coder<T>::factor) factor;
+};
+// a group's statistics on their way to the channels and, by the block that has the group's first pixels, to memory
+template <typename T, bool KEEP> ACTNN_DEV Group<T> group_of(const Forward& f, const Partial& v, int64_t at, bool first) {
+  Group<T> g;
+  g.mean = v.mean;
+  g.rstd = 1.0f / __builtin_sqrtf(v.squares / v.count + f.eps);
+  g.factor = 0;
+  if constexpr (KEEP) {
+    const TokenScale s = token_scale(v.top);
+    if (s.keep) g.factor = Coder<T>(v.top).factor;
+    if (first) f.scale[at] = s.scale;
   }
-  __syncthreads();
-  const int mine = b.mine();
-  if (mine == 0) return;
+  if (first) {
+    f.mean[at] = g.mean;
+    f.rstd[at] = g.rstd;
+  }
+  return g;
+}
+// what goes by channel for a thread's vector
+template <typename T, bool WHOLE, bool SILU, bool KEEP> struct Normalise {
+  static constexpr int E = kVector<T>;
   float mean[E], a[E], add[E];
-  Coder<T> coder[E] = {};
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    const int ch = b.col * E + e < b.channels ? b.col * E + e : b.channels - 1;
-    const Moments m = s_group[c.per ? ch / c.width : 0];
-    mean[e] = m.mean;
-    a[e] = f.weight ? m.rstd * f.weight[b.c0 + ch] : m.rstd;
-    add[e] = f.bias ? f.bias[b.c0 + ch] : 0.0f;
-    if constexpr (KEEP) {
-      if (token_scale(m.top).keep) coder[e] = Coder<T>(m.top);      // (else a factor of 0: codes 0)
-    }
+  Coder<T> coder[E];
+  ACTNN_DEV void init(const Forward& f, const Group<T>* groups, const Cut& c, const Place& b) {
+    by_channel<E, WHOLE>(f.weight, b, 1.0f, a);
+    by_channel<E, WHOLE>(f.bias, b, 0.0f, add);
+    by_group<E>(c, b, [&](int e, int g) {
+      mean[e] = groups[g].mean;
+      a[e] *= groups[g].rstd;
+      if constexpr (KEEP) coder[e].factor = groups[g].factor;
+    });
   }
-  const Source<T, WHOLE> src(x, c, b);
-  const int64_t step = (int64_t)b.rows * c.C, base = src.at - x;
-  int64_t at = (int64_t)b.row * c.C;
-  const T* none = nullptr;
-  auto put = [&](int64_t offset, const u32x4& raw) {
+  ACTNN_DEV void put(T* y, int8_t* codes, const u32x4& raw, int valid) const {
+    const T* none = nullptr;
     float v[E];
     widen(none, raw, v);
     if constexpr (KEEP) {
@@ -377,28 +505,44 @@ __global__ __launch_bounds__(kThreads) void group_norm_apply_kernel(const T* __r
       typename CodeWords<T>::type w;
       if constexpr (E == 4) w = pack_codes(q[0], q[1], q[2], q[3]);
       else w = (u32x2){pack_codes(q[0], q[1], q[2], q[3]), pack_codes(q[4 % E], q[5 % E], q[6 % E], q[7 % E])};
-      put_codes<T, WHOLE>(f.codes + base + offset, w, src.valid);
+      put_codes<T, WHOLE>(codes, w, valid);
     }
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       const float z = __builtin_fmaf(v[e] - mean[e], a[e], add[e]);
       v[e] = SILU ? z * sigmoid(z) : z;
     }
-    put_vector<T, WHOLE>(y + base + offset, narrow(none, v), src.valid);
-  };
-  int i = 0;
-  for (; i + 4 <= mine; i += 4) {
-    u32x4 raw[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) raw[j] = src.get(at + j * step);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) put(at + j * step, raw[j]);
-    at += 4 * step;
+    put_vector<T, WHOLE>(y, narrow(none, v), valid);
   }
-  for (; i < mine; ++i) {
-    put(at, src.get(at));
-    at += step;
+};
+// ONCE: the statistics too, from this block's own pixels; else from the table.
+template <typename T, bool WHOLE, bool SILU, bool KEEP, bool ONCE>
+__global__ __launch_bounds__(kThreads) void group_norm_apply_kernel(const T* __restrict__ x, T* __restrict__ y, Forward f, Cut c) {
+  __shared__ Group<T> s_group[kThreads * kVector<T>];
+  const Place b(c, kVector<T>, !ONCE);
+  const Source<T, WHOLE> src(x, c, b);
+  auto get = [&](int offset) { return src.get(offset); };
+  Walk<u32x4, 2> walk;
+  walk.begin(c, b, get);                                 // (before the statistics are joined)
+  if constexpr (ONCE) {
+    ChannelStats<T> stats;
+    walk.run(get, [&](const u32x4& raw, int, int i) { stats.add(raw, i, walk.mine - 1); });
+    walk.begin(c, b, get);
+    block_stats(stats, c, b, [&](int g, const Partial& v) { s_group[g] = group_of<T, KEEP>(f, v, (int64_t)b.n * c.G + b.g0 + g, true); });
+  } else {
+    const Team team(b.groups);
+    for (int g = team.first; g < b.groups; g += team.step) {
+      const int64_t at = (int64_t)b.n * c.G + b.g0 + g;
+      const Partial v = join(team, f.table + at * c.slots(), c.slots());
+      if (team.lane == 0) s_group[g] = group_of<T, KEEP>(f, v, at, b.slice == 0 && b.part == 0);
+    }
   }
+  __syncthreads();
+  Normalise<T, WHOLE, SILU, KEEP> norm;
+  norm.init(f, s_group, c, b);
+  T* to = y + (src.at - x);
+  int8_t* codes = f.codes + (src.at - x);
+  walk.run(get, [&](const u32x4& raw, int offset, int) { norm.put(to + offset, codes + offset, raw, src.valid); });
 }
 
 // ------------------------------------------------------------------------------------------
@@ -417,29 +561,17 @@ template <typename T, bool WHOLE, bool SILU, bool CODES> struct Slope {
   static constexpr int E = kVector<T>;
   float by[E], less[E], w[E], add[E];    // n = value * by - less
   ACTNN_DEV void init(const Backward& k, const Cut& c, const Place& b) {
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const int ch = b.col * E + e < b.channels ? b.col * E + e : b.channels - 1;
-      const int64_t g = (int64_t)b.n * c.G + b.g0 + (c.per ? ch / c.width : 0);
-      const float rstd = k.rstd[g];
-      if constexpr (CODES) {
-        by[e] = k.scale[g] * rstd;
-        less[e] = k.mean[g] * rstd;
-      } else {
-        by[e] = rstd;
-        less[e] = k.mean[g];
-      }
-      w[e] = k.weight ? k.weight[b.c0 + ch] : 1.0f;
-      add[e] = k.bias ? k.bias[b.c0 + ch] : 0.0f;
-    }
+    by_channel<E, WHOLE>(k.weight, b, 1.0f, w);
+    if constexpr (SILU) by_channel<E, WHOLE>(k.bias, b, 0.0f, add);
+    const int64_t at = (int64_t)b.n * c.G + b.g0;
+    by_group<E>(c, b, [&](int e, int g) {
+      const float rstd = k.rstd[at + g];
+      by[e] = CODES ? k.scale[at + g] * rstd : rstd;
+      less[e] = CODES ? k.mean[at + g] * rstd : k.mean[at + g];
+    });
   }
   typedef typename CodeWords<T>::type Words;
   struct Raw { u32x4 dy, x; Words codes; };
-  ACTNN_DEV void fetch(Raw& r, const Source<T, WHOLE>& dy, const Source<T, WHOLE>& x, const int8_t* codes, int64_t at) const {
-    r.dy = dy.get(at);
-    if constexpr (CODES) r.codes = get_codes<T, WHOLE>(codes + at, dy.valid);
-    else r.x = x.get(at);
-  }
   ACTNN_DEV void values(const Raw& r, float (&n)[E], float (&dz)[E]) const {
     const T* none = nullptr;
     widen(none, r.dy, dz);
@@ -461,208 +593,255 @@ template <typename T, bool WHOLE, bool SILU, bool CODES> struct Slope {
     }
   }
 };
+template <typename T, bool WHOLE, bool SILU, bool CODES> struct Saved {
+  typedef typename Slope<T, WHOLE, SILU, CODES>::Raw Raw;
+  Source<T, WHOLE> dy, x;
+  const int8_t* codes;
+  ACTNN_DEV Saved(const T* g, const T* in, const int8_t* q, const Cut& c, const Place& b)
+      : dy(g, c, b), x(CODES ? g : in, c, b), codes(q + (dy.at - g)) {}
+  ACTNN_DEV Raw get(int offset) const {
+    Raw r;
+    r.dy = dy.get(offset);
+    if constexpr (CODES) r.codes = get_codes<T, WHOLE>(codes + offset, dy.valid);
+    else r.x = x.get(offset);
+    return r;
+  }
+};
+// a thread's sums over its pixels, by channel: dz, dz n
+template <typename T> struct ChannelSums {
+  static constexpr int E = kVector<T>;
+  float plain[E], by_n[E];
+  ACTNN_DEV ChannelSums() {
+#pragma unroll
+    for (int e = 0; e < E; ++e) plain[e] = by_n[e] = 0.0f;
+  }
+  template <typename SLOPE> ACTNN_DEV void add(const SLOPE& slope, const typename SLOPE::Raw& r) {
+    float n[E], dz[E];
+    slope.values(r, n, dz);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      plain[e] += dz[e];
+      by_n[e] = __builtin_fmaf(dz[e], n[e], by_n[e]);
+    }
+  }
+};
+// dx of a pixel: rstd (u - first - n second), the factors with rstd in them
+template <typename T, bool WHOLE, bool SILU, bool CODES> struct Gradient {
+  static constexpr int E = kVector<T>;
+  float by[E], first[E], second[E];
+  ACTNN_DEV void init(const Slope<T, WHOLE, SILU, CODES>& slope, const Backward& k, const float* firsts, const float* seconds,
+                      const Cut& c, const Place& b) {
+    const int64_t at = (int64_t)b.n * c.G + b.g0;
+    by_group<E>(c, b, [&](int e, int g) {
+      const float rstd = k.rstd[at + g];
+      by[e] = slope.w[e] * rstd;
+      first[e] = firsts[g] * rstd;
+      second[e] = seconds[g] * rstd;
+    });
+  }
+  ACTNN_DEV void put(T* dx, const Slope<T, WHOLE, SILU, CODES>& slope, const typename Slope<T, WHOLE, SILU, CODES>::Raw& r, int valid) const {
+    float n[E], dz[E];
+    slope.values(r, n, dz);
+#pragma unroll
+    for (int e = 0; e < E; ++e) dz[e] = __builtin_fmaf(-n[e], second[e], __builtin_fmaf(dz[e], by[e], -first[e]));
+    put_vector<T, WHOLE>(dx, narrow(static_cast<const T*>(nullptr), dz), valid);
+  }
+};
+
+// the threads' sums by channel, over the rows of threads: emit(which, channel of the chunk, sum)
+template <typename T, typename F>
+ACTNN_DEV void block_sums(const ChannelSums<T>& mine, const Cut& c, const Place& b, F emit) {
+  constexpr int E = kVector<T>;
+  __shared__ float s_sum[2][kThreads * E];
+  const int pitch = c.cols * E;
+  if (b.row < c.rows) {
+    const int at = b.row * pitch + b.col * E;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      s_sum[0][at + e] = mine.plain[e];
+      s_sum[1][at + e] = mine.by_n[e];
+    }
+  }
+  __syncthreads();
+  // lanes that share a channel: as many as there are threads for
+  const Team team(2 * b.channels);
+  for (int i = team.first; i < 2 * b.channels; i += team.step) {
+    const int which = i >= b.channels, ch = which ? i - b.channels : i;
+    float v = 0.0f;
+    for (int r = team.lane; r < c.rows; r += team.size) v += s_sum[which][r * pitch + ch];
+    v = team.sum(v);
+    if (team.lane == 0) emit(which, ch, v);
+  }
+}
 
 template <typename T, bool WHOLE, bool SILU, bool CODES>
 __global__ __launch_bounds__(kThreads) void group_norm_backward_sums_kernel(const T* __restrict__ dy, const T* __restrict__ x,
                                                                             Backward k, Cut c) {
-  constexpr int E = kVector<T>;
-  __shared__ float s_sum[2][kThreads * E];
-  const Place b(c, blockIdx.x, E, false);
-  const int mine = b.mine();
-  float sum[E], by_n[E];
-#pragma unroll
-  for (int e = 0; e < E; ++e) sum[e] = by_n[e] = 0.0f;
-  if (mine > 0) {
-    Slope<T, WHOLE, SILU, CODES> slope;
-    slope.init(k, c, b);
-    const Source<T, WHOLE> sdy(dy, c, b), sx(CODES ? dy : x, c, b);
-    const int8_t* codes = k.codes + (sdy.at - dy);
-    const int64_t step = (int64_t)b.rows * c.C;
-    int64_t at = (int64_t)b.row * c.C;
-    typename Slope<T, WHOLE, SILU, CODES>::Raw raw[4];
-    auto add = [&](int j) {
-      float n[E], dz[E];
-      slope.values(raw[j], n, dz);
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        sum[e] += dz[e];
-        by_n[e] = __builtin_fmaf(dz[e], n[e], by_n[e]);
-      }
-    };
-    int i = 0;
-    for (; i + 4 <= mine; i += 4) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) slope.fetch(raw[j], sdy, sx, codes, at + j * step);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) add(j);
-      at += 4 * step;
-    }
-    for (; i < mine; ++i) {
-      slope.fetch(raw[0], sdy, sx, codes, at);
-      add(0);
-      at += step;
-    }
-  }
-  if (b.row < b.rows) {
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      s_sum[0][(b.row * b.cols + b.col) * E + e] = sum[e];
-      s_sum[1][(b.row * b.cols + b.col) * E + e] = by_n[e];
-    }
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < 2 * b.channels; i += kThreads) {
-    const int which = i >= b.channels, ch = which ? i - b.channels : i;
-    float v = 0.0f;
-    for (int r = 0; r < b.rows; ++r) v += s_sum[which][r * b.cols * E + ch];
+  const Place b(c, kVector<T>, false);
+  typedef Saved<T, WHOLE, SILU, CODES> SavedT;
+  const SavedT saved(dy, x, k.codes, c, b);
+  auto get = [&](int offset) { return saved.get(offset); };
+  Walk<typename SavedT::Raw, 2> walk;
+  walk.begin(c, b, get);
+  Slope<T, WHOLE, SILU, CODES> slope;
+  slope.init(k, c, b);
+  ChannelSums<T> sums;
+  walk.run(get, [&](const typename SavedT::Raw& raw, int, int) { sums.add(slope, raw); });
+  block_sums(sums, c, b, [&](int which, int ch, float v) {
     k.sums[(((int64_t)b.n * c.slices + b.slice) * 2 + which) * c.C + b.c0 + ch] = v;
-  }
+  });
 }
 
-template <typename T, bool WHOLE, bool SILU, bool CODES>
+// ONCE: the sums too, from this block's own pixels; else from the table.
+template <typename T, bool WHOLE, bool SILU, bool CODES, bool ONCE>
 __global__ __launch_bounds__(kThreads) void group_norm_backward_apply_kernel(const T* __restrict__ dy, const T* __restrict__ x,
                                                                              T* __restrict__ dx, Backward k, Cut c) {
   constexpr int E = kVector<T>;
+  typedef Saved<T, WHOLE, SILU, CODES> SavedT;
   __shared__ float s_mean[2][kThreads * E];
-  const Place b(c, blockIdx.x, E, true);
-  const Team team(b.groups);
-  const float all = 1.0f / ((float)c.pixels * (float)c.width);
-  for (int g = team.first; g < b.groups; g += team.step) {
-    float first = 0.0f, second = 0.0f;
-    const float* sums = k.sums + (int64_t)b.n * c.slices * 2 * c.C + (int64_t)(b.g0 + g) * c.width;
-    for (int ch = team.lane; ch < c.width; ch += team.size) {
-      float s = 0.0f, t = 0.0f;
-      for (int j = 0; j < c.slices; ++j) {
-        s += sums[(int64_t)(2 * j) * c.C + ch];
-        t += sums[(int64_t)(2 * j + 1) * c.C + ch];
-      }
-      const float w = k.weight ? k.weight[(b.g0 + g) * c.width + ch] : 1.0f;
-      first = __builtin_fmaf(w, s, first);
-      second = __builtin_fmaf(w, t, second);
-    }
-    first = team.sum(first);
-    second = team.sum(second);
-    if (team.lane == 0) {
-      s_mean[0][g] = first * all;
-      s_mean[1][g] = second * all;
-    }
-  }
-  __syncthreads();
-  const int mine = b.mine();
-  if (mine == 0) return;
+  const Place b(c, E, !ONCE);
+  const SavedT saved(dy, x, k.codes, c, b);
+  auto get = [&](int offset) { return saved.get(offset); };
+  Walk<typename SavedT::Raw, 2> walk;
+  walk.begin(c, b, get);                                 // (before the sums are joined)
   Slope<T, WHOLE, SILU, CODES> slope;
   slope.init(k, c, b);
-  float rstd[E], first[E], second[E];
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    const int ch = b.col * E + e < b.channels ? b.col * E + e : b.channels - 1;
-    const int g = c.per ? ch / c.width : 0;
-    rstd[e] = k.rstd[(int64_t)b.n * c.G + b.g0 + g];
-    first[e] = s_mean[0][g] * rstd[e];
-    second[e] = s_mean[1][g] * rstd[e];
-  }
-  const Source<T, WHOLE> sdy(dy, c, b), sx(CODES ? dy : x, c, b);
-  const int64_t base = sdy.at - dy;
-  const int8_t* codes = k.codes + base;
-  const int64_t step = (int64_t)b.rows * c.C;
-  int64_t at = (int64_t)b.row * c.C;
-  typename Slope<T, WHOLE, SILU, CODES>::Raw raw[4];
-  const T* none = nullptr;
-  auto put = [&](int j, int64_t offset) {
-    float n[E], dz[E];
-    slope.values(raw[j], n, dz);
-#pragma unroll
-    for (int e = 0; e < E; ++e)
-      dz[e] = __builtin_fmaf(dz[e], slope.w[e] * rstd[e], -first[e]) - n[e] * second[e];
-    put_vector<T, WHOLE>(dx + base + offset, narrow(none, dz), sdy.valid);
+  const Team team(b.groups);
+  const float all = 1.0f / ((float)c.pixels * (float)c.width);
+  // a group's means of u and u n from its channels' sums, `rows` of them
+  auto means = [&](int rows, auto sum_of) {
+    for (int g = team.first; g < b.groups; g += team.step) {
+      float first = 0.0f, second = 0.0f;
+      each_entry(team, c, c.width, rows, [&](int j, int in) {
+        const int ch = g * c.width + in;
+        const float w = k.weight ? k.weight[b.g0 * c.width + ch] : 1.0f;
+        first = __builtin_fmaf(w, sum_of(j, 0, ch), first);
+        second = __builtin_fmaf(w, sum_of(j, 1, ch), second);
+      });
+      first = team.sum(first);
+      second = team.sum(second);
+      if (team.lane == 0) {
+        s_mean[0][g] = first * all;
+        s_mean[1][g] = second * all;
+      }
+    }
   };
-  int i = 0;
-  for (; i + 4 <= mine; i += 4) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) slope.fetch(raw[j], sdy, sx, codes, at + j * step);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) put(j, at + j * step);
-    at += 4 * step;
+  if constexpr (ONCE) {
+    __shared__ float s_total[2][kThreads * E];
+    ChannelSums<T> sums;
+    walk.run(get, [&](const typename SavedT::Raw& raw, int, int) { sums.add(slope, raw); });
+    walk.begin(c, b, get);
+    block_sums(sums, c, b, [&](int which, int ch, float v) {
+      s_total[which][ch] = v;
+      k.sums[((int64_t)b.n * 2 + which) * c.C + b.c0 + ch] = v;
+    });
+    __syncthreads();
+    if (!dx) return;
+    means(1, [&](int, int which, int ch) { return s_total[which][ch]; });
+  } else {
+    const float* sums = k.sums + (int64_t)b.n * c.slices * 2 * c.C + (int64_t)b.g0 * c.width;
+    means(c.slices, [&](int j, int which, int ch) { return sums[(int64_t)(2 * j + which) * c.C + ch]; });
   }
-  for (; i < mine; ++i) {
-    slope.fetch(raw[0], sdy, sx, codes, at);
-    put(0, at);
-    at += step;
-  }
+  __syncthreads();
+  Gradient<T, WHOLE, SILU, CODES> gradient;
+  gradient.init(slope, k, s_mean[0], s_mean[1], c, b);
+  T* to = dx + (saved.dy.at - dy);
+  walk.run(get, [&](const typename SavedT::Raw& raw, int offset, int) { gradient.put(to + offset, slope, raw, saved.dy.valid); });
 }
 
-// dw, db: the table's sums over samples and slices, 64 channels a block, 16 rows of the table at a time.
-__global__ __launch_bounds__(1024) void group_norm_backward_parameters_kernel(Backward k, Cut c) {
-  __shared__ float s_sum[16][64];
-  const int lane = threadIdx.x & 63, row = threadIdx.x >> 6;
-  const int which = blockIdx.y, ch = blockIdx.x * 64 + lane;
-  const int64_t rows = (int64_t)c.N * c.slices;
-  float v = 0.0f;
-  if (ch < c.C)
-    for (int64_t r = row; r < rows; r += 16) v += k.sums[(2 * r + which) * c.C + ch];
-  s_sum[row][lane] = v;
+// dw, db: the table's sums over samples and slices, 16 channels a block, 64 rows of the table at a time.
+__global__ __launch_bounds__(kWide) void group_norm_backward_parameters_kernel(Backward k, Cut c) {
+  constexpr int kChannels = 16, kRows = kWide / kChannels;
+  __shared__ float s_sum[kWide / 64][kChannels];
+  const int which = blockIdx.y, in = threadIdx.x & (kChannels - 1), ch = blockIdx.x * kChannels + in;
+  const int rows = c.N * c.slices;
+  const float* from = k.sums + (int64_t)which * c.C + (ch < c.C ? ch : c.C - 1);
+  const int64_t pitch = (int64_t)2 * c.C;
+  float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  int r = threadIdx.x / kChannels;
+  for (; r + 3 * kRows < rows; r += 4 * kRows)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] += from[(r + j * kRows) * pitch];
+  for (; r < rows; r += kRows) v[0] += from[r * pitch];
+  float sum = (v[0] + v[1]) + (v[2] + v[3]);
+  sum += __shfl_xor(sum, 16);
+  sum += __shfl_xor(sum, 32);
+  if ((threadIdx.x & 63) < kChannels) s_sum[threadIdx.x >> 6][in] = sum;
   __syncthreads();
-  if (row == 0 && ch < c.C) {
-    for (int r = 1; r < 16; ++r) v += s_sum[r][lane];
+  if (threadIdx.x < kChannels && ch < c.C) {
+    sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWide / 64; ++w) sum += s_sum[w][in];
     float* to = which ? k.dweight : k.dbias;
-    if (to) to[ch] = v;
+    if (to) to[ch] = sum;
   }
 }
 
 enum { kNone = 0, kSilu = 1 };
 
-template <typename T> int forward(const void* x, void* y, Forward f, const Cut& c, bool silu, bool keep, void* ws, hipStream_t s) {
-  const dim3 grid((unsigned)((int64_t)c.N * c.chunks * c.slices)), blk(kThreads);
+// picks the template's flags at run time
+template <typename F> void with_flag(bool flag, F f) {
+  if (flag) f(std::true_type{});
+  else f(std::false_type{});
+}
+
+template <typename T> int forward(const void* x, void* y, Forward f, Cut c, bool silu, bool keep, void* ws, hipStream_t s) {
+  const bool once = cut_once(c, kVector<T>);
+  const dim3 grid((unsigned)c.blocks()), blk(kThreads);
   const T* px = static_cast<const T*>(x);
   T* py = static_cast<T*>(y);
   f.table = static_cast<Partial*>(ws);
-  auto go = [&](auto whole) {
-    constexpr bool W = decltype(whole)::value;
-    group_norm_stats_kernel<T, W><<<grid, blk, 0, s>>>(px, static_cast<Partial*>(ws), c);
-    if (silu && keep) group_norm_apply_kernel<T, W, true, true><<<grid, blk, 0, s>>>(px, py, f, c);
-    else if (silu) group_norm_apply_kernel<T, W, true, false><<<grid, blk, 0, s>>>(px, py, f, c);
-    else if (keep) group_norm_apply_kernel<T, W, false, true><<<grid, blk, 0, s>>>(px, py, f, c);
-    else group_norm_apply_kernel<T, W, false, false><<<grid, blk, 0, s>>>(px, py, f, c);
-  };
-  const bool aligned = aligned16(x) && aligned16(y) && reinterpret_cast<uintptr_t>(f.codes) % 8 == 0;
-  if (aligned && whole_vectors<T>(c)) go(std::true_type{});
-  else go(std::false_type{});
+  const bool whole = whole_vectors(c, kVector<T>) && aligned16(x) && aligned16(y) && aligned16(f.weight) && aligned16(f.bias) &&
+                     reinterpret_cast<uintptr_t>(f.codes) % 8 == 0;
+  with_flag(whole, [&](auto W) {
+    if (!once) group_norm_stats_kernel<T, decltype(W)::value><<<grid, blk, 0, s>>>(px, static_cast<Partial*>(ws), c);
+    with_flag(silu, [&](auto S) {
+      with_flag(keep, [&](auto K) {
+        with_flag(once, [&](auto O) {
+          group_norm_apply_kernel<T, decltype(W)::value, decltype(S)::value, decltype(K)::value, decltype(O)::value>
+              <<<grid, blk, 0, s>>>(px, py, f, c);
+        });
+      });
+    });
+  });
   ACTNN_RETURN_LAUNCH_STATUS();
 }
 
 template <typename T>
-int backward(const void* dy, const void* x, void* dx, const Backward& k, const Cut& c, bool silu, hipStream_t s) {
-  const dim3 grid((unsigned)((int64_t)c.N * c.chunks * c.slices)), blk(kThreads);
+int backward(const void* dy, const void* x, void* dx, const Backward& k, Cut c, bool silu, hipStream_t s) {
+  const bool once = cut_once(c, kVector<T>);
+  const dim3 grid((unsigned)c.blocks()), blk(kThreads);
   const T *pdy = static_cast<const T*>(dy), *px = static_cast<const T*>(x);
   T* pdx = static_cast<T*>(dx);
-  auto go = [&](auto whole, auto act, auto codes) {
-    constexpr bool W = decltype(whole)::value, S = decltype(act)::value, Q = decltype(codes)::value;
-    group_norm_backward_sums_kernel<T, W, S, Q><<<grid, blk, 0, s>>>(pdy, px, k, c);
-    if (dx) group_norm_backward_apply_kernel<T, W, S, Q><<<grid, blk, 0, s>>>(pdy, px, pdx, k, c);
-    if (k.dweight || k.dbias)
-      group_norm_backward_parameters_kernel<<<dim3((unsigned)((c.C + 63) / 64), 2), dim3(1024), 0, s>>>(k, c);
-  };
-  auto by_source = [&](auto whole, auto act) {
-    if (k.codes) go(whole, act, std::true_type{});
-    else go(whole, act, std::false_type{});
-  };
-  auto by_act = [&](auto whole) {
-    if (silu) by_source(whole, std::true_type{});
-    else by_source(whole, std::false_type{});
-  };
-  const bool aligned = aligned16(dy) && (!x || aligned16(x)) && (!dx || aligned16(dx)) && reinterpret_cast<uintptr_t>(k.codes) % 8 == 0;
-  if (aligned && whole_vectors<T>(c)) by_act(std::true_type{});
-  else by_act(std::false_type{});
+  const bool whole = whole_vectors(c, kVector<T>) && aligned16(dy) && aligned16(x) && aligned16(dx) && aligned16(k.weight) &&
+                     aligned16(k.bias) && reinterpret_cast<uintptr_t>(k.codes) % 8 == 0;
+  with_flag(whole, [&](auto W) {
+    with_flag(silu, [&](auto S) {
+      with_flag(k.codes != nullptr, [&](auto Q) {
+        constexpr bool w = decltype(W)::value, a = decltype(S)::value, q = decltype(Q)::value;
+        if (once) {
+          group_norm_backward_apply_kernel<T, w, a, q, true><<<grid, blk, 0, s>>>(pdy, px, pdx, k, c);
+        } else {
+          group_norm_backward_sums_kernel<T, w, a, q><<<grid, blk, 0, s>>>(pdy, px, k, c);
+          if (dx) group_norm_backward_apply_kernel<T, w, a, q, false><<<grid, blk, 0, s>>>(pdy, px, pdx, k, c);
+        }
+      });
+    });
+  });
+  if (k.dweight || k.dbias)
+    group_norm_backward_parameters_kernel<<<dim3((unsigned)((c.C + 15) / 16), 2), dim3(kWide), 0, s>>>(k, c);
   ACTNN_RETURN_LAUNCH_STATUS();
 }
 
 int check(int64_t N, int64_t C, int64_t P, int64_t G, int dtype) {
-  if (N < 0 || C < 1 || P < 0 || G < 1 || C % G || N > 0x7fffff || C > 0x7fffff || P > 0x7fffffffLL) return ACTNN_EINVAL;
+  if (N < 0 || C < 1 || P < 0 || G < 1 || C % G || N > 0x7fffff || C > 0x3fffff || P > 0x7fffffffLL) return ACTNN_EINVAL;
   if (dtype != ACTNN_F32 && dtype != ACTNN_F16 && dtype != ACTNN_BF16) return ACTNN_EDTYPE;
   return ACTNN_OK;
 }
 int64_t forward_bytes(const Cut& c) { return (int64_t)c.N * c.G * c.slots() * (int64_t)sizeof(Partial); }
 int64_t backward_bytes(const Cut& c) { return (int64_t)c.N * c.slices * 2 * c.C * 4; }
+// (the block's number and the table's rows are 32-bit)
+bool too_many(const Cut& c) { return c.blocks() > 0x7fffffffLL || (int64_t)c.N * c.slices > 0x7fffff00LL; }
 
 }  // namespace
 }  // namespace actnn
@@ -688,7 +867,7 @@ extern "C" int actnn_group_norm_forward(const void* x, const float* weight, cons
   const int64_t size = dtype == ACTNN_F32 ? 4 : 2;
   if (reinterpret_cast<uintptr_t>(x) % size || reinterpret_cast<uintptr_t>(y) % size || !aligned16(workspace)) return ACTNN_EALIGN;
   const Cut c = cut_of(N, C, pixels, groups, dtype == ACTNN_F32 ? 4 : 8);
-  if (workspace_bytes < forward_bytes(c) || (int64_t)c.N * c.chunks * c.slices > 0x7fffffffLL) return ACTNN_EINVAL;
+  if (workspace_bytes < forward_bytes(c) || too_many(c)) return ACTNN_EINVAL;
   Forward f{nullptr, weight, bias, mean, rstd, scale, codes, (float)eps};
   hipStream_t s = static_cast<hipStream_t>(stream);
   const bool silu = activation == kSilu;
@@ -712,7 +891,7 @@ extern "C" int actnn_group_norm_backward(const void* dy, const int8_t* codes, co
       !aligned16(workspace))
     return ACTNN_EALIGN;
   const Cut c = cut_of(N, C, pixels, groups, dtype == ACTNN_F32 ? 4 : 8);
-  if (workspace_bytes < backward_bytes(c) || (int64_t)c.N * c.chunks * c.slices > 0x7fffffffLL) return ACTNN_EINVAL;
+  if (workspace_bytes < backward_bytes(c) || too_many(c)) return ACTNN_EINVAL;
   const Backward k{codes, scale, weight, bias, mean, rstd, static_cast<float*>(workspace), dweight, dbias};
   hipStream_t s = static_cast<hipStream_t>(stream);
   const bool silu = activation == kSilu;

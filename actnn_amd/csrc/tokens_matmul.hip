@@ -339,55 +339,65 @@ __global__ __launch_bounds__(kThreads, 1) void tokens_tile_kernel(Product p, int
 }
 
 // ------------------------------------------------------------------------------------------
-// Few tokens: 16 channels a block, MT tiles of 16 tokens, the waves share the features in pieces of 64.
+// Few tokens: 16 NT channels a block, MT tiles of 16 tokens; the waves share the features, a run of pieces of 64 each.
 // ------------------------------------------------------------------------------------------
-template <typename TY, int MT, int WAVES>
+template <typename TY, int MT, int NT, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void tokens_few_kernel(Product p) {
   constexpr int kAhead = 4;
-  __shared__ i32x4 s_sum[WAVES][MT][64];
+  __shared__ i32x4 s_sum[WAVES][NT * MT][64];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int o0 = blockIdx.x * 16;
+  const int o0 = blockIdx.x * 16 * NT;
   const int row = lane & 15, part = lane >> 4;
-  const int8_t* wp = p.w + (int64_t)(o0 + row < p.O ? o0 + row : p.O - 1) * p.ldw;
-  const int8_t* xp[MT];
+  const int8_t *wp[NT], *xp[MT];
+#pragma unroll
+  for (int i = 0; i < NT; ++i) wp[i] = p.w + (int64_t)(o0 + 16 * i + row < p.O ? o0 + 16 * i + row : p.O - 1) * p.ldw;
 #pragma unroll
   for (int i = 0; i < MT; ++i) xp[i] = p.x + (int64_t)(16 * i + row < p.M ? 16 * i + row : p.M - 1) * p.ldx;
-  i32x4 acc[MT];
+  i32x4 acc[NT][MT];
 #pragma unroll
-  for (int i = 0; i < MT; ++i) acc[i] = (i32x4){0, 0, 0, 0};
-  const int pieces = (p.K + 63) / 64;
-  for (int c0 = wave; c0 < pieces; c0 += kAhead * WAVES) {
-    u32x4 fw[kAhead], fx[kAhead][MT];
+  for (int i = 0; i < NT; ++i)
+#pragma unroll
+    for (int j = 0; j < MT; ++j) acc[i][j] = (i32x4){0, 0, 0, 0};
+  const int pieces = (p.K + 63) / 64, per = (pieces + WAVES - 1) / WAVES;
+  const int end = (wave + 1) * per < pieces ? (wave + 1) * per : pieces;
+  for (int c0 = wave * per; c0 < end; c0 += kAhead) {
+    u32x4 fw[kAhead][NT], fx[kAhead][MT];
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) {
-      int k = (c0 + j * WAVES) * 64 + part * 16;
-      k = k < p.K ? k : 0;                                             // (masked below)
-      fw[j] = load16(wp + k);
+      int k = (c0 + j) * 64 + part * 16;
+      k = k < p.K && c0 + j < end ? k : 0;                             // (masked below)
+#pragma unroll
+      for (int i = 0; i < NT; ++i) fw[j][i] = load16(wp[i] + k);
 #pragma unroll
       for (int i = 0; i < MT; ++i) fx[j][i] = load16(xp[i] + k);
     }
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) {
-      const int k = (c0 + j * WAVES) * 64 + part * 16;
-      if (k + 16 > p.K) fw[j] = first_bytes(fw[j], p.K - k);
+      const int left = c0 + j < end ? p.K - (c0 + j) * 64 - part * 16 : 0;
 #pragma unroll
-      for (int i = 0; i < MT; ++i)
-        acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, fw[j]), __builtin_bit_cast(i32x4, fx[j][i]),
-                                                       acc[i], 0, 0, 0);
+      for (int i = 0; i < NT; ++i) {
+        const u32x4 w = left < 16 ? first_bytes(fw[j][i], left) : fw[j][i];
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+          acc[i][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, w), __builtin_bit_cast(i32x4, fx[j][t]), acc[i][t], 0, 0, 0);
+      }
     }
   }
 #pragma unroll
-  for (int i = 0; i < MT; ++i) s_sum[wave][i][lane] = acc[i];
+  for (int i = 0; i < NT; ++i)
+#pragma unroll
+    for (int t = 0; t < MT; ++t) s_sum[wave][i * MT + t][lane] = acc[i][t];
   __syncthreads();
   // accumulator register c of a lane: channel 4 (lane / 16) + c, token lane % 16
-  for (int i = threadIdx.x; i < MT * 64; i += 64 * WAVES) {
-    i32x4 v = s_sum[0][i >> 6][i & 63];
+  for (int i = threadIdx.x; i < NT * MT * 64; i += 64 * WAVES) {
+    const int tile = i >> 6, in = i & 63;
+    i32x4 v = s_sum[0][tile][in];
 #pragma unroll
-    for (int w = 1; w < WAVES; ++w) v += s_sum[w][i >> 6][i & 63];
+    for (int w = 1; w < WAVES; ++w) v += s_sum[w][tile][in];
     const int sum[4] = {v.x, v.y, v.z, v.w};
-    const int channel = o0 + 4 * ((i & 63) >> 4);
-    if (channel < p.O) put4<TY>(p, 16 * (i >> 6) + (i & 15), channel, sum);
+    const int channel = o0 + 16 * (tile / MT) + 4 * (in >> 4);
+    if (channel < p.O) put4<TY>(p, 16 * (tile % MT) + (in & 15), channel, sum);
   }
 }
 
@@ -412,12 +422,14 @@ Plan plan_of(int64_t M, int64_t K, int64_t O) {
   const int64_t steps = (K + 63) / 64;
   auto tiles = [&](int64_t edge) { return ((M + edge - 1) / edge) * ((O + edge - 1) / edge); };
   const int edge = tiles(256) >= kCUs ? 256 : tiles(128) >= kCUs ? 128 : 64;
+  // Slices: a step of a block takes 0.35 us for the smaller tiles; the second launch about 4.5, and the sums are written and
+  // read back at some 4 TB/s.
   int64_t slices = 1;
-  if (tiles(edge) < kCUs) {
-    slices = kCUs / tiles(edge);
-    if (slices > steps / 8) slices = steps / 8;                        // eight steps at least
-    if (slices < 1) slices = 1;
-  }
+  auto cost_us = [&](int64_t n) {
+    return 0.35 * (double)((steps + n - 1) / n) + (n > 1 ? 4.5 + 8.0 * (double)n * (double)M * (double)O / 4.0e6 : 0.0);
+  };
+  for (int64_t n = 2; n * tiles(edge) <= 2 * kCUs && n <= 16 && n <= steps; n *= 2)
+    if (cost_us(n) < cost_us(slices)) slices = n;
   const int64_t per = (steps + slices - 1) / slices;
   return Plan{edge, (int)((steps + per - 1) / per), (int)per};
 }
@@ -433,13 +445,24 @@ template <typename TY> void launch_edge(const Product& p, const Plan& plan, int6
   else launch_tiles<TY, 1>(p, plan, blocks, s);
 }
 
+template <typename TY, int MT, int NT, int WAVES> void launch_few(const Product& p, hipStream_t s) {
+  tokens_few_kernel<TY, MT, NT, WAVES><<<dim3((unsigned)((p.O + 16LL * NT - 1) / (16 * NT))), dim3(64 * WAVES), 0, s>>>(p);
+}
+
 template <typename TY> int product(const Product& p, void* workspace, int64_t workspace_bytes, hipStream_t s) {
   Plan plan = plan_of(p.M, p.K, p.O);
   if (plan.edge == 0) {
-    const dim3 grid((unsigned)((p.O + 15) / 16)), blk(512);
-    if (p.M <= 16) tokens_few_kernel<TY, 1, 8><<<grid, blk, 0, s>>>(p);
-    else if (p.M <= 32) tokens_few_kernel<TY, 2, 8><<<grid, blk, 0, s>>>(p);
-    else tokens_few_kernel<TY, 4, 8><<<grid, blk, 0, s>>>(p);
+    // More channels to a block re-read the tokens less often, where 64 of them leave blocks for most of the chip; more waves to a
+    // block keep more loads in flight, where each has features enough (us, 16 channels / 64: [24, 4096] -> 16384 23.8 / 16.0,
+    // -> 4096 8.2 / 14.5; 4 waves / 16: [16, 1024] -> 4096 3.0 / 5.7, [32, 4096] -> 4096 by 16 channels 10.1 / 8.2).
+    const bool wide = p.O >= 12288, deep = p.K >= 2048;
+    if (p.M <= 16) launch_few<TY, 1, 1, 4>(p, s);
+    else if (p.M <= 32 && wide) launch_few<TY, 2, 4, 4>(p, s);
+    else if (p.M <= 32 && deep) launch_few<TY, 2, 1, 16>(p, s);
+    else if (p.M <= 32) launch_few<TY, 2, 1, 4>(p, s);
+    else if (wide) launch_few<TY, 4, 4, 4>(p, s);
+    else if (deep) launch_few<TY, 4, 1, 16>(p, s);
+    else launch_few<TY, 4, 1, 4>(p, s);
     ACTNN_RETURN_LAUNCH_STATUS();
   }
   const int64_t n = (int64_t)p.M * p.O;

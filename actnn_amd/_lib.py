@@ -89,6 +89,7 @@ SIGNATURES = {
     "actnn_tokens_dequantize": [c_vp, c_i64, c_vp, c_vp, c_i64, c_i64, c_i32, c_vp],
     "actnn_tokens_matmul_workspace_bytes": [c_i64, c_i64, c_i64],
     "actnn_tokens_matmul": [c_vp, c_i64, c_vp, c_vp, c_i64, c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_i32, c_vp, c_i64, c_vp],
+    "actnn_tokens_linear_few": [c_vp, c_i64, c_vp, c_i64, c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_i32, c_vp],
     "actnn_tokens_grad_weight_workspace_bytes": [c_i64, c_i64, c_i64],
     "actnn_tokens_grad_weight_wants_chunks": [c_i64, c_i64, c_i64],
     "actnn_tokens_grad_weight": [c_vp, c_i64, c_vp, c_i64, c_vp, c_vp, c_i64, c_i64, c_i64, c_i32, c_i32, c_vp, c_i64, c_vp],

@@ -737,6 +737,18 @@ PyObject* linear_tokens(PyObject* const* a, Py_ssize_t n) {
   const Rows rows(data, "data");
   const c10::DeviceGuard guard(data.device());
   const Weight w(wcodes, wscale, bias, data, rows.K);
+  const int64_t vector = 16 / data.element_size();
+  if (!keep && rows.M >= 1 && rows.M <= 4 && rows.K <= 16384 && rows.K % vector == 0 && rows.ld % vector == 0 &&
+      reinterpret_cast<uintptr_t>(rows.held.data_ptr()) % 16 == 0) {
+    std::vector<int64_t> size(data.sizes().begin(), data.sizes().end());
+    size.back() = w.rows.M;
+    const Tensor out = empty(size, data, data.scalar_type());
+    launch("linear_tokens", [&] {
+      return actnn_tokens_linear_few(ptr(rows.held), rows.ld, w.rows.data(), w.rows.ld, f32(w.scale), f32(w.bias), ptr(out), rows.M,
+                                     rows.K, w.rows.M, code_of(data.scalar_type()), stream_of(data));
+    });
+    return tuple_of(out, Tensor(), Tensor());
+  }
   const NewCodes kept(data);
   const CodeRows x(kept.codes, "codes");
   launch("linear_tokens", [&] {

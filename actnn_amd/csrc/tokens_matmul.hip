@@ -90,11 +90,9 @@ struct Product {
 ACTNN_DEV float scaled(int sum, float xs, float ws, float bias) { return __builtin_fmaf((float)sum * xs, ws, bias); }
 
 // four consecutive channels of a token, from their integer sums
-template <typename TY> ACTNN_DEV void put4(const Product& p, int64_t token, int channel, const int (&sum)[4]) {
-  if (token >= p.M) return;
+template <typename TY> ACTNN_DEV void put4(const Product& p, int64_t token, int channel, const int (&sum)[4], float xs) {
   TY* to = static_cast<TY*>(p.y) + token * p.O + channel;
   float v[4];
-  const float xs = p.xs[token];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int c = channel + i < p.O ? channel + i : p.O - 1;
@@ -104,14 +102,6 @@ template <typename TY> ACTNN_DEV void put4(const Product& p, int64_t token, int 
   for (int i = 0; i < 4; ++i)
     if (channel + i < p.O) Conv<TY>::store(to, i, v[i]);
 }
-template <> ACTNN_DEV void put4<int>(const Product& p, int64_t token, int channel, const int (&sum)[4]) {
-  if (token >= p.M) return;
-  int* to = static_cast<int*>(p.y) + token * p.O + channel;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (channel + i < p.O) to[i] = sum[i];
-}
-
 // the integer sums of 16 bytes' worth of channels of a token, of which `valid` exist
 template <typename TY, int V>
 ACTNN_DEV void put_row(TY* to, int valid, const int (&sum)[V], float xs, const float (&ws)[V], const float (&bias)[V]) {
@@ -397,7 +387,88 @@ __global__ __launch_bounds__(64 * WAVES) void tokens_few_kernel(Product p) {
     for (int w = 1; w < WAVES; ++w) v += s_sum[w][tile][in];
     const int sum[4] = {v.x, v.y, v.z, v.w};
     const int channel = o0 + 16 * (tile / MT) + 4 * (in >> 4);
-    if (channel < p.O) put4<TY>(p, 16 * (tile % MT) + (in & 15), channel, sum);
+    const int token = 16 * (tile % MT) + (in & 15);
+    if (channel < p.O && token < p.M) put4<TY>(p, token, channel, sum, p.xs[token]);
+  }
+}
+
+// ------------------------------------------------------------------------------------------
+// One to four tokens in full precision: every block turns them into codes for itself, in LDS, while its first pieces of the
+// weight are on their way; a launch and the wait between two are saved (one bf16 token x [4096, 4096]: 9.7 us by two kernels).
+// ------------------------------------------------------------------------------------------
+constexpr int kFused = 4;
+constexpr int kFusedFeatures = 16384;
+template <typename T>
+__global__ __launch_bounds__(kThreads) void tokens_linear_few_kernel(Product p, const T* __restrict__ x, int64_t ld) {
+  constexpr int E = kVector<T>, WAVES = kThreads / 64, kAhead = 4;
+  extern __shared__ __attribute__((aligned(16))) uint8_t s_codes[];    // [M][K to the next multiple of 64]
+  __shared__ uint32_t s_top[WAVES][kFused], s_scale[kFused];
+  __shared__ i32x4 s_sum[WAVES][64];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int o0 = blockIdx.x * 16;
+  const int row = lane & 15, part = lane >> 4;
+  const int8_t* wp = p.w + (int64_t)(o0 + row < p.O ? o0 + row : p.O - 1) * p.ldw;
+  const int pieces = (p.K + 63) / 64, per = (pieces + WAVES - 1) / WAVES, pitch = pieces * 64;
+  const int first = wave * per, end = first + per < pieces ? first + per : pieces;
+  u32x4 next[kAhead];
+  auto fetch = [&](int c0) {
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const int k = (c0 + j) * 64 + part * 16;
+      next[j] = load16(wp + (k < p.K && c0 + j < end ? k : 0));        // (the codes behind the last feature are zeros)
+    }
+  };
+  fetch(first);
+  const int vectors = p.K / E;
+  for (int m = 0; m < p.M; ++m) {
+    Top<T> top;
+    for (int v = threadIdx.x; v < vectors; v += kThreads) top.add(load16(x + m * ld + (int64_t)v * E));
+    const uint32_t largest = lanes_largest(top.one());
+    if (lane == 0) s_top[wave][m] = largest;
+  }
+  __syncthreads();
+  for (int m = 0; m < p.M; ++m) {
+    uint32_t largest = s_top[0][m];
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) largest = largest > s_top[w][m] ? largest : s_top[w][m];
+    const float value = Top<T>::value(largest);
+    const TokenScale ts = token_scale(value);
+    const Coder<T> coder(value);
+    typedef typename CodeWords<T>::type Words;
+    Words* codes = reinterpret_cast<Words*>(s_codes + m * pitch);
+    for (int v = threadIdx.x; v < pitch / E; v += kThreads) {
+      float f[E];
+      widen(static_cast<const T*>(nullptr), load16(x + m * ld + (int64_t)(v < vectors ? v : 0) * E), f);
+      codes[v] = codes_of<T>(coder, f, v < vectors ? ts.keep : 0u);
+    }
+    if (threadIdx.x == 0) s_scale[m] = as_uint(ts.scale);
+  }
+  __syncthreads();
+  const uint8_t* xp = s_codes + (row < p.M ? row : 0) * pitch;
+  i32x4 acc = {0, 0, 0, 0};
+  for (int c0 = first; c0 < end; c0 += kAhead) {
+    u32x4 fw[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) fw[j] = next[j];
+    fetch(c0 + kAhead);
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const u32x4 zero = {0u, 0u, 0u, 0u};
+      const u32x4 fx = *reinterpret_cast<const u32x4*>(xp + (c0 + j < end ? c0 + j : first) * 64 + part * 16);
+      const u32x4 w = c0 + j < end ? fw[j] : zero;
+      acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, w), __builtin_bit_cast(i32x4, fx), acc, 0, 0, 0);
+    }
+  }
+  s_sum[wave][lane] = acc;
+  __syncthreads();
+  if (wave == 0) {
+    i32x4 v = s_sum[0][lane];
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) v += s_sum[w][lane];
+    const int sum[4] = {v.x, v.y, v.z, v.w};
+    const int channel = o0 + 4 * part;
+    if (channel < p.O && row < p.M) put4<T>(p, row, channel, sum, as_float(s_scale[row]));
   }
 }
 
@@ -509,4 +580,33 @@ extern "C" int actnn_tokens_matmul(const int8_t* codes, int64_t ldc, const float
   if (dtype == ACTNN_F32) return product<float>(p, workspace, workspace_bytes, s);
   if (dtype == ACTNN_F16) return product<__half>(p, workspace, workspace_bytes, s);
   return product<bf16_t>(p, workspace, workspace_bytes, s);
+}
+
+namespace actnn {
+namespace {
+template <typename T> void launch_linear_few(const Product& p, const void* x, int64_t ld, hipStream_t s) {
+  const size_t lds = (size_t)p.M * ((p.K + 63) / 64 * 64);
+  tokens_linear_few_kernel<T><<<dim3((unsigned)((p.O + 15) / 16)), dim3(kThreads), lds, s>>>(p, static_cast<const T*>(x), ld);
+}
+}  // namespace
+}  // namespace actnn
+
+extern "C" int actnn_tokens_linear_few(const void* data, int64_t ld, const int8_t* weight_codes, int64_t ldw,
+                                       const float* weight_scale, const float* bias, void* out, int64_t M, int64_t K, int64_t O,
+                                       int dtype, void* stream) {
+  using namespace actnn;
+  if (M < 0 || M > kFused || K < 1 || K > kFusedFeatures || O < 0 || O > 0x7fffff00LL || ld < 0) return ACTNN_EINVAL;
+  if (ldw < K || ldw % 16 || ldw > kMostStride) return ACTNN_EINVAL;
+  if (dtype != ACTNN_F32 && dtype != ACTNN_F16 && dtype != ACTNN_BF16) return ACTNN_EDTYPE;
+  const int64_t vector = dtype == ACTNN_F32 ? 4 : 8;
+  if (K % vector || ld % vector) return ACTNN_EINVAL;
+  if (M == 0 || O == 0) return ACTNN_OK;
+  if (!data || !weight_codes || !weight_scale || !out) return ACTNN_EINVAL;
+  if (!aligned16(data) || !aligned16(weight_codes) || reinterpret_cast<uintptr_t>(out) % (16 / vector)) return ACTNN_EALIGN;
+  const Product p{nullptr, nullptr, weight_codes, weight_scale, bias, out, 0, ldw, (int)M, (int)K, (int)O};
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (dtype == ACTNN_F32) launch_linear_few<float>(p, data, ld, s);
+  else if (dtype == ACTNN_F16) launch_linear_few<__half>(p, data, ld, s);
+  else launch_linear_few<bf16_t>(p, data, ld, s);
+  ACTNN_RETURN_LAUNCH_STATUS();
 }

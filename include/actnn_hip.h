@@ -528,6 +528,11 @@ int64_t actnn_tokens_matmul_workspace_bytes(int64_t M, int64_t K, int64_t O);
 int actnn_tokens_matmul(const int8_t* codes, int64_t ldc, const float* scale, const int8_t* weight_codes, int64_t ldw,
                         const float* weight_scale, const float* bias, void* out, int64_t M, int64_t K, int64_t O,
                         int dtype, void* workspace, int64_t workspace_bytes, void* stream);
+/* The same from one to four tokens in full precision, data [M, K] in dtype (the output's too), in one launch: the values of
+ * actnn_tokens_quantize and actnn_tokens_matmul after each other.  M <= 4, K <= 16384; rows of whole 16-byte vectors (data
+ * 16-byte aligned, K and ld multiples of 16 bytes). */
+int actnn_tokens_linear_few(const void* data, int64_t ld, const int8_t* weight_codes, int64_t ldw, const float* weight_scale,
+                            const float* bias, void* out, int64_t M, int64_t K, int64_t O, int dtype, void* stream);
 /* grad_w[O, I] (contiguous, out_dtype: that of grad_out or fp32) = grad_out[M, O]^T @ (codes * scale)[M, I], the values of the
  * codes rounded to grad_out's type (fp16 or bf16), the sum in fp32.  Rows of grad_out are ldg elements apart, at any
  * element address; a grad_out of fewer than 8 elements wants ldg >= 8 and that much memory for each row.  M >= 1.

@@ -69,7 +69,8 @@ def test_the_largest_sums(M, sign):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("M,K,O", [(1, 64, 40), (9, 1003, 130), (70, 200, 70), (600, 1030, 250)])
+@pytest.mark.parametrize("M,K,O", [(1, 64, 40), (1, 4096, 50), (1, 24, 17), (2, 1000, 33), (3, 1003, 16), (4, 4104, 100), (4, 16384, 20), (4, 16392, 20),
+                                   (5, 256, 48), (9, 1003, 130), (70, 200, 70), (600, 1030, 250)])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
 def test_linear_is_its_two_steps(M, K, O, dtype):
     gen = torch.Generator().manual_seed(M)
@@ -90,14 +91,14 @@ def test_linear_is_its_two_steps(M, K, O, dtype):
 
 @pytest.mark.gpu
 def test_a_bad_token_spoils_its_own_row_only():
-    for M in (5, 300):
+    for M in (4, 5, 300):
         x = torch.randn(M, 100, device=DEV)
         wcodes, wscale = tokens.quantize_tokens(torch.randn(70, 100, device=DEV))
         clean = tokens.linear_tokens(x, wcodes, wscale)
-        x[2, 50], x[4, 0] = float("nan"), float("-inf")
+        x[1, 50], x[3, 0] = float("nan"), float("-inf")
         y = tokens.linear_tokens(x, wcodes, wscale)
-        assert torch.isnan(y[[2, 4]]).all()
-        rest = [i for i in range(M) if i not in (2, 4)]
+        assert torch.isnan(y[[1, 3]]).all()
+        rest = [i for i in range(M) if i not in (1, 3)]
         assert torch.equal(y[rest], clean[rest])
 
 
@@ -180,5 +181,12 @@ def test_c_abi_refuses_bad_sizes(lib):
     assert f(None, 16, None, None, 16, None, None, None, 4, 16, 4, 9, None, 0, None) == -2
     assert f(8, 16, 16, 16, 16, 16, None, 16, 4, 16, 4, 0, None, 0, None) == -4
     assert lib.actnn_tokens_matmul_workspace_bytes(70, 8192, 64) > 0
+    few = lib.actnn_tokens_linear_few
+    assert few(None, 16, None, 16, None, None, None, 0, 16, 4, 0, None) == 0
+    assert few(None, 16, None, 16, None, None, None, 5, 16, 4, 0, None) == -1                    # more tokens than it takes
+    assert few(None, 18, None, 32, None, None, None, 1, 18, 4, 0, None) == -1                    # no whole vectors
+    assert few(None, 16400, None, 16400, None, None, None, 1, 16400, 4, 0, None) == -1
+    assert few(None, 16, None, 16, None, None, None, 1, 16, 4, 7, None) == -2
+    assert few(8, 16, 16, 16, 16, None, 16, 1, 16, 4, 0, None) == -4
     assert lib.actnn_tokens_matmul_workspace_bytes(8192, 4096, 4096) == 0
     assert lib.actnn_tokens_matmul_workspace_bytes(0, 4096, 4096) == 0

@@ -7,11 +7,9 @@
 // rounding; the sums are fp32).  v_mfma_f32_32x32x16, both tiles in LDS as they lie in memory, [token][column]; the
 // transposing read ds_read_b64_tr_b16 gives a lane four consecutive tokens of its column.
 //
-// Tile: 128 outputs x 128 features, four waves of 64 x 64, 64 tokens a step, two buffers.  A row of a tile is 256
-// bytes, all banks once; its 16-byte chunks lie at chunk ^ 4 (row % 4), so that the four rows which 32 lanes of a transposing
-// read touch (64 bytes each) fall into the four quarters of the banks.  Everything goes through registers: rows of any length at any
-// address, tokens past the end are zeros in both operands.  Few tiles: the tokens are split over blocks that leave fp32 tiles in a
-// workspace, a second kernel adds them in a fixed order.
+// Large products take tiles of 256 outputs x 256 features, fed by loads straight into LDS; small ones, and rows of
+// grad_out at any address, tiles of 64 or 128 fed through registers.  Few tiles: the tokens are split over blocks that leave fp32
+// tiles in a workspace, a second kernel adds them in a fixed order.
 #include <type_traits>
 
 #include "token_math.h"
@@ -60,131 +58,6 @@ struct Grad {
   int M, O, I;
 };
 
-template <typename T, typename TY>
-__global__ __launch_bounds__(kThreads, 2) void tokens_grad_kernel(Grad p, int splits, int tokens_per_split) {
-  constexpr int BO = 128, BI = 128, BK = 64, kRow = 256, kTile = BK * kRow;
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[4 * kTile];
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wr = wave & 1, wn = wave >> 1;
-  const int tiles_i = (p.I + BI - 1) / BI, tiles = (p.O + BO - 1) / BO * tiles_i;
-  const int split = blockIdx.x / tiles, tile = blockIdx.x % tiles;
-  const int o0 = tile / tiles_i * BO, i0 = tile % tiles_i * BI;
-  const int m0 = split * tokens_per_split;
-  const int m1 = p.M - m0 < tokens_per_split ? p.M : m0 + tokens_per_split;
-  TY* out = static_cast<TY*>(p.out) + (int64_t)split * p.O * p.I;
-
-  // ---- staging: thread -> chunk of eight columns tid % 16, rows tid / 16 + 16 j of both tiles
-  const int ch = tid & 15, row0 = tid >> 4;
-  const T* last = static_cast<const T*>(p.g) + p.g_last;
-  const bool in_x = i0 + ch * 8 < p.I;                  // (a row of codes is whole to the next multiple of 16)
-  RowVector rg[4];
-  u32x2 rx[4];
-  float rs[4];
-  auto fetch = [&](int m) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int at = m + row0 + 16 * j;
-      const int64_t row = at < m1 ? at : m1 - 1;
-      rg[j] = load16_row<T>(static_cast<const T*>(p.g) + row * p.ldg + o0 + ch * 8, at < m1 ? p.O - (o0 + ch * 8) : 0, last);
-      rx[j] = *reinterpret_cast<const u32x2*>(p.x + row * p.ldx + (in_x ? i0 + ch * 8 : 0));
-      rs[j] = p.scale[row];
-    }
-  };
-  auto stage = [&](int buffer, int m) {
-    uint8_t* tg = smem + buffer * 2 * kTile;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int row = row0 + 16 * j;
-      const int at = row * kRow + ((ch ^ ((row & 3) << 2)) << 4);
-      *reinterpret_cast<u32x4*>(tg + at) = row_vector_ends<T>(rg[j]);
-      *reinterpret_cast<u32x4*>(tg + kTile + at) = values_of<T>(rx[j], m + row < m1 ? rs[j] : 0.0f);
-    }
-  };
-
-  // ---- fragments: lane -> column n0 + lane % 32, tokens 16 kb + 8 (lane / 32) ..
-  const int blk = lane >> 4, r = lane & 15;
-  const int f_row = 8 * (blk >> 1) + (r >> 2);
-  auto fragment_at = [&](int n0) {
-    const int c = n0 / 8 + 2 * (blk & 1) + ((r & 3) >> 1);
-    return (uint32_t)(f_row * kRow + ((c ^ ((f_row & 3) << 2)) << 4) + (r & 1) * 8);
-  };
-  const uint32_t lds0 = lds_address(smem);
-  uint32_t ag[2], ax[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    ag[i] = lds0 + fragment_at(wr * 64 + 32 * i);
-    ax[i] = lds0 + kTile + fragment_at(wn * 64 + 32 * i);
-  }
-  f32x16 acc[2][2];
-#pragma unroll
-  for (int e = 0; e < 2; ++e)
-#pragma unroll
-    for (int a = 0; a < 2; ++a)
-#pragma unroll
-      for (int c = 0; c < 16; ++c) acc[e][a][c] = 0.0f;
-
-  if (m0 < m1) {
-    fetch(m0);
-    stage(0, m0);
-  }
-  __syncthreads();
-  int buffer = 0;
-  for (int m = m0; m < m1; m += BK) {
-    const bool more = m + BK < m1;
-    if (more) fetch(m + BK);
-    const uint32_t base = buffer * 2 * kTile;
-#pragma unroll
-    for (int kb = 0; kb < 4; ++kb) {
-      u32x4 fg[2], fx[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const u32x2 a = read_transposed(ag[i] + base + kb * 16 * kRow), b = read_transposed(ag[i] + base + (kb * 16 + 4) * kRow);
-        fg[i] = (u32x4){a.x, a.y, b.x, b.y};
-        const u32x2 c = read_transposed(ax[i] + base + kb * 16 * kRow), d = read_transposed(ax[i] + base + (kb * 16 + 4) * kRow);
-        fx[i] = (u32x4){c.x, c.y, d.x, d.y};
-      }
-#pragma unroll
-      for (int e = 0; e < 2; ++e)
-#pragma unroll
-        for (int a = 0; a < 2; ++a) acc[e][a] = mma16<T>(fx[e], fg[a], acc[e][a]);
-    }
-    if (more) stage(1 - buffer, m + BK);                // (its last readers passed the barrier of the step before)
-    __syncthreads();
-    buffer = 1 - buffer;
-  }
-
-  // accumulator register c of a lane: feature 8 (c / 4) + 4 (lane / 32) + c % 4 of the fragment, output lane % 32
-#pragma unroll
-  for (int a = 0; a < 2; ++a) {
-    const int o = o0 + wr * 64 + 32 * a + (lane & 31);
-    if (o >= p.O) continue;
-#pragma unroll
-    for (int e = 0; e < 2; ++e)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int i = i0 + wn * 64 + 32 * e + 8 * q + 4 * (lane >> 5);
-        TY* to = out + (int64_t)o * p.I + i;
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-          if (i + c < p.I) Conv<TY>::store(to, c, acc[e][a][4 * q + c]);
-      }
-  }
-}
-
-// ------------------------------------------------------------------------------------------
-// Large products: 256 outputs x 256 features a block, four waves of 128 x 128, 32 tokens a step.
-//
-// grad_out's rows go straight into LDS (global_load_lds; rows of whole 16-byte chunks), four buffers, loads three steps ahead.
-// The codes go into LDS as they are too, four steps ahead, each wave those of its eight tokens of a step with their scales; one
-// step ahead the wave turns them into values in the tile that the transposing reads take (two buffers).  So every load is one
-// whose arrival the kernel counts itself, and the step only waits for those of two steps before.  A row of a tile is 512 bytes, its
-// 32 chunks at chunk ^ 4 (row % 8).  Everything but the MFMAs stands beside one of them, about six instructions at most: fragment
-// reads and loads in the first eight of a group of sixteen, the values two at a time in the other eight.
-//
-// The first tokens, up to a multiple of 128, go through registers, masked: behind the last token there is nothing that may be
-// multiplied, an infinite gradient times a zero would be a NaN.
-// ------------------------------------------------------------------------------------------
 template <int N> struct Const { static constexpr int value = N; };
 template <int N, typename F> ACTNN_DEV void for_each(F&& f) {
   if constexpr (N > 0) {
@@ -215,6 +88,162 @@ ACTNN_DEV void wave_lds_fence() {                       // between writes and re
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
+// eight columns of a row of grad_out at any address: what lies behind the row's last column only reaches outputs that are not
+// stored; a vector that would end behind the tensor is read from its last 16 bytes
+template <typename T> ACTNN_DEV u32x4 load_columns(const T* at, const T* last) {
+  const int64_t over = at - last;
+  u32x4 v = load16_any(over > 0 ? last : at);
+  for (int i = 0; i < over && i < 8; ++i)
+    v = (u32x4){__builtin_amdgcn_alignbit(v.y, v.x, 16), __builtin_amdgcn_alignbit(v.z, v.y, 16), __builtin_amdgcn_alignbit(v.w, v.z, 16), v.w >> 16};
+  return v;
+}
+
+// ------------------------------------------------------------------------------------------
+// Small products, and rows at any address: 64 N outputs x 64 N features a block, four waves of 32 N x 32 N, 64 tokens a step,
+// two buffers, everything through registers; tokens past the end are zeros in both operands.
+// ------------------------------------------------------------------------------------------
+template <typename T, typename TY, int N>
+__global__ __launch_bounds__(kThreads) void tokens_grad_kernel(Grad p, int splits, int tokens_per_split) {
+  constexpr int kEdge = 64 * N, BK = 64, kRow = 2 * kEdge, kTile = BK * kRow;
+  constexpr int kChunks = kEdge / 8, kDown = kThreads / kChunks, kRounds = BK / kDown;
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[4 * kTile];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wr = wave & 1, wn = wave >> 1;
+  const int tiles_i = (p.I + kEdge - 1) / kEdge, tiles = (p.O + kEdge - 1) / kEdge * tiles_i;
+  const int split = splits > 1 ? blockIdx.x / tiles : 0, tile = splits > 1 ? blockIdx.x % tiles : blockIdx.x;
+  const int o0 = tile / tiles_i * kEdge, i0 = tile % tiles_i * kEdge;
+  const int m0 = split * tokens_per_split;
+  const int m1 = p.M - m0 < tokens_per_split ? p.M : m0 + tokens_per_split;
+  // chunk ch of row k lies at ch ^ swizzle(k): the four rows that 32 lanes of a transposing read touch, 64 bytes each, fall into
+  // the four quarters of the banks (rows of 256 bytes; of 128, where two rows share the banks)
+  auto swizzle = [](int row) { return N == 2 ? (row & 3) << 2 : ((row >> 1) & 1) << 2; };
+
+  // ---- staging: thread -> chunk of eight columns, rows tid / kChunks + kDown j of both tiles
+  const int ch = tid % kChunks, row0 = tid / kChunks;
+  const T* g = static_cast<const T*>(p.g);
+  const T* last = g + p.g_last;
+  const int g_col = o0 + ch * 8 < p.O ? o0 + ch * 8 : o0, x_col = i0 + ch * 8 < p.I ? i0 + ch * 8 : i0;
+  u32x4 rg[kRounds];
+  u32x2 rx[kRounds];
+  float rs[kRounds];
+  auto fetch = [&](int m) {
+#pragma unroll
+    for (int j = 0; j < kRounds; ++j) {
+      const int at = m + row0 + kDown * j;
+      const int64_t row = at < m1 ? at : m1 - 1;
+      rg[j] = load_columns(g + row * p.ldg + g_col, last);
+      rx[j] = *reinterpret_cast<const u32x2*>(p.x + row * p.ldx + x_col);
+      rs[j] = p.scale[row];
+    }
+  };
+  auto stage = [&](int buffer, int m) {
+    uint8_t* tg = smem + buffer * 2 * kTile;
+#pragma unroll
+    for (int j = 0; j < kRounds; ++j) {
+      const int row = row0 + kDown * j;
+      const bool valid = m + row < m1;
+      const int at = row * kRow + ((ch ^ swizzle(row)) << 4);
+      const u32x4 none = {0u, 0u, 0u, 0u};
+      *reinterpret_cast<u32x4*>(tg + at) = valid ? rg[j] : none;
+      *reinterpret_cast<u32x4*>(tg + kTile + at) = values_of<T>(rx[j], valid ? rs[j] : 0.0f);
+    }
+  };
+
+  // ---- fragments: lane -> column n0 + lane % 32, tokens 16 kb + 8 (lane / 32) ..
+  const int blk = lane >> 4, r = lane & 15;
+  const int f_row = 8 * (blk >> 1) + (r >> 2);
+  auto fragment_at = [&](int n0) {
+    const int c = n0 / 8 + 2 * (blk & 1) + ((r & 3) >> 1);
+    return (uint32_t)(f_row * kRow + ((c ^ swizzle(f_row)) << 4) + (r & 1) * 8);
+  };
+  const uint32_t lds0 = lds_address(smem);
+  uint32_t ag[N], ax[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    ag[i] = lds0 + fragment_at(wr * 32 * N + 32 * i);
+    ax[i] = lds0 + kTile + fragment_at(wn * 32 * N + 32 * i);
+  }
+  f32x16 acc[N][N];
+#pragma unroll
+  for (int e = 0; e < N; ++e)
+#pragma unroll
+    for (int a = 0; a < N; ++a)
+#pragma unroll
+      for (int c = 0; c < 16; ++c) acc[e][a][c] = 0.0f;
+
+  fetch(m0);
+  stage(0, m0);
+  __syncthreads();
+  uint32_t base = 0;
+  for (int m = m0; m < m1; m += BK) {
+    const bool more = m + BK < m1;
+    if (more) fetch(m + BK);
+#pragma unroll
+    for (int kb = 0; kb < 4; ++kb) {
+      auto fragment = [&](uint32_t at) {
+        const u32x2 a = read_transposed(at + base + kb * 16 * kRow), b = read_transposed(at + base + (kb * 16 + 4) * kRow);
+        return (u32x4){a.x, a.y, b.x, b.y};
+      };
+      u32x4 fg[N], fx[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        fg[i] = fragment(ag[i]);
+        fx[i] = fragment(ax[i]);
+      }
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+#pragma unroll
+        for (int a = 0; a < N; ++a) acc[e][a] = mma16<T>(fx[e], fg[a], acc[e][a]);
+    }
+    if (more) stage(base ? 0 : 1, m + BK);              // (its last readers passed the barrier of the step before)
+    __syncthreads();
+    base ^= 2 * kTile;
+  }
+
+  // accumulator register c of a lane: feature 8 (c / 4) + 4 (lane / 32) + c % 4 of the fragment, output lane % 32: through
+  // LDS, 32 outputs of the wave's features at a time, so that whole lines are stored
+  constexpr int kFeatures = 32 * N, kPitch = 4 * kFeatures + 16, V = 16 / sizeof(TY), kAcross = kFeatures / V, kOutputs = 64 / kAcross;
+  static_assert(4 * 32 * kPitch <= 4 * kTile, "the sums of 32 outputs of four waves fit");
+  const uint32_t slab = lds0 + (uint32_t)(wave * 32 * kPitch);
+  const int feature = i0 + wn * kFeatures + lane % kAcross * V;
+  TY* const out = static_cast<TY*>(p.out) + (int64_t)split * p.O * p.I + feature;
+#pragma unroll
+  for (int a = 0; a < N; ++a) {
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        lds_store(slab + (uint32_t)((lane & 31) * kPitch + 4 * (32 * e + 8 * q + 4 * (lane >> 5))),
+                  (u32x4){as_uint(acc[e][a][4 * q]), as_uint(acc[e][a][4 * q + 1]), as_uint(acc[e][a][4 * q + 2]), as_uint(acc[e][a][4 * q + 3])});
+    wave_lds_fence();
+    for (int j = lane / kAcross; j < 32; j += kOutputs) {
+      const int o = o0 + wr * 32 * N + 32 * a + j;
+      float v[V];
+#pragma unroll
+      for (int i = 0; i < V; i += 4) {
+        const u32x4 w = lds_load<u32x4>(slab + (uint32_t)(j * kPitch + (lane % kAcross * V + i) * 4));
+        v[i] = as_float(w.x); v[i + 1] = as_float(w.y); v[i + 2] = as_float(w.z); v[i + 3] = as_float(w.w);
+      }
+      store16_part<false>(out + (int64_t)o * p.I, narrow(static_cast<const TY*>(nullptr), v), o < p.O ? p.I - feature : 0);
+    }
+    wave_lds_fence();
+  }
+}
+
+// ------------------------------------------------------------------------------------------
+// Large products: 256 outputs x 256 features a block, four waves of 128 x 128, 32 tokens a step.
+//
+// grad_out's rows go straight into LDS (global_load_lds; rows of whole 16-byte chunks), four buffers, loads three steps ahead.
+// The codes go into LDS as they are too, four steps ahead, each wave those of its eight tokens of a step with their scales; one
+// step ahead the wave turns them into values in the tile that the transposing reads take (two buffers).  So every load is one
+// whose arrival the kernel counts itself, and the step only waits for those of two steps before.  A row of a tile is 512 bytes, its
+// 32 chunks at chunk ^ 4 (row % 8).  Everything but the MFMAs stands beside one of them, about six instructions at most: fragment
+// reads and loads in the first eight of a group of sixteen, the values two at a time in the other eight.
+//
+// The first tokens, up to a multiple of 128, go through registers, masked: behind the last token there is nothing that may be
+// multiplied, an infinite gradient times a zero would be a NaN.
+// ------------------------------------------------------------------------------------------
 template <typename T, typename TY>
 __global__ __launch_bounds__(kThreads, 1) void tokens_grad_large_kernel(Grad p, int splits, int tokens_per_split) {
   constexpr int BO = 256, BI = 256, BK = 32, kRow = 512, kTile = BK * kRow, NA = 4, NE = 4;
@@ -452,20 +481,26 @@ __global__ __launch_bounds__(kThreads) void tokens_grad_sum_kernel(const float* 
   Conv<TY>::store(out, i, v);
 }
 
-// Which kernel, and how many blocks share the tokens of a tile (`tokens` each).
+// Which kernel (the edge of its tiles), and how many blocks share the tokens of a tile (`tokens` each).
 struct Plan { int edge, splits, tokens; };
 Plan plan_of(int64_t M, int64_t O, int64_t I, bool aligned) {
   auto tiles = [&](int64_t edge) { return ((O + edge - 1) / edge) * ((I + edge - 1) / edge); };
-  auto cut = [&](int edge, int64_t unit, int64_t blocks, int64_t least) {   // about `blocks` of them, `least` units of tokens each
+  // Splits: a step of `unit` tokens takes step_us, the second launch about 4.5 us, and the partial tiles are written and read
+  // back at some 4 TB/s.
+  auto cut = [&](int edge, int64_t unit, double step_us, int64_t most_blocks) {
     const int64_t units = (M + unit - 1) / unit;
-    int64_t splits = tiles(edge) >= blocks ? 1 : blocks / tiles(edge);
-    if (splits > units / least) splits = units / least;
-    if (splits < 1) splits = 1;
+    auto cost_us = [&](int64_t n) {
+      return step_us * (double)((units + n - 1) / n) + (n > 1 ? 4.5 + 8.0 * (double)n * (double)O * (double)I / 4.0e6 : 0.0);
+    };
+    int64_t splits = 1;
+    for (int64_t n = 2; n * tiles(edge) <= most_blocks && n <= 64 && n <= units; n *= 2)
+      if (cost_us(n) < cost_us(splits)) splits = n;
     const int64_t per = (units + splits - 1) / splits;
     return Plan{edge, (int)((units + per - 1) / per), (int)(per * unit)};
   };
-  if (aligned && M >= 2048 && tiles(256) >= 64) return cut(256, 128, 256, 8);
-  return cut(128, 64, 512, 4);
+  if (aligned && M >= 2048 && tiles(256) >= 64) return cut(256, 128, 4.0, 256);
+  if (tiles(128) >= 192) return cut(128, 64, 1.1, 512);
+  return cut(64, 64, 0.6, 1024);
 }
 
 template <typename T, typename TY>
@@ -480,7 +515,8 @@ int launch_grad(Grad p, bool aligned, void* workspace, int64_t workspace_bytes, 
     using TO = std::remove_pointer_t<decltype(to)>;
     p.out = to;
     if (edge == 256) tokens_grad_large_kernel<T, TO><<<grid, blk, 0, s>>>(p, plan.splits, plan.tokens);
-    else tokens_grad_kernel<T, TO><<<grid, blk, 0, s>>>(p, plan.splits, plan.tokens);
+    else if (edge == 128) tokens_grad_kernel<T, TO, 2><<<grid, blk, 0, s>>>(p, plan.splits, plan.tokens);
+    else tokens_grad_kernel<T, TO, 1><<<grid, blk, 0, s>>>(p, plan.splits, plan.tokens);
   };
   TY* out = static_cast<TY*>(p.out);
   if (plan.splits == 1) {

@@ -474,33 +474,45 @@ __global__ __launch_bounds__(kThreads, 1) void tokens_grad_large_kernel(Grad p, 
 template <typename TY>
 __global__ __launch_bounds__(kThreads) void tokens_grad_sum_kernel(const float* __restrict__ part, TY* __restrict__ out,
                                                                    int64_t n, int splits) {
+  constexpr int kAhead = 8;                              // loads on their way; the additions keep their order
   const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
   if (i >= n) return;
   float v = 0.0f;
-  for (int s = 0; s < splits; ++s) v += part[s * n + i];
+  for (int s0 = 0; s0 < splits; s0 += kAhead) {
+    float w[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) w[j] = part[(s0 + j < splits ? s0 + j : 0) * n + i];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) v += s0 + j < splits ? w[j] : 0.0f;
+  }
   Conv<TY>::store(out, i, v);
 }
 
-// Which kernel (the edge of its tiles), and how many blocks share the tokens of a tile (`tokens` each).
+// Which kernel (the edge of its tiles), and how many blocks share the tokens of a tile (`tokens` each): the cheapest by this
+// estimate, us.  A step of a tile's tokens (32 for the large tiles, 64 for the others) takes step_us for each round of blocks over
+// the chip's 256 CUs (the small tiles: two blocks a CU at the same time); the start and the end of a block `fixed`; splits a
+// second launch of about 4.5, and their fp32 tiles are written and read back at some 8 TB/s (mostly in the last cache).  (Measured, large / 128 / 64: one
+// round of 256 steps 250, two of 16 59, one of 16 12.)
 struct Plan { int edge, splits, tokens; };
+struct Kernel { int edge, step, unit; double fixed, step_us; int64_t at_once; };
+constexpr Kernel kKernels[] = {{64, 64, 64, 3.0, 0.55, 512}, {128, 64, 64, 4.0, 1.0, 256}, {256, 32, 128, 8.0, 0.9, 256}};
 Plan plan_of(int64_t M, int64_t O, int64_t I, bool aligned) {
-  auto tiles = [&](int64_t edge) { return ((O + edge - 1) / edge) * ((I + edge - 1) / edge); };
-  // Splits: a step of `unit` tokens takes step_us, the second launch about 4.5 us, and the partial tiles are written and read
-  // back at some 4 TB/s.
-  auto cut = [&](int edge, int64_t unit, double step_us, int64_t most_blocks) {
-    const int64_t units = (M + unit - 1) / unit;
-    auto cost_us = [&](int64_t n) {
-      return step_us * (double)((units + n - 1) / n) + (n > 1 ? 4.5 + 8.0 * (double)n * (double)O * (double)I / 4.0e6 : 0.0);
-    };
-    int64_t splits = 1;
-    for (int64_t n = 2; n * tiles(edge) <= most_blocks && n <= 64 && n <= units; n *= 2)
-      if (cost_us(n) < cost_us(splits)) splits = n;
-    const int64_t per = (units + splits - 1) / splits;
-    return Plan{edge, (int)((units + per - 1) / per), (int)(per * unit)};
-  };
-  if (aligned && M >= 2048 && tiles(256) >= 64) return cut(256, 128, 4.0, 256);
-  if (tiles(128) >= 192) return cut(128, 64, 1.1, 512);
-  return cut(64, 64, 0.6, 1024);
+  Plan best{0, 1, 0};
+  double least = 0.0;
+  for (const Kernel& k : kKernels) {
+    if (k.edge == 256 && (!aligned || M < 512)) continue;
+    const int64_t tiles = ((O + k.edge - 1) / k.edge) * ((I + k.edge - 1) / k.edge), units = (M + k.unit - 1) / k.unit;
+    for (int64_t n = 1; n <= 64 && n <= units && (n == 1 || n * tiles <= 1024); n *= 2) {
+      const int64_t per = (units + n - 1) / n, rounds = (tiles * n + k.at_once - 1) / k.at_once;
+      const double us = k.fixed + k.step_us * (double)(rounds * per * (k.unit / k.step)) +
+                        (n > 1 ? 4.5 + 8.0 * (double)n * (double)O * (double)I / 8.0e6 : 0.0);
+      if (best.edge == 0 || us < least) {
+        least = us;
+        best = Plan{k.edge, (int)((units + per - 1) / per), (int)(per * k.unit)};
+      }
+    }
+  }
+  return best;
 }
 
 template <typename T, typename TY>

@@ -97,6 +97,12 @@ Cut cut_of(int64_t N, int64_t C, int64_t pixels, int64_t G, int E) {
     if (slices > 64) slices = 64;
     if ((int64_t)c.N * c.chunks * slices >= 768) break;
   }
+  if ((int64_t)c.N * c.chunks * slices < 768) {          // few blocks: four rounds ([5, 55 * 55, 96] 30.4 us, 27.9 like this)
+    const int rows = kThreads / c.cols;
+    int64_t most = (pixels + 4 * rows - 1) / (4 * rows);
+    if (most > 64) most = 64;
+    if (slices < most) slices = most;
+  }
   const int64_t needed = (pixels * C >> 30) + 1;        // (offsets inside a slice are 32-bit)
   if (slices < needed) slices = needed < pixels ? needed : pixels;
   cut_pixels(c, slices);

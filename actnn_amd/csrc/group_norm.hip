@@ -42,8 +42,13 @@ struct Cut {
   int64_t blocks() const { return (int64_t)N * chunks * slices; }
 };
 
-// vectors that are whole and lie at multiples of 16 bytes
-bool whole_vectors(const Cut& c, int E) { return c.C % E == 0 && c.chunk % E == 0 && (c.per || c.width % E == 0); }
+// Every chunk has a vector's channels.  Then all vectors are whole: where a chunk's channels are no whole number of them, the last
+// one begins earlier and shares channels with the one before (both compute and store the same).  Global memory takes
+// 16-byte accesses at any address.
+bool whole_vectors(const Cut& c, int E) {
+  const int last = c.per ? (c.G - (c.chunks - 1) * c.per) * c.width : c.width - (c.parts - 1) * c.chunk;
+  return c.chunk >= E && last >= E;
+}
 
 int gcd(int a, int b) { return b ? gcd(b, a % b) : a; }
 
@@ -53,8 +58,8 @@ void cut_channels(Cut& c, int E, int least) {
   if (c.width > most) {
     c.per = 0;
     c.parts = (c.width + most - 1) / most;
-    c.chunk = ((c.width + c.parts - 1) / c.parts + E - 1) / E * E;
-    c.parts = (c.width + c.chunk - 1) / c.chunk;
+    c.chunk = (c.width + c.parts - 1) / c.parts;
+    if ((int64_t)(c.parts - 1) * ((c.chunk + E - 1) / E * E) <= c.width - E) c.chunk = (c.chunk + E - 1) / E * E;
     c.chunks = c.G * c.parts;
   } else {
     int unit = E / gcd(c.width, E);
@@ -62,6 +67,9 @@ void cut_channels(Cut& c, int E, int least) {
     int per = unit;
     while (per < c.G && (int64_t)per * c.width < least * E && (int64_t)(per + unit) * c.width <= most) per += unit;
     if (per > c.G) per = c.G;
+    const int chunks = (c.G + per - 1) / per;            // as many groups to each
+    per = (c.G + chunks - 1) / chunks;
+    if (per % unit && per + unit - per % unit <= c.G && (int64_t)(per + unit - per % unit) * c.width <= most) per += unit - per % unit;
     c.per = per;
     c.parts = 1;
     c.chunk = per * c.width;
@@ -130,9 +138,9 @@ struct Place {
   int c0, channels, g0, groups;          // first channel, number of them; first group, number of them
   int64_t p0;                            // first pixel, and how many
   int count;
-  int col, row;                          // this thread's vector, and its first pixel
+  int cs, row;                           // the first channel of this thread's vector in the chunk, and its first pixel
   int rounds, over;                      // pixels of every row of threads, and the rows that have one more
-  ACTNN_DEV Place(const Cut& c, int E, bool backwards) {
+  ACTNN_DEV Place(const Cut& c, int E, bool backwards, bool whole) {
     const uint32_t rest = c.by_chunks.div(blockIdx.x);
     const int chunk = (int)(blockIdx.x - rest * c.chunks);
     n = (int)c.by_slices.div(rest);
@@ -154,42 +162,47 @@ struct Place {
     p0 = (int64_t)slice * c.slice;
     count = c.pixels - p0 < c.slice ? (int)(c.pixels - p0) : c.slice;
     row = (int)c.by_cols.div(threadIdx.x);
-    col = (int)threadIdx.x - row * c.cols;
+    cs = ((int)threadIdx.x - row * c.cols) * E;
     rounds = (int)c.by_rows.div((uint32_t)count);
     over = count - rounds * c.rows;
-    at_end = col * E >= channels;                        // (the last chunk may have fewer vectors)
+    at_end = cs >= channels;                             // (the last chunk may have fewer vectors)
+    if (whole) cs = cs < channels - E ? cs : channels - E;
+    else if (at_end) cs = 0;
   }
   bool at_end;
   ACTNN_DEV int of_row(int r) const { return rounds + (r < over); }
   ACTNN_DEV int mine(const Cut& c) const { return row < c.rows && !at_end ? of_row(row) : 0; }     // this thread's pixels
-  ACTNN_DEV int valid(int E) const { return channels - col * E < E ? channels - col * E : E; }
+  ACTNN_DEV int valid(int E) const { return channels - cs < E ? channels - cs : E; }
 };
 
-// vectors of 16 bytes of a tensor, whole and aligned or not
+// vectors of 16 bytes of a tensor, whole or not
 template <typename T, bool WHOLE> struct Source {
   const T* at;                           // this thread's vector of the slice's first pixel
   const T* last;
   int valid;
   ACTNN_DEV Source(const T* base, const Cut& c, const Place& b) {
     constexpr int E = kVector<T>;
-    at = base + ((int64_t)b.n * c.pixels + b.p0) * c.C + b.c0 + (b.at_end ? 0 : b.col * E);
+    at = base + ((int64_t)b.n * c.pixels + b.p0) * c.C + b.c0 + b.cs;
     const int64_t all = (int64_t)c.N * c.pixels * c.C;
     last = base + (all > E ? all - E : 0);               // (a smaller tensor has room for 16 bytes)
     valid = b.valid(E);
   }
   ACTNN_DEV u32x4 get(int offset) const {
-    if constexpr (WHOLE) return load16(at + offset);
+    if constexpr (WHOLE) return load16_any(at + offset);
     else return row_vector_ends<T>(load16_row<T>(at + offset, valid, last));
   }
 };
 template <typename T, bool WHOLE> ACTNN_DEV void put_vector(T* to, const u32x4& v, int valid) {
-  if constexpr (WHOLE) store16(to, v);
+  if constexpr (WHOLE) store16_any<false>(to, v);
   else store16_part<false>(to, v, valid);
 }
+typedef u32x2 u32x2_a1 __attribute__((aligned(1)));
+typedef uint32_t u32_a1 __attribute__((aligned(1)));
+template <typename T> struct CodesAnywhere { typedef u32x2_a1 type; };
+template <> struct CodesAnywhere<float> { typedef u32_a1 type; };
 template <typename T, bool WHOLE> ACTNN_DEV void put_codes(int8_t* to, typename CodeWords<T>::type w, int valid) {
-  typedef typename CodeWords<T>::type Words;
   if constexpr (WHOLE) {
-    *reinterpret_cast<Words*>(to) = w;
+    *reinterpret_cast<typename CodesAnywhere<T>::type*>(to) = w;
   } else {
     uint32_t words[2];
     if constexpr (sizeof(T) == 4) { words[0] = w; words[1] = 0; } else { words[0] = w.x; words[1] = w.y; }
@@ -201,7 +214,7 @@ template <typename T, bool WHOLE> ACTNN_DEV void put_codes(int8_t* to, typename 
 template <typename T, bool WHOLE> ACTNN_DEV typename CodeWords<T>::type get_codes(const int8_t* from, int valid) {
   typedef typename CodeWords<T>::type Words;
   if constexpr (WHOLE) {
-    return *reinterpret_cast<const Words*>(from);
+    return *reinterpret_cast<const typename CodesAnywhere<T>::type*>(from);
   } else {
     uint32_t words[2] = {0u, 0u};
 #pragma unroll
@@ -341,8 +354,8 @@ ACTNN_DEV void block_stats(const ChannelStats<T>& mine, const Cut& c, const Plac
   __shared__ float s_mean[kThreads * E], s_squares[kThreads * E];
   __shared__ uint32_t s_top[kThreads * E];
   const int pitch = c.cols * E;
-  if (b.row < c.rows) {
-    const int at = b.row * pitch + b.col * E;
+  if (b.row < c.rows && !b.at_end) {
+    const int at = b.row * pitch + b.cs;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       s_mean[at + e] = mine.mean[e];
@@ -382,7 +395,7 @@ ACTNN_DEV void block_stats(const ChannelStats<T>& mine, const Cut& c, const Plac
 // Forward, first pass: partial statistics [N][G][slots].
 template <typename T, bool WHOLE>
 __global__ __launch_bounds__(kThreads) void group_norm_stats_kernel(const T* __restrict__ x, Partial* __restrict__ table, Cut c) {
-  const Place b(c, kVector<T>, false);
+  const Place b(c, kVector<T>, false, WHOLE);
   const Source<T, WHOLE> src(x, c, b);
   ChannelStats<T> stats;
   Walk<u32x4, 2> walk;
@@ -425,25 +438,24 @@ template <int E, bool WHOLE> ACTNN_DEV void by_channel(const float* p, const Pla
 #pragma unroll
   for (int e = 0; e < E; ++e) v[e] = fallback;
   if (!p) return;
-  const float* from = p + b.c0 + (b.at_end ? 0 : b.col * E);
+  const float* from = p + b.c0 + b.cs;
   if constexpr (WHOLE) {
 #pragma unroll
     for (int i = 0; i < E; i += 4) {
-      const u32x4 w = load16(from + i);
+      const u32x4 w = load16_any(from + i);
       v[i] = as_float(w.x); v[i + 1] = as_float(w.y); v[i + 2] = as_float(w.z); v[i + 3] = as_float(w.w);
     }
   } else {
 #pragma unroll
-    for (int e = 0; e < E; ++e) v[e] = from[e < b.valid(E) && !b.at_end ? e : 0];
+    for (int e = 0; e < E; ++e) v[e] = from[e < b.valid(E) ? e : 0];
   }
 }
 // f(e, group in the chunk) for the channels of a thread's vector
 template <int E, typename F> ACTNN_DEV void by_group(const Cut& c, const Place& b, F f) {
   int g = 0, left = c.C;
   if (c.per) {
-    const int ch = b.at_end ? 0 : b.col * E;
-    g = (int)c.by_width.div((uint32_t)ch);
-    left = (g + 1) * c.width - ch;
+    g = (int)c.by_width.div((uint32_t)b.cs);
+    left = (g + 1) * c.width - b.cs;
   }
 #pragma unroll
   for (int e = 0; e < E; ++e) {
@@ -525,7 +537,7 @@ template <typename T, bool WHOLE, bool SILU, bool KEEP> struct Normalise {
 template <typename T, bool WHOLE, bool SILU, bool KEEP, bool ONCE>
 __global__ __launch_bounds__(kThreads) void group_norm_apply_kernel(const T* __restrict__ x, T* __restrict__ y, Forward f, Cut c) {
   __shared__ Group<T> s_group[kThreads * kVector<T>];
-  const Place b(c, kVector<T>, !ONCE);
+  const Place b(c, kVector<T>, !ONCE, WHOLE);
   const Source<T, WHOLE> src(x, c, b);
   auto get = [&](int offset) { return src.get(offset); };
   Walk<u32x4, 2> walk;
@@ -660,8 +672,8 @@ ACTNN_DEV void block_sums(const ChannelSums<T>& mine, const Cut& c, const Place&
   constexpr int E = kVector<T>;
   __shared__ float s_sum[2][kThreads * E];
   const int pitch = c.cols * E;
-  if (b.row < c.rows) {
-    const int at = b.row * pitch + b.col * E;
+  if (b.row < c.rows && !b.at_end) {
+    const int at = b.row * pitch + b.cs;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       s_sum[0][at + e] = mine.plain[e];
@@ -683,7 +695,7 @@ ACTNN_DEV void block_sums(const ChannelSums<T>& mine, const Cut& c, const Place&
 template <typename T, bool WHOLE, bool SILU, bool CODES>
 __global__ __launch_bounds__(kThreads) void group_norm_backward_sums_kernel(const T* __restrict__ dy, const T* __restrict__ x,
                                                                             Backward k, Cut c) {
-  const Place b(c, kVector<T>, false);
+  const Place b(c, kVector<T>, false, WHOLE);
   typedef Saved<T, WHOLE, SILU, CODES> SavedT;
   const SavedT saved(dy, x, k.codes, c, b);
   auto get = [&](int offset) { return saved.get(offset); };
@@ -705,7 +717,7 @@ __global__ __launch_bounds__(kThreads) void group_norm_backward_apply_kernel(con
   constexpr int E = kVector<T>;
   typedef Saved<T, WHOLE, SILU, CODES> SavedT;
   __shared__ float s_mean[2][kThreads * E];
-  const Place b(c, E, !ONCE);
+  const Place b(c, E, !ONCE, WHOLE);
   const SavedT saved(dy, x, k.codes, c, b);
   auto get = [&](int offset) { return saved.get(offset); };
   Walk<typename SavedT::Raw, 2> walk;
@@ -797,9 +809,7 @@ template <typename T> int forward(const void* x, void* y, Forward f, Cut c, bool
   const T* px = static_cast<const T*>(x);
   T* py = static_cast<T*>(y);
   f.table = static_cast<Partial*>(ws);
-  const bool whole = whole_vectors(c, kVector<T>) && aligned16(x) && aligned16(y) && aligned16(f.weight) && aligned16(f.bias) &&
-                     reinterpret_cast<uintptr_t>(f.codes) % 8 == 0;
-  with_flag(whole, [&](auto W) {
+  with_flag(whole_vectors(c, kVector<T>), [&](auto W) {
     if (!once) group_norm_stats_kernel<T, decltype(W)::value><<<grid, blk, 0, s>>>(px, static_cast<Partial*>(ws), c);
     with_flag(silu, [&](auto S) {
       with_flag(keep, [&](auto K) {
@@ -819,9 +829,7 @@ int backward(const void* dy, const void* x, void* dx, const Backward& k, Cut c, 
   const dim3 grid((unsigned)c.blocks()), blk(kThreads);
   const T *pdy = static_cast<const T*>(dy), *px = static_cast<const T*>(x);
   T* pdx = static_cast<T*>(dx);
-  const bool whole = whole_vectors(c, kVector<T>) && aligned16(dy) && aligned16(x) && aligned16(dx) && aligned16(k.weight) &&
-                     aligned16(k.bias) && reinterpret_cast<uintptr_t>(k.codes) % 8 == 0;
-  with_flag(whole, [&](auto W) {
+  with_flag(whole_vectors(c, kVector<T>), [&](auto W) {
     with_flag(silu, [&](auto S) {
       with_flag(k.codes != nullptr, [&](auto Q) {
         constexpr bool w = decltype(W)::value, a = decltype(S)::value, q = decltype(Q)::value;

@@ -90,12 +90,14 @@ __global__ __launch_bounds__(kThreads) void tokens_quantize_kernel(ROWS rows, in
 template <typename T>
 __global__ void tokens_quantize_tiny_kernel(const T* __restrict__ x, int64_t ld, int8_t* __restrict__ codes, int64_t ldc,
                                             float* __restrict__ scale, int M, int K) {
-  const int m = threadIdx.x;
+  const int m = blockIdx.x * 64 + threadIdx.x;           // (rows of a stride of 0 may be many)
   if (m >= M) return;
+  codes += (int64_t)m * ldc;
+  x += (int64_t)m * ld;
   float top = 0.0f;
   bool bad = false;
   for (int k = 0; k < K; ++k) {
-    const float v = __builtin_fabsf(Conv<T>::load(x, m * ld + k));
+    const float v = __builtin_fabsf(Conv<T>::load(x, k));
     bad = bad || !(v <= 3.402823466e38f);
     top = v > top ? v : top;
   }
@@ -103,7 +105,7 @@ __global__ void tokens_quantize_tiny_kernel(const T* __restrict__ x, int64_t ld,
   const TokenScale ts = token_scale(top);
   const Coder<T> coder(top);
   for (int k = 0; k < ldc && k < 16; ++k)
-    codes[m * ldc + k] = k < K && ts.keep ? (int8_t)coder.code(Conv<T>::load(x, m * ld + k)) : (int8_t)0;
+    codes[k] = k < K && ts.keep ? (int8_t)coder.code(Conv<T>::load(x, k)) : (int8_t)0;
   scale[m] = ts.scale;
 }
 
@@ -131,7 +133,7 @@ int quantize(const void* x, int64_t ldx, int8_t* codes, int64_t ldc, float* scal
   constexpr int E = kVector<T>;
   const T* p = static_cast<const T*>(x);
   if ((M - 1) * ldx + K < E) {
-    tokens_quantize_tiny_kernel<T><<<dim3(1), dim3(64), 0, s>>>(p, ldx, codes, ldc, scale, (int)M, (int)K);
+    tokens_quantize_tiny_kernel<T><<<dim3((unsigned)((M + 63) / 64)), dim3(64), 0, s>>>(p, ldx, codes, ldc, scale, (int)M, (int)K);
   } else {
     const T* last = p + (M - 1) * ldx + K - E;
     if (aligned16(x) && K % E == 0 && ldx % E == 0)

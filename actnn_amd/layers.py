@@ -209,14 +209,17 @@ class QInt8Linear(nn.Linear):
 
     _held = None
 
+    def _version(self):
+        return None if self.weight.is_inference() else self.weight._version    # (inference tensors count no changes)
+
     def hold_weight(self):
         with torch.no_grad():
-            self._held = (self.weight, self.weight._version, *ext_tokens.quantize_tokens(self.weight))
+            self._held = (self.weight, self._version(), *ext_tokens.quantize_tokens(self.weight))
         return self
 
     def _weight_tokens(self):
         held = self._held
-        if held is not None and held[0] is self.weight and held[1] == self.weight._version:
+        if held is not None and held[0] is self.weight and held[1] == self._version():
             return held[2:]
         self._held = None
         return ext_tokens.quantize_tokens(self.weight)

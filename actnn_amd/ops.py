@@ -7,7 +7,7 @@ import math
 
 import torch
 import torch.nn.functional as F
-from torch.autograd.function import Function
+from torch.autograd.function import Function, once_differentiable
 from torch.nn.modules.utils import _pair, _single, _triple
 
 from .conf import config
@@ -560,6 +560,7 @@ class int8_linear(Function):
         return output
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad_output):
         codes, scale, weight = ctx.saved_tensors
         go = grad_output.reshape(-1, grad_output.shape[-1])
@@ -903,6 +904,7 @@ class group_norm(Function):
         return output
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad_output):
         codes, scale, input, weight, bias, mean, rstd = ctx.saved_tensors
         grad_input, grad_weight, grad_bias = ext_backward_func.hip_group_norm_backward(

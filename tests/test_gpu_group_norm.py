@@ -225,6 +225,29 @@ def test_nothing_behind_the_tensors_is_written(lib):
 
 
 @pytest.mark.gpu
+def test_offsets_past_32_bits():
+    # 2.2e9 values in one sample, and in many: the last group, the last sample are what they are by themselves
+    x = torch.zeros(1, 6000, 6000, 64, dtype=torch.bfloat16, device=DEV).permute(0, 3, 1, 2)
+    last = torch.randn(1, 8, 6000, 6000, device=DEV).bfloat16()
+    x[:, 56:] = last
+    y, mean, rstd, codes, scale = bf.hip_group_norm_forward(x, 8, None, None, 1e-5, "silu", keep=True)
+    v = last.double()
+    m, var = v.mean(), v.var(unbiased=False)
+    assert abs(mean[0, 7].item() - m.item()) < 1e-5 and abs(rstd[0, 7].item() - (var + 1e-5).rsqrt().item()) < 1e-5
+    z = (v[0, :, -3:] - m) * (var + 1e-5).rsqrt()
+    exact = z * torch.sigmoid(z)
+    assert ((y[0, 56:, -3:].double() - exact).abs() <= 2.0 ** -8 * exact.abs() + 1e-4).all() and not y[:, :56].any()
+    assert torch.equal(codes[0, 56:, -3:].cpu().double(), oracle.kept(last, 1)[0][0, :, -3:])
+    dx, _, _ = bf.hip_group_norm_backward(y, codes, scale, 8, None, None, mean, rstd, "silu")
+    assert not dx[:, :56].any() and dx[0, 56:, -1].abs().max() > 0.1
+    del dx, y, codes, v, last, z, x
+    x = torch.zeros(8400, 16, 16, 1024, dtype=torch.float16, device=DEV).permute(0, 3, 1, 2)
+    x[-1] = torch.randn(1024, 16, 16, device=DEV)
+    y = bf.hip_group_norm_forward(x, 32, None, None, 1e-5)[0]
+    assert torch.equal(y[-1:], bf.hip_group_norm_forward(x[-1:], 32, None, None, 1e-5)[0]) and not y[:-1].any()
+
+
+@pytest.mark.gpu
 def test_empty_tensors():
     for shape in ((0, 8, 4, 4), (2, 8, 0, 4)):
         x = torch.zeros(shape, device=DEV)

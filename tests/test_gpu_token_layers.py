@@ -133,6 +133,25 @@ def test_held_weights():
 
 
 @pytest.mark.gpu
+def test_weights_held_in_inference_mode():
+    with torch.inference_mode():
+        layer = layers.QInt8Linear(64, 8).to(DEV)
+        x = torch.randn(3, 64, device=DEV)
+        want = layer(x)
+        assert torch.equal(layer.hold_weight()(x), want) and layer._held is not None
+
+
+@pytest.mark.gpu
+def test_second_derivatives_are_refused():
+    layer, norm = layers.QInt8Linear(16, 8).to(DEV), layers.QGroupNorm(2, 16).to(DEV)
+    x = torch.randn(4, 16, device=DEV, requires_grad=True)
+    for f in (lambda: layer(x), lambda: norm(x)):
+        (g,) = torch.autograd.grad(f().square().sum(), x, create_graph=True)
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            g.sum().backward()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("compress", [True, False])
 @pytest.mark.parametrize("shape,groups", [((3, 24, 10, 6), 4), ((2, 33, 7), 11), ((5, 16), 2), ((2, 8, 3, 4, 5), 2)])

@@ -105,7 +105,7 @@ def test_rows_of_zeros_tiny_values_nan_and_infinity(K, dtype):
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_strides_offsets_and_leading_dimensions(dtype):
     base = make(40, 1024, dtype, 3).to(DEV)
-    for x in (base[:, 3:700], base[::3, :513], base[5:6, 1:], base.t()[:77], base[:1].expand(9, 1024), base.view(4, 10, 1024)[:, 2:5, 8:80],
+    for x in (base[:1, :3].expand(1000, 3), base[:1, 5:6].expand(70, 1), base[:, 3:700], base[::3, :513], base[5:6, 1:], base.t()[:77], base[:1].expand(9, 1024), base.view(4, 10, 1024)[:, 2:5, 8:80],
               base.view(2, 2, 10, 1024)[1:], base[0], base[:, 100:101], base[3:3]):
         codes, scale = tokens.quantize_tokens(x)
         check_codes(x, codes, scale)
@@ -130,6 +130,29 @@ def test_nothing_behind_the_rows_is_written():
     assert lib.actnn_tokens_dequantize(room.data_ptr(), 48, scale.data_ptr(), out.data_ptr(), 6, 37, 1,
                                        torch.cuda.current_stream().cuda_stream) == 0
     assert (out[6 * 37:] == 5).all()
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits():
+    # 2.4e9 values: the last rows are what they are by themselves, through every operator that walks over tokens
+    M, K, O = 300_000, 8192, 24
+    x = torch.zeros(M, K, dtype=torch.bfloat16, device=DEV)
+    tail = make(300, K, torch.bfloat16, 9).to(DEV)
+    x[-300:] = tail
+    codes, scale = tokens.quantize_tokens(x)
+    c, s = tokens.quantize_tokens(tail)
+    assert torch.equal(codes[-300:], c) and torch.equal(scale[-300:], s) and not scale[:-300].any() and not codes[M // 2].any()
+    del x
+    assert torch.equal(tokens.dequantize_tokens(codes, scale, torch.bfloat16)[-300:], tokens.dequantize_tokens(c, s, torch.bfloat16))
+    wcodes, wscale = tokens.quantize_tokens(torch.randn(O, K, device=DEV))
+    y = tokens.matmul_tokens(codes, scale, wcodes, wscale)
+    assert torch.equal(y[-300:], tokens.matmul_tokens(c, s, wcodes, wscale)) and not y[:-300].any()
+    g = torch.zeros(M, O, dtype=torch.bfloat16, device=DEV)
+    g[-300:] = torch.randn(300, O, device=DEV)
+    gw = tokens.linear_tokens_grad_weight(g, codes, scale, torch.float32)
+    values = (c.float() * s[:, None]).bfloat16().double()
+    exact, size = g[-300:].double().t() @ values, g[-300:].double().abs().t() @ values.abs()
+    assert ((gw.double() - exact).abs() <= 2.0 ** -23 * 302 * size).all()
 
 
 @pytest.mark.gpu

@@ -11,8 +11,8 @@
 //     straight into the operand registers of v_mfma_i32_16x16x64_i8, the waves of a block share the features of the same
 //     channels and add their sums in LDS.
 //   * tiles of 64, 128 or 256 channels by as many tokens, for everything else: v_mfma_i32_32x32x32_i8 out of LDS.  Four buffers of
-//     64 features; both operands go from global memory straight into LDS (global_load_lds, 16 bytes a lane), rows as they lie in
-//     memory, their four 16-byte chunks at chunk ^ (row / 4) % 4: 16 rows that are read together meet every bank once.
+//     64 or 128 features; both operands go from global memory straight into LDS (global_load_lds, 16 bytes a lane), rows as they
+//     lie in memory, their 16-byte chunks permuted so that 16 rows that are read together meet every bank once.
 //   * tiles that do not fill the chip take slices of the features; a second kernel adds the slices.
 // Rows and channels past the end are read from the last one and not stored; features past the end are read from the
 // step's first chunk and masked out of the weight's operand.
@@ -120,14 +120,15 @@ ACTNN_DEV void put_row(TY* to, int valid, const int (&sum)[V], float xs, const f
 // ------------------------------------------------------------------------------------------
 // Tiles.  Four waves, two by two; a wave has NA x NE fragments of 32 channels x 32 tokens.
 // ------------------------------------------------------------------------------------------
-// WHOLE: the features are whole steps.
-template <typename TY, int NA, int NE, bool WHOLE>
+// BK features a step; WHOLE: the features are whole steps.
+template <typename TY, int NA, int NE, int BK, bool WHOLE>
 __global__ __launch_bounds__(kThreads, 1) void tokens_tile_kernel(Product p, int slices, int steps_per_slice) {
-  constexpr int BO = 64 * NA, BT = 64 * NE, BK = 64, kBuffers = 4;
+  constexpr int BO = 64 * NA, BT = 64 * NE, kBuffers = 4, kBlocks = BK / 32;
+  constexpr int kChunks = BK / 16, kPieceRows = 64 / kChunks;         // 16-byte chunks of a row, rows of a direct load
   constexpr int kBuffer = (BO + BT) * BK;
-  constexpr int kGroup = NA * NE, kSlots = 2 * kGroup, kFragments = NA + NE;
+  constexpr int kGroup = NA * NE, kSlots = kBlocks * kGroup, kFragments = NA + NE;
   constexpr int kReads = (kFragments + kGroup - 1) / kGroup;          // fragment reads beside an MFMA
-  constexpr int kPieces = NA + NE;                                    // direct loads of a wave and step: 16 rows each
+  constexpr int kPieces = kBuffer / (kThreads * 16), kWeightPieces = BO * BK / (kThreads * 16);   // direct loads of a wave and step
   __shared__ __attribute__((aligned(1024))) uint8_t smem[kBuffers * kBuffer];
 
   const int lane = threadIdx.x & 63;
@@ -158,14 +159,18 @@ __global__ __launch_bounds__(kThreads, 1) void tokens_tile_kernel(Product p, int
   const uint32_t lds0 = lds_address(smem);
   const uint32_t lds_wave = __builtin_amdgcn_readfirstlane(lds0 + wave * 1024);
 
-  // ---- direct loads: piece j is 16 rows of the weight's tile or, behind those, of the tokens'
-  const int row_in = lane >> 2;
-  const int chunk = (lane & 3) ^ ((lane >> 4) & 3);
+  // Chunk c of row r lies at c ^ swizzle(r): 16 rows that are read together meet every bank once.
+  auto swizzle = [](int row) { return (row * kChunks / 16) & (kChunks - 1); };
+
+  // ---- direct loads: piece j is kPieceRows rows of the weight's tile or, behind those, of the tokens'; a wave's pieces
+  // are 4 kPieceRows rows apart, which leaves the swizzle as it is
+  const int row_in = lane / kChunks;
+  const int chunk = (lane % kChunks) ^ swizzle(kPieceRows * wave + row_in);
   uint32_t off[kPieces];
 #pragma unroll
   for (int i = 0; i < kPieces; ++i) {
-    const int row = 16 * (wave + 4 * i) + row_in;
-    if (i < NA) {
+    const int row = kPieceRows * (wave + 4 * i) + row_in;
+    if (i < kWeightPieces) {
       const int at = o0 + row < p.O ? row : p.O - 1 - o0;
       off[i] = (uint32_t)at * (uint32_t)p.ldw + (uint32_t)chunk * 16u;
     } else {
@@ -181,17 +186,16 @@ __global__ __launch_bounds__(kThreads, 1) void tokens_tile_kernel(Product p, int
     const int step = first + (t < steps ? t : steps - 1);
     uint32_t at = off[i];
     if constexpr (!WHOLE) {
-      if (step * 4 + chunk >= chunks) at -= (uint32_t)chunk * 16u;     // past the row's end: the step's first chunk
+      if (step * kChunks + chunk >= chunks) at -= (uint32_t)chunk * 16u;     // past the row's end: the step's first chunk
     }
-    const int8_t* base = (i < NA ? wp : xp) + (int64_t)step * BK;
+    const int8_t* base = (i < kWeightPieces ? wp : xp) + (int64_t)step * BK;
     load_rows(base, at, lds_wave + decltype(BUF)::value * kBuffer + i * 4096);
   };
 
   // ---- fragments: lane -> row lane % 32, features 32 kb + 16 (lane / 32) ..
-  const uint32_t in_row = (uint32_t)(lane & 31) * BK + (uint32_t)(((lane >> 5) ^ ((lane >> 2) & 3)) << 4);
+  const uint32_t in_row = (uint32_t)(lane & 31) * BK + (uint32_t)(((lane >> 5) ^ swizzle(lane & 31)) << 4);
   const uint32_t at_w = lds0 + (uint32_t)(wr * 32 * NA) * BK + in_row;
   const uint32_t at_x = lds0 + (uint32_t)(BO + wn * 32 * NE) * BK + in_row;
-  const uint32_t at_w2 = at_w ^ 32u, at_x2 = at_x ^ 32u;              // the second k-block
 
   i32x16 acc[NE][NA];
 #pragma unroll
@@ -212,28 +216,28 @@ __global__ __launch_bounds__(kThreads, 1) void tokens_tile_kernel(Product p, int
     constexpr int kb = decltype(KB)::value, f = decltype(F)::value;
     constexpr uint32_t buf = decltype(BUF)::value * kBuffer;
     if constexpr (f < NA) {
-      u32x4 v = lds_load16((kb ? at_w2 : at_w) + buf + f * 32 * BK);
+      u32x4 v = lds_load16((at_w ^ (kb << 5)) + buf + f * 32 * BK);
       if constexpr (decltype(TAIL)::value != 0) v = first_bytes(v, features - (t * BK + kb * 32 + (lane >> 5) * 16));
-      fw[kb][f] = v;
+      fw[kb & 1][f] = v;
     } else {
-      fx[kb][f - NA] = lds_load16((kb ? at_x2 : at_x) + buf + (f - NA) * 32 * BK);
+      fx[kb & 1][f - NA] = lds_load16((at_x ^ (kb << 5)) + buf + (f - NA) * 32 * BK);
     }
   };
   auto mma = [&](auto KB, int e, int a) {
-    constexpr int h = decltype(KB)::value;
+    constexpr int h = decltype(KB)::value & 1;
     acc[e][a] = __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(i32x4, fw[h][a]), __builtin_bit_cast(i32x4, fx[h][e]),
                                                       acc[e][a], 0, 0, 0);
   };
 
-  // Step t is multiplied out of buffer t % 4.  Between two barriers: the MFMAs of the second k-block of the step before (its
-  // fragments are in registers) and of the first of this one, the fragments of each k-block read beside the MFMAs of the
+  // Step t is multiplied out of buffer t % 4.  Between two barriers: the MFMAs of the last k-block of the step before (its
+  // fragments are in registers) and of all but the last of this one, the fragments of each k-block read beside the MFMAs of the
   // one before, and the direct loads of step t + 3 into the buffer whose last readers passed the barrier before.  The step
   // ends when the loads of step t + 1 have landed: those of two steps may be on their way.
   // (a direct load and what it takes stand beside MFMAs without fragment reads where there are any, half of them in either
   // group: about six instructions fit beside one)
-  constexpr bool kRoom = kGroup >= kFragments + kPieces;
+  constexpr bool kRoom = kBlocks == 2 && kGroup >= kFragments + kPieces;
   constexpr auto load_slot = [](int i) {
-    return !kRoom ? i * (kSlots / kPieces) : i < kPieces / 2 ? kFragments + 2 * i : kGroup + kFragments + 2 * (i - kPieces / 2);
+    return !kRoom ? i * kSlots / kPieces : i < kPieces / 2 ? kFragments + 2 * i : kGroup + kFragments + 2 * (i - kPieces / 2);
   };
   static_assert(load_slot(kPieces - 1) < kSlots, "every load has its place");
   constexpr int kLandedOne = waitcnt_all_but(2 * kPieces);
@@ -243,7 +247,7 @@ __global__ __launch_bounds__(kThreads, 1) void tokens_tile_kernel(Product p, int
     constexpr bool ahead = decltype(AHEAD)::value != 0;
     for_each<kSlots>([&](auto S) {
       constexpr int slot = decltype(S)::value, in = slot % kGroup;
-      mma(Const<1 - slot / kGroup>{}, in / NA, in % NA);
+      mma(Const<(slot / kGroup + 1) % 2>{}, in / NA, in % NA);              // (of the k-block before: kBlocks is even)
       for_each<kReads>([&](auto R) {
         constexpr int f = in * kReads + decltype(R)::value;
         if constexpr (f < kFragments) read_fragment(Const<buf>{}, Const<slot / kGroup>{}, Const<f>{}, TAIL, t);
@@ -485,44 +489,56 @@ __global__ __launch_bounds__(kThreads) void tokens_sum_slices_kernel(Product p, 
   }
 }
 
-// Which kernel: tile edge (0: few tokens) and slices of the features.
-struct Plan { int edge, slices, steps_per_slice; };
+// Which kernel - the tile, 0: few tokens - and slices of the features, of `steps` steps each: the cheapest by this estimate, us.
+// A step takes step_us for each round of blocks over the chip's 256 CUs, two thirds of it for half a round or less; the start and
+// the end of a block, the fetch of its code among them, `fixed`; slices a second launch of about 4.5, and their sums are written and read back at some 8 TB/s.
+// Measured, tile 64 by 64 features / 64 by 128 / 128 / 256, us: 256 x 4096 x 4096 (tokens, features, outputs) 12.2, 10.0, 18.9, 42;
+// 1024 x 4096 x 4096 36.1, 29.6, 27.9, 42.8; 8192 x 4096 x 4096 248, 205, 169, 125; 512 x 1024 x 2048 6.3, 6.6, 7.6, 18.8.
+struct Plan { int tile, slices, steps; };
+struct Tile { int edge, features; double fixed, step_us; };
+constexpr Tile kTiles[] = {{0, 1, 0.0, 0.0}, {64, 64, 3.0, 0.15}, {64, 128, 4.0, 0.25}, {128, 64, 5.0, 0.32}, {256, 64, 12.0, 0.88}};
 Plan plan_of(int64_t M, int64_t K, int64_t O) {
   if (M <= 64) return Plan{0, 1, 0};
-  constexpr int64_t kCUs = 256;
-  const int64_t steps = (K + 63) / 64;
-  auto tiles = [&](int64_t edge) { return ((M + edge - 1) / edge) * ((O + edge - 1) / edge); };
-  const int edge = tiles(256) >= kCUs ? 256 : tiles(128) >= kCUs ? 128 : 64;
-  // Slices: a step of a block takes 0.35 us for the smaller tiles; the second launch about 4.5, and the sums are written and
-  // read back at some 4 TB/s.
-  int64_t slices = 1;
-  auto cost_us = [&](int64_t n) {
-    return 0.35 * (double)((steps + n - 1) / n) + (n > 1 ? 4.5 + 8.0 * (double)n * (double)M * (double)O / 4.0e6 : 0.0);
-  };
-  for (int64_t n = 2; n * tiles(edge) <= 2 * kCUs && n <= 16 && n <= steps; n *= 2)
-    if (cost_us(n) < cost_us(slices)) slices = n;
-  const int64_t per = (steps + slices - 1) / slices;
-  return Plan{edge, (int)((steps + per - 1) / per), (int)per};
+  Plan best{0, 1, 0};
+  double least = 0.0;
+  for (int i = 1; i < 5; ++i) {
+    const Tile& t = kTiles[i];
+    const int64_t tiles = ((M + t.edge - 1) / t.edge) * ((O + t.edge - 1) / t.edge), steps = (K + t.features - 1) / t.features;
+    for (int64_t n = 1; n <= 16 && n <= steps && (n == 1 || n * tiles <= 512); n *= 2) {
+      const int64_t per = (steps + n - 1) / n;
+      const double rounds = tiles * n <= 128 ? 0.7 : (double)((tiles * n + 255) / 256);
+      const double us = t.fixed + t.step_us * rounds * (double)per +
+                        (n > 1 ? 4.5 + 8.0 * (double)n * (double)M * (double)O / 8.0e6 : 0.0);
+      if (best.tile == 0 || us < least) {
+        least = us;
+        best = Plan{i, (int)((steps + per - 1) / per), (int)per};
+      }
+    }
+  }
+  return best;
 }
 
-template <typename TY, int N> void launch_tiles(const Product& p, const Plan& plan, int64_t blocks, hipStream_t s) {
+template <typename TY, int I> void launch_tiles(const Product& p, const Plan& plan, int64_t blocks, hipStream_t s) {
+  constexpr int N = kTiles[I].edge / 64, BK = kTiles[I].features;
   const dim3 grid((unsigned)blocks), blk(kThreads);
-  if (p.K % 64 == 0) tokens_tile_kernel<TY, N, N, true><<<grid, blk, 0, s>>>(p, plan.slices, plan.steps_per_slice);
-  else tokens_tile_kernel<TY, N, N, false><<<grid, blk, 0, s>>>(p, plan.slices, plan.steps_per_slice);
+  if (p.K % BK == 0) tokens_tile_kernel<TY, N, N, BK, true><<<grid, blk, 0, s>>>(p, plan.slices, plan.steps);
+  else tokens_tile_kernel<TY, N, N, BK, false><<<grid, blk, 0, s>>>(p, plan.slices, plan.steps);
 }
-template <typename TY> void launch_edge(const Product& p, const Plan& plan, int64_t blocks, hipStream_t s) {
-  if (plan.edge == 256) launch_tiles<TY, 4>(p, plan, blocks, s);
-  else if (plan.edge == 128) launch_tiles<TY, 2>(p, plan, blocks, s);
-  else launch_tiles<TY, 1>(p, plan, blocks, s);
+template <typename TY> void launch_tile(const Product& p, const Plan& plan, int64_t blocks, hipStream_t s) {
+  switch (plan.tile) {
+    case 1: return launch_tiles<TY, 1>(p, plan, blocks, s);
+    case 2: return launch_tiles<TY, 2>(p, plan, blocks, s);
+    case 3: return launch_tiles<TY, 3>(p, plan, blocks, s);
+    default: return launch_tiles<TY, 4>(p, plan, blocks, s);
+  }
 }
-
 template <typename TY, int MT, int NT, int WAVES> void launch_few(const Product& p, hipStream_t s) {
   tokens_few_kernel<TY, MT, NT, WAVES><<<dim3((unsigned)((p.O + 16LL * NT - 1) / (16 * NT))), dim3(64 * WAVES), 0, s>>>(p);
 }
 
 template <typename TY> int product(const Product& p, void* workspace, int64_t workspace_bytes, hipStream_t s) {
   Plan plan = plan_of(p.M, p.K, p.O);
-  if (plan.edge == 0) {
+  if (plan.tile == 0) {
     // More channels to a block re-read the tokens less often, where 64 of them leave blocks for most of the chip; more waves to a
     // block keep more loads in flight, where each has features enough (us, 16 channels / 64: [24, 4096] -> 16384 23.8 / 16.0,
     // -> 4096 8.2 / 14.5; 4 waves / 16: [16, 1024] -> 4096 3.0 / 5.7, [32, 4096] -> 4096 by 16 channels 10.1 / 8.2).
@@ -537,16 +553,17 @@ template <typename TY> int product(const Product& p, void* workspace, int64_t wo
     ACTNN_RETURN_LAUNCH_STATUS();
   }
   const int64_t n = (int64_t)p.M * p.O;
-  if (plan.slices > 1 && (!workspace || workspace_bytes < 4 * n * plan.slices)) plan = Plan{plan.edge, 1, 0};
-  const int64_t blocks = (p.M + plan.edge - 1) / plan.edge * ((p.O + plan.edge - 1) / plan.edge) * plan.slices;
+  if (plan.slices > 1 && (!workspace || workspace_bytes < 4 * n * plan.slices)) plan = Plan{plan.tile, 1, 0};
+  const int64_t edge = kTiles[plan.tile].edge;
+  const int64_t blocks = (p.M + edge - 1) / edge * ((p.O + edge - 1) / edge) * plan.slices;
   if (blocks > 0x7fffffffLL) return ACTNN_EINVAL;
   if (plan.slices == 1) {
-    launch_edge<TY>(p, plan, blocks, s);
+    launch_tile<TY>(p, plan, blocks, s);
   } else {
     if (!aligned16(workspace)) return ACTNN_EALIGN;
     Product parts = p;
     parts.y = workspace;
-    launch_edge<int>(parts, plan, blocks, s);
+    launch_tile<int>(parts, plan, blocks, s);
     const int64_t sums = (n + kThreads - 1) / kThreads;
     tokens_sum_slices_kernel<TY><<<dim3((unsigned)(sums < 4096 ? sums : 4096)), dim3(kThreads), 0, s>>>(
         p, static_cast<const int*>(workspace), plan.slices);

@@ -40,10 +40,11 @@ def check(y, codes, scale, wcodes, wscale, bias, dtype):
     assert (err <= bound).all(), float((err / bound.clamp(min=1e-300)).max())
 
 
-# few tokens in one to four tiles of 16; tiles of 64 with and without slices, of 128 and of 256; odd everything
+# few tokens in one to four tiles of 16; tiles of 64 (by 64 and 128 features) with and without slices, of 128 and of 256; odd everything
 SHAPES = [(1, 1, 1), (1, 16, 16), (1, 4096, 300), (2, 100, 17), (3, 1003, 33), (15, 64, 64), (16, 65, 1), (17, 128, 130), (24, 4100, 257),
           (32, 31, 16), (33, 513, 100), (64, 1000, 1003), (65, 15, 3), (65, 8192, 70), (100, 16, 64), (128, 128, 128), (129, 129, 65),
-          (197, 1000, 1003), (70, 5000, 4), (300, 2000, 301), (1100, 257, 2100), (2048, 144, 2050), (2048, 200, 8192), (4100, 272, 4100), (66, 127, 20000)]
+          (197, 1000, 1003), (70, 5000, 4), (300, 2000, 301), (1100, 257, 2100), (2048, 144, 2050), (2048, 200, 8192), (4100, 272, 4100), (66, 127, 20000), (130, 2048, 2000),
+          (256, 2100, 4096), (100, 8200, 300)]
 
 
 @pytest.mark.gpu

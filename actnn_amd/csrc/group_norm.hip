@@ -10,7 +10,7 @@
 // everything that goes by channel stays in its registers, and sums are made per channel first and per group at the end.
 // Each direction is two passes over the data with a table of partial results between them: a block of the second pass adds up
 // the entries of its own groups before it starts.  The second pass takes the samples in the opposite order: the first one's last
-// samples are still in the caches.
+// samples are still in the caches.  [128, 56 * 56, 256] bf16 takes 333 us in both directions, 1.54 GB at 4.6 TB/s (a copy: 5.1).
 //
 // Small tensors are bound by the instructions: a kernel's code comes from the L2 at about a microsecond a kilobyte when it is
 // run once.  So small planes take one kernel instead of two, a block to a plane's chunk that reads it twice; loops over
@@ -27,6 +27,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWide = 1024;              // of the kernel that adds up the parameters' gradients
 constexpr int kRun = 32;                 // pixels summed about the same value
+constexpr int64_t kMostBlocks = 0xffffff;   // (a launch counts its work items in 32 bits)
 
 // How a tensor [N, pixels, C] in G groups is cut into blocks: `chunk` channels (`per` whole groups, or a part of one wider than
 // a block takes), `slice` pixels.
@@ -69,7 +70,8 @@ void cut_channels(Cut& c, int E, int least) {
     if (per > c.G) per = c.G;
     const int chunks = (c.G + per - 1) / per;            // as many groups to each
     per = (c.G + chunks - 1) / chunks;
-    if (per % unit && per + unit - per % unit <= c.G && (int64_t)(per + unit - per % unit) * c.width <= most) per += unit - per % unit;
+    const int up = per % unit ? unit - per % unit : 0;   // to whole units
+    if (per + up <= c.G && (int64_t)(per + up) * c.width <= most) per += up;
     c.per = per;
     c.parts = 1;
     c.chunk = per * c.width;
@@ -128,6 +130,7 @@ bool cut_once(Cut& c, int E) {
   const int64_t mine = (c.pixels + kThreads / once.cols - 1) / (kThreads / once.cols);
   if (mine > kFewPixels && (mine > kSomePixels || (int64_t)c.N * once.chunks < 256)) return false;
   cut_pixels(once, 1);
+  if (once.blocks() > kMostBlocks) return false;
   c = once;
   return true;
 }
@@ -546,7 +549,9 @@ __global__ __launch_bounds__(kThreads) void group_norm_apply_kernel(const T* __r
     ChannelStats<T> stats;
     walk.run(get, [&](const u32x4& raw, int, int i) { stats.add(raw, i, walk.mine - 1); });
     walk.begin(c, b, get);
-    block_stats(stats, c, b, [&](int g, const Partial& v) { s_group[g] = group_of<T, KEEP>(f, v, (int64_t)b.n * c.G + b.g0 + g, true); });
+    block_stats(stats, c, b, [&](int g, const Partial& v) {
+      s_group[g] = group_of<T, KEEP>(f, v, (int64_t)b.n * c.G + b.g0 + g, true);
+    });
   } else {
     const Team team(b.groups);
     for (int g = team.first; g < b.groups; g += team.step) {
@@ -657,7 +662,8 @@ template <typename T, bool WHOLE, bool SILU, bool CODES> struct Gradient {
       second[e] = seconds[g] * rstd;
     });
   }
-  ACTNN_DEV void put(T* dx, const Slope<T, WHOLE, SILU, CODES>& slope, const typename Slope<T, WHOLE, SILU, CODES>::Raw& r, int valid) const {
+  typedef Slope<T, WHOLE, SILU, CODES> SlopeT;
+  ACTNN_DEV void put(T* dx, const SlopeT& slope, const typename SlopeT::Raw& r, int valid) const {
     float n[E], dz[E];
     slope.values(r, n, dz);
 #pragma unroll
@@ -854,8 +860,8 @@ int check(int64_t N, int64_t C, int64_t P, int64_t G, int dtype) {
 }
 int64_t forward_bytes(const Cut& c) { return (int64_t)c.N * c.G * c.slots() * (int64_t)sizeof(Partial); }
 int64_t backward_bytes(const Cut& c) { return (int64_t)c.N * c.slices * 2 * c.C * 4; }
-// (the block's number and the table's rows are 32-bit)
-bool too_many(const Cut& c) { return c.blocks() > 0x7fffffffLL || (int64_t)c.N * c.slices > 0x7fffff00LL; }
+// (the table's rows are 32-bit)
+bool too_many(const Cut& c) { return c.blocks() > kMostBlocks || (int64_t)c.N * c.slices > 0x7fffff00LL; }
 
 }  // namespace
 }  // namespace actnn

@@ -7,9 +7,9 @@
 //
 // The codes are exactly that: no rounding of the arithmetic moves one across a half.  127 |x| / top can only lie exactly
 // on a half or at least 1 / (254 X) of its own size from it, X being the significand of x as a whole number: 2^-19 for
-// fp16, 2^-16 for bf16, 2^-32 for fp32.  So the factor 127 / top is taken larger by a share below that distance and above the errors of
-// the factor, the product and the sum: a half is then always rounded up, and nothing below it is.  16-bit types compute
-// in fp32 (factor larger by 2^-21, errors below 2^-22), fp32 values in fp64 (2^-45, 2^-50).
+// fp16, 2^-16 for bf16, 2^-32 for fp32.  So the factor 127 / top is taken larger by a share below that distance and above the
+// errors of the factor, the product and the sum: a half is then always rounded up, and nothing below it is.  16-bit types
+// compute in fp32 (factor larger by 2^-21, errors below 2^-22), fp32 values in fp64 (2^-45, 2^-50).
 #pragma once
 
 #include "device_utils.h"
@@ -116,7 +116,8 @@ template <typename T> ACTNN_DEV u32x4 narrow(const T* p, const float (&f)[8]) { 
 // the packed codes of a vector: one word of four for fp32, two words for 16-bit types
 template <typename T> struct CodeWords { typedef u32x2 type; };
 template <> struct CodeWords<float> { typedef uint32_t type; };
-template <typename T> ACTNN_DEV typename CodeWords<T>::type codes_of(const Coder<T>& coder, const float (&f)[kVector<T>], uint32_t keep) {
+template <typename T>
+ACTNN_DEV typename CodeWords<T>::type codes_of(const Coder<T>& coder, const float (&f)[kVector<T>], uint32_t keep) {
   if constexpr (sizeof(T) == 4) {
     return pack_codes(coder.code(f[0]), coder.code(f[1]), coder.code(f[2]), coder.code(f[3])) & keep;
   } else {
@@ -138,8 +139,12 @@ ACTNN_DEV void code_values(u32x2 v, float (&f)[8]) {
 // behind the exponent of 1024, and a mixed multiply-add rounds their product with the fp32 scale), two for bf16 (to 32 bits
 // first).  Two and two and a half instructions a value.
 template <typename T, int J> ACTNN_DEV uint32_t code_pair(uint32_t word, float scale);
-template <> ACTNN_DEV uint32_t code_pair<bf16_t, 0>(uint32_t w, float s) { return pack_bf16x2(code_value<0>(w) * s, code_value<1>(w) * s); }
-template <> ACTNN_DEV uint32_t code_pair<bf16_t, 1>(uint32_t w, float s) { return pack_bf16x2(code_value<2>(w) * s, code_value<3>(w) * s); }
+template <> ACTNN_DEV uint32_t code_pair<bf16_t, 0>(uint32_t w, float s) {
+  return pack_bf16x2(code_value<0>(w) * s, code_value<1>(w) * s);
+}
+template <> ACTNN_DEV uint32_t code_pair<bf16_t, 1>(uint32_t w, float s) {
+  return pack_bf16x2(code_value<2>(w) * s, code_value<3>(w) * s);
+}
 typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
 template <int J> ACTNN_DEV uint32_t half_code_pair(uint32_t w, float s) {
   const f16x2_t off = {(_Float16)-1152.0f, (_Float16)-1152.0f};

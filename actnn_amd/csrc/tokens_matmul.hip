@@ -18,6 +18,7 @@
 // step's first chunk and masked out of the weight's operand.
 #include <type_traits>
 
+#include "matrix_tiles.h"
 #include "token_math.h"
 
 namespace actnn {
@@ -29,41 +30,7 @@ typedef int i32x16 __attribute__((ext_vector_type(16)));
 constexpr int kThreads = 256;
 constexpr int64_t kMostFeatures = 131071;               // the integer sum of so many products fits 32 bits
 constexpr int64_t kMostStride = 0x7fffff;               // 256 rows of so many bytes stay below 2 GiB
-
-template <int N> struct Const { static constexpr int value = N; };
-template <int N, typename F> ACTNN_DEV void for_each(F&& f) {
-  if constexpr (N > 0) {
-    for_each<N - 1>(f);
-    f(Const<N - 1>{});
-  }
-}
-
-typedef __attribute__((address_space(3))) uint8_t* lds_ptr_t;
-ACTNN_DEV uint32_t lds_address(const void* p) {
-  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint8_t*)p;
-}
-ACTNN_DEV u32x4 lds_load16(uint32_t address) {
-  return *reinterpret_cast<const __attribute__((address_space(3))) u32x4*>((lds_ptr_t)(uintptr_t)address);
-}
-
-ACTNN_DEV void lds_store16(uint32_t address, u32x4 v) {
-  *reinterpret_cast<__attribute__((address_space(3))) u32x4*>((lds_ptr_t)(uintptr_t)address) = v;
-}
-// what s_waitcnt takes to wait for LDS and for all but the last n loads
-constexpr int waitcnt_all_but(int n) { return (n & 15) | 7 << 4 | (n >> 4) << 14; }
-// 16 bytes a lane from a base that the wave shares, plus the lane's offset, to LDS: lane l's at lds + 16 l (asynchronous)
-#pragma clang diagnostic push
-#pragma clang diagnostic ignored "-Winline-asm"
-ACTNN_DEV void load_rows(const int8_t* base, uint32_t lane_bytes, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(lds), "v"(lane_bytes), "s"(base) : "memory", "m0");
-}
-#pragma clang diagnostic pop
-// between writes and reads of the same wave: LDS operations of a wave complete in order
-ACTNN_DEV void wave_lds_fence() {
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-}
+constexpr int64_t kMostOutputs = 0x3ffffff;             // 16 of them to a block of up to 1024 threads
 
 // the first `valid` of 16 bytes, the others 0
 ACTNN_DEV u32x4 first_bytes(u32x4 v, int valid) {
@@ -119,6 +86,11 @@ ACTNN_DEV void put_row(TY* to, int valid, const int (&sum)[V], float xs, const f
 
 // ------------------------------------------------------------------------------------------
 // Tiles.  Four waves, two by two; a wave has NA x NE fragments of 32 channels x 32 tokens.
+//
+// Bound by the matrix pipes and by what reaches them: a wave of the largest tile holds 128 x 128 sums in its 256 accumulation
+// registers, so that a byte read from LDS meets 64 products.  [8192, 4096] x [4096, 4096] takes 125 to 130 us, 2.1 to 2.2 POPS (the
+// library's product of such matrices in bf16: 1.2; the pipes alone, fed from registers, reach 3.2 on such codes, 4.4 on zeros:
+// the clock follows the power).  When it took 136 us, 113 remained without the loads into LDS and 87 without the reads from it.
 // ------------------------------------------------------------------------------------------
 // BK features a step; WHOLE: the features are whole steps.
 template <typename TY, int NA, int NE, int BK, bool WHOLE>
@@ -216,11 +188,11 @@ __global__ __launch_bounds__(kThreads, 1) void tokens_tile_kernel(Product p, int
     constexpr int kb = decltype(KB)::value, f = decltype(F)::value;
     constexpr uint32_t buf = decltype(BUF)::value * kBuffer;
     if constexpr (f < NA) {
-      u32x4 v = lds_load16((at_w ^ (kb << 5)) + buf + f * 32 * BK);
+      u32x4 v = lds_load<u32x4>((at_w ^ (kb << 5)) + buf + f * 32 * BK);
       if constexpr (decltype(TAIL)::value != 0) v = first_bytes(v, features - (t * BK + kb * 32 + (lane >> 5) * 16));
       fw[kb & 1][f] = v;
     } else {
-      fx[kb & 1][f - NA] = lds_load16((at_x ^ (kb << 5)) + buf + (f - NA) * 32 * BK);
+      fx[kb & 1][f - NA] = lds_load<u32x4>((at_x ^ (kb << 5)) + buf + (f - NA) * 32 * BK);
     }
   };
   auto mma = [&](auto KB, int e, int a) {
@@ -312,7 +284,7 @@ __global__ __launch_bounds__(kThreads, 1) void tokens_tile_kernel(Product p, int
     for (int a = 0; a < NA; ++a)
 #pragma unroll
       for (int q = 0; q < 4; ++q)
-        lds_store16(slab + (uint32_t)((lane & 31) * kPitch + 4 * (32 * a + 8 * q + 4 * (lane >> 5))),
+        lds_store(slab + (uint32_t)((lane & 31) * kPitch + 4 * (32 * a + 8 * q + 4 * (lane >> 5))),
                     (u32x4){(uint32_t)acc[e][a][4 * q], (uint32_t)acc[e][a][4 * q + 1], (uint32_t)acc[e][a][4 * q + 2],
                             (uint32_t)acc[e][a][4 * q + 3]});
     wave_lds_fence();
@@ -323,7 +295,7 @@ __global__ __launch_bounds__(kThreads, 1) void tokens_tile_kernel(Product p, int
       int sum[V];
 #pragma unroll
       for (int i = 0; i < V; i += 4) {
-        const u32x4 v = lds_load16(at + 4 * i);
+        const u32x4 v = lds_load<u32x4>(at + 4 * i);
         sum[i] = (int)v.x; sum[i + 1] = (int)v.y; sum[i + 2] = (int)v.z; sum[i + 3] = (int)v.w;
       }
       put_row<TY>(out + token * p.O, token < p.M ? valid : 0, sum, xs[j], ws, bias);
@@ -333,7 +305,8 @@ __global__ __launch_bounds__(kThreads, 1) void tokens_tile_kernel(Product p, int
 }
 
 // ------------------------------------------------------------------------------------------
-// Few tokens: 16 NT channels a block, MT tiles of 16 tokens; the waves share the features, a run of pieces of 64 each.
+// Few tokens: 16 NT channels a block, MT tiles of 16 tokens; the waves share the features, a run of pieces of 64 each.  Bound by
+// the weight, which is read once: [24, 4096] -> 16384 takes 16.0 us beside its quantisation, 67 MB at 4.2 TB/s.
 // ------------------------------------------------------------------------------------------
 template <typename TY, int MT, int NT, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void tokens_few_kernel(Product p) {
@@ -374,7 +347,8 @@ __global__ __launch_bounds__(64 * WAVES) void tokens_few_kernel(Product p) {
         const u32x4 w = left < 16 ? first_bytes(fw[j][i], left) : fw[j][i];
 #pragma unroll
         for (int t = 0; t < MT; ++t)
-          acc[i][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, w), __builtin_bit_cast(i32x4, fx[j][t]), acc[i][t], 0, 0, 0);
+          acc[i][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, w), __builtin_bit_cast(i32x4, fx[j][t]),
+                                                            acc[i][t], 0, 0, 0);
       }
     }
   }
@@ -398,7 +372,8 @@ __global__ __launch_bounds__(64 * WAVES) void tokens_few_kernel(Product p) {
 
 // ------------------------------------------------------------------------------------------
 // One to four tokens in full precision: every block turns them into codes for itself, in LDS, while its first pieces of the
-// weight are on their way; a launch and the wait between two are saved (one bf16 token x [4096, 4096]: 9.7 us by two kernels).
+// weight are on their way; a launch and the wait between two are saved (one bf16 token x [4096, 4096]: 6.5 us, 9.7 by two
+// kernels; its 16.8 MB of codes come at 2.6 TB/s, bound by the latencies of the start).
 // ------------------------------------------------------------------------------------------
 constexpr int kFused = 4;
 constexpr int kFusedFeatures = 16384;
@@ -490,18 +465,20 @@ __global__ __launch_bounds__(kThreads) void tokens_sum_slices_kernel(Product p, 
 }
 
 // Which kernel - the tile, 0: few tokens - and slices of the features, of `steps` steps each: the cheapest by this estimate, us.
-// A step takes step_us for each round of blocks over the chip's 256 CUs, two thirds of it for half a round or less; the start and
-// the end of a block, the fetch of its code among them, `fixed`; slices a second launch of about 4.5, and their sums are written and read back at some 8 TB/s.
-// Measured, tile 64 by 64 features / 64 by 128 / 128 / 256, us: 256 x 4096 x 4096 (tokens, features, outputs) 12.2, 10.0, 18.9, 42;
-// 1024 x 4096 x 4096 36.1, 29.6, 27.9, 42.8; 8192 x 4096 x 4096 248, 205, 169, 125; 512 x 1024 x 2048 6.3, 6.6, 7.6, 18.8.
+// A step takes step_us for each round of blocks over the chip's 256 CUs, 0.7 of it for half a round or less; the start and the
+// end of a block, the fetch of its code among them, `fixed`; slices a second launch of about 4.5, and their sums are written and
+// read back at some 8 TB/s.  Measured, tile 64 by 64 features / 64 by 128 / 128 / 256, us: 256 x 4096 x 4096 (tokens, features,
+// outputs) 12.2, 10.0, 18.9, 42; 1024 x 4096 x 4096 36.1, 29.6, 27.9, 42.8; 8192 x 4096 x 4096 248, 205, 169, 125;
+// 512 x 1024 x 2048 6.3, 6.6, 7.6, 18.8.
 struct Plan { int tile, slices, steps; };
 struct Tile { int edge, features; double fixed, step_us; };
-constexpr Tile kTiles[] = {{0, 1, 0.0, 0.0}, {64, 64, 3.0, 0.15}, {64, 128, 4.0, 0.25}, {128, 64, 5.0, 0.32}, {256, 64, 12.0, 0.88}};
+constexpr Tile kTiles[] = {{0, 1, 0.0, 0.0}, {64, 64, 3.0, 0.15}, {64, 128, 4.0, 0.25}, {128, 64, 5.0, 0.32},
+                           {256, 64, 12.0, 0.88}};
 Plan plan_of(int64_t M, int64_t K, int64_t O) {
   if (M <= 64) return Plan{0, 1, 0};
   Plan best{0, 1, 0};
   double least = 0.0;
-  for (int i = 1; i < 5; ++i) {
+  for (int i = 1; i < (int)(sizeof(kTiles) / sizeof(kTiles[0])); ++i) {
     const Tile& t = kTiles[i];
     const int64_t tiles = ((M + t.edge - 1) / t.edge) * ((O + t.edge - 1) / t.edge), steps = (K + t.features - 1) / t.features;
     for (int64_t n = 1; n <= 16 && n <= steps && (n == 1 || n * tiles <= 512); n *= 2) {
@@ -556,7 +533,7 @@ template <typename TY> int product(const Product& p, void* workspace, int64_t wo
   if (plan.slices > 1 && (!workspace || workspace_bytes < 4 * n * plan.slices)) plan = Plan{plan.tile, 1, 0};
   const int64_t edge = kTiles[plan.tile].edge;
   const int64_t blocks = (p.M + edge - 1) / edge * ((p.O + edge - 1) / edge) * plan.slices;
-  if (blocks > 0x7fffffffLL) return ACTNN_EINVAL;
+  if (blocks > kMostBlocks) return ACTNN_EINVAL;
   if (plan.slices == 1) {
     launch_tile<TY>(p, plan, blocks, s);
   } else {
@@ -576,7 +553,7 @@ template <typename TY> int product(const Product& p, void* workspace, int64_t wo
 
 extern "C" int64_t actnn_tokens_matmul_workspace_bytes(int64_t M, int64_t K, int64_t O) {
   using namespace actnn;
-  if (M < 1 || K < 1 || O < 1 || M > 0x7fffff00LL || O > 0x7fffff00LL || K > kMostFeatures) return 0;
+  if (M < 1 || K < 1 || O < 1 || M > 0x7fffff00LL || O > kMostOutputs || K > kMostFeatures) return 0;
   const Plan plan = plan_of(M, K, O);
   return plan.slices > 1 ? 4 * M * O * plan.slices : 0;
 }
@@ -585,7 +562,7 @@ extern "C" int actnn_tokens_matmul(const int8_t* codes, int64_t ldc, const float
                                    int64_t ldw, const float* weight_scale, const float* bias, void* out, int64_t M,
                                    int64_t K, int64_t O, int dtype, void* workspace, int64_t workspace_bytes, void* stream) {
   using namespace actnn;
-  if (M < 0 || O < 0 || K < 1 || K > kMostFeatures || M > 0x7fffff00LL || O > 0x7fffff00LL) return ACTNN_EINVAL;
+  if (M < 0 || O < 0 || K < 1 || K > kMostFeatures || M > 0x7fffff00LL || O > kMostOutputs) return ACTNN_EINVAL;
   if (ldc < K || ldc % 16 || ldc > kMostStride || ldw < K || ldw % 16 || ldw > kMostStride) return ACTNN_EINVAL;
   if (dtype != ACTNN_F32 && dtype != ACTNN_F16 && dtype != ACTNN_BF16) return ACTNN_EDTYPE;
   if (M == 0 || O == 0) return ACTNN_OK;
@@ -612,7 +589,7 @@ extern "C" int actnn_tokens_linear_few(const void* data, int64_t ld, const int8_
                                        const float* weight_scale, const float* bias, void* out, int64_t M, int64_t K, int64_t O,
                                        int dtype, void* stream) {
   using namespace actnn;
-  if (M < 0 || M > kFused || K < 1 || K > kFusedFeatures || O < 0 || O > 0x7fffff00LL || ld < 0) return ACTNN_EINVAL;
+  if (M < 0 || M > kFused || K < 1 || K > kFusedFeatures || O < 0 || O > kMostOutputs || ld < 0) return ACTNN_EINVAL;
   if (ldw < K || ldw % 16 || ldw > kMostStride) return ACTNN_EINVAL;
   if (dtype != ACTNN_F32 && dtype != ACTNN_F16 && dtype != ACTNN_BF16) return ACTNN_EDTYPE;
   const int64_t vector = dtype == ACTNN_F32 ? 4 : 8;

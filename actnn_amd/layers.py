@@ -205,7 +205,8 @@ class QInt8Linear(nn.Linear):
     pass and its gradient is that of the kept values.
 
     A layer that only answers rounds its weight once: `hold_weight()`, to be called again after the weight has been replaced
-    (changes in place, load_state_dict, .to() and train() are noticed and end the hold)."""
+    (changes in place, load_state_dict, .to() and train() are noticed and end the hold; what is written past autograd, through
+    `weight.data` or into inference tensors, is not)."""
 
     _held = None
 

@@ -522,7 +522,7 @@ int actnn_tokens_dequantize(const int8_t* codes, int64_t ldc, const float* scale
                             int dtype, void* stream);
 /* out[M, O] (contiguous, dtype, at any element address) = scale[m] * weight_scale[o] * sum_k codes[m, k] * weight_codes[o, k]
  * + bias[o] (fp32 or null): tokens times a weight kept as tokens itself, one scale for each of its O rows.  The sum is exact
- * (K <= 131071); strides up to 2^23 - 1 bytes.  Shapes that fill the chip only when their sums are split want a
+ * (K <= 131071); strides up to 2^23 - 1 bytes, O < 2^26.  Shapes that fill the chip only when their sums are split want a
  * workspace of _workspace_bytes (0: none; without one the call is slower, its results the same). */
 int64_t actnn_tokens_matmul_workspace_bytes(int64_t M, int64_t K, int64_t O);
 int actnn_tokens_matmul(const int8_t* codes, int64_t ldc, const float* scale, const int8_t* weight_codes, int64_t ldw,

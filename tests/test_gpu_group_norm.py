@@ -328,5 +328,6 @@ def test_c_abi_refuses_bad_sizes(lib):
     at = [16, None, None, 16, 16, 16, None, None]
     assert f(*at, 2, 64, 100, 8, 1e-5, 0, 2, 16, 8, None) == -1               # workspace too small
     assert f(*at, 2, 64, 100, 8, 1e-5, 0, 2, 8, 1 << 20, None) == -4
+    assert f(*at, 0x7fffff, 4096, 1, 32, 1e-5, 0, 2, 16, 1 << 60, None) == -1 # more blocks than a launch takes
     assert g(*[None] * 11, 2, 64, 100, 8, 0, 2, None, 0, None) == -1
     assert g(*[None] * 11, 2, 64, 100, 8, 0, 9, None, 0, None) == -2

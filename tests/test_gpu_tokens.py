@@ -156,6 +156,18 @@ def test_offsets_past_32_bits():
 
 
 @pytest.mark.gpu
+def test_more_rows_than_a_row_of_blocks():
+    # (four rows to a block, and one)
+    for M, K in ((2 ** 26 + 5, 8), (2 ** 20 + 3, 2056)):
+        print(f"[tokens] {M}x{K}", flush=True)
+        x = make(1, K, torch.float16, K).to(DEV)
+        codes, scale = tokens.quantize_tokens(x.expand(M, K))
+        c, s = tokens.quantize_tokens(x)
+        assert (codes == c).all() and (scale == s).all()
+        assert (tokens.dequantize_tokens(codes, scale, torch.float16) == tokens.dequantize_tokens(c, s, torch.float16)).all()
+
+
+@pytest.mark.gpu
 def test_tokens_on_another_stream():
     x = make(512, 1024, torch.bfloat16, 2).to(DEV)
     side = torch.cuda.Stream()

@@ -164,6 +164,7 @@ def test_c_abi_refuses_bad_sizes(lib):
     assert f(None, 8, None, 16, None, None, 4, 8, 17, 1, 1, None, 0, None) == -1          # rows shorter than I
     assert f(None, 8, None, 24, None, None, 4, 8, 16, 1, 1, None, 0, None) == -1          # no multiple of 16
     assert f(None, 8, None, 16, None, None, 4, 8, 16, 1, 1, None, 0, None) == -1          # null pointers
+    assert f(16, 8, 16, 16, 16, 16, 1, 0x7fffff00, 16, 1, 1, None, 0, None) == -1         # more blocks than a launch takes
     assert f(16, 8, 16, 16, 16, 16, 0, 8, 16, 1, 1, None, 0, None) == -1                  # no tokens
     assert f(16, 1, 16, 16, 16, 16, 2, 1, 16, 1, 1, None, 0, None) == -1                  # below 16 bytes without room
     assert f(16, 8, 8, 16, 16, 16, 4, 8, 16, 1, 1, None, 0, None) == -4

@@ -178,6 +178,8 @@ def test_c_abi_refuses_bad_sizes(lib):
     assert f(None, 16, None, None, 16, None, None, None, 4, 17, 4, 0, None, 0, None) == -1       # rows shorter than K
     assert f(None, 24, None, None, 16, None, None, None, 4, 16, 4, 0, None, 0, None) == -1       # no multiple of 16
     assert f(None, 1 << 23, None, None, 16, None, None, None, 4, 16, 4, 0, None, 0, None) == -1  # stride
+    assert f(16, 16, 16, 16, 16, 16, None, 16, 4, 16, 1 << 26, 0, None, 0, None) == -1           # more blocks than a launch takes
+    assert f(16, 16, 16, 16, 16, 16, None, 16, 0x7fffff00, 16, 4, 0, None, 0, None) == -1
     assert f(None, 131072, None, None, 131072, None, None, None, 4, 131072, 4, 0, None, 0, None) == -1
     assert f(None, 16, None, None, 16, None, None, None, 4, 16, 4, 9, None, 0, None) == -2
     assert f(8, 16, 16, 16, 16, 16, None, 16, 4, 16, 4, 0, None, 0, None) == -4
@@ -186,6 +188,7 @@ def test_c_abi_refuses_bad_sizes(lib):
     assert few(None, 16, None, 16, None, None, None, 0, 16, 4, 0, None) == 0
     assert few(None, 16, None, 16, None, None, None, 5, 16, 4, 0, None) == -1                    # more tokens than it takes
     assert few(None, 18, None, 32, None, None, None, 1, 18, 4, 0, None) == -1                    # no whole vectors
+    assert few(16, 16, 16, 16, 16, None, 16, 1, 16, 1 << 26, 0, None) == -1
     assert few(None, 16400, None, 16400, None, None, None, 1, 16400, 4, 0, None) == -1
     assert few(None, 16, None, 16, None, None, None, 1, 16, 4, 7, None) == -2
     assert few(8, 16, 16, 16, 16, None, 16, 1, 16, 4, 0, None) == -4

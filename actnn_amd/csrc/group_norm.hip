@@ -8,8 +8,8 @@
 // Large tensors are bound by memory.  A pixel's channels are consecutive, a group's are not: blocks take whole groups side
 // by side (128 bytes of a pixel at least), a thread keeps the same 16 bytes of channels from pixel to pixel, so that
 // everything that goes by channel stays in its registers, and sums are made per channel first and per group at the end.
-// Each direction is two passes over the data with a table of partial results between them: a block of the second pass adds up
-// the entries of its own groups before it starts.  The second pass takes the samples in the opposite order: the first one's last
+// Each direction is two passes over the data with a table of partial results by group between them: a block of the second pass adds
+// up the entries of its own groups before it starts.  The second pass takes the samples in the opposite order: the first one's last
 // samples are still in the caches.  [128, 56 * 56, 256] bf16 takes 333 us in both directions, 1.54 GB at 4.6 TB/s (a copy: 5.1).
 //
 // Small tensors are bound by the instructions: a kernel's code comes from the L2 at about a microsecond a kilobyte when it is
@@ -121,14 +121,21 @@ Cut cut_of(int64_t N, int64_t C, int64_t pixels, int64_t G, int E) {
 
 // One kernel: a block to a sample's chunk of 8 vectors at least, where a thread has few pixels ([4, 16 * 16, 320] fp16 both
 // directions 24.9 us, by two kernels each 27.4) or the blocks fill the chip anyway ([64, 28 * 28, 256] bf16 45.9, 67.9; 64 blocks
-// of 32 pixels a thread, [16, 32 * 32, 256]: 47.7, 34.0).  False: the plane is too large, or a group wider than a block.
+// of 32 pixels a thread, [16, 32 * 32, 256]: 47.7, 34.0).  Few blocks with several pixels a thread take chunks of 4 vectors (C
+// entry points, 8 vectors / 4: [4, 16 * 16, 320] 25.2 / 20.7, [32, 22 * 22, 64] in 8 groups 30.6 / 22.7), where those have two
+// groups: a wave adds up a group (forward of one in [4, 16 * 16, 1280] 12.1 / 12.8).  False: the plane is too large, or a group
+// wider than a block.
 constexpr int kFewPixels = 16, kSomePixels = 64;
 bool cut_once(Cut& c, int E) {
   Cut once = c;
   cut_channels(once, E, 8);
   if (!once.per || c.pixels * c.C >> 30) return false;
   const int64_t mine = (c.pixels + kThreads / once.cols - 1) / (kThreads / once.cols);
-  if (mine > kFewPixels && (mine > kSomePixels || (int64_t)c.N * once.chunks < 256)) return false;
+  const bool few = (int64_t)c.N * once.chunks < 256;
+  if (mine > kFewPixels && (mine > kSomePixels || few)) return false;
+  Cut half = once;
+  cut_channels(half, E, 4);
+  if (mine >= 6 && few && half.per >= 2) once = half;
   cut_pixels(once, 1);
   if (once.blocks() > kMostBlocks) return false;
   c = once;
@@ -576,6 +583,8 @@ struct Backward {
   const float* scale;
   const float *weight, *bias, *mean, *rstd;
   float* sums;                           // [N][slices][2][C]: sum dz, sum dz n
+  float* group_sums;                     // [N][G][slots][2]: the same times the weight, over a group's channels (joining `sums`
+                                         // in the second pass instead: [2, 20 * 20, 4096] in one group 1081 us backward, 24)
   float *dweight, *dbias;
 };
 
@@ -697,6 +706,24 @@ ACTNN_DEV void block_sums(const ChannelSums<T>& mine, const Cut& c, const Place&
     if (team.lane == 0) emit(which, ch, v);
   }
 }
+// and over the channels of each group in the block, times the weight: emit(g, sum u, sum u n)
+template <typename F>
+ACTNN_DEV void block_group_sums(const float* plain, const float* by_n, const float* weight, const Cut& c, const Place& b, F emit) {
+  const int width = c.per ? c.width : b.channels;
+  const Team team(b.groups);
+  for (int g = team.first; g < b.groups; g += team.step) {
+    float first = 0.0f, second = 0.0f;
+    for (int in = team.lane; in < width; in += team.size) {
+      const int ch = g * width + in;
+      const float w = weight ? weight[b.c0 + ch] : 1.0f;
+      first = __builtin_fmaf(w, plain[ch], first);
+      second = __builtin_fmaf(w, by_n[ch], second);
+    }
+    first = team.sum(first);
+    second = team.sum(second);
+    if (team.lane == 0) emit(g, first, second);
+  }
+}
 
 template <typename T, bool WHOLE, bool SILU, bool CODES>
 __global__ __launch_bounds__(kThreads) void group_norm_backward_sums_kernel(const T* __restrict__ dy, const T* __restrict__ x,
@@ -711,8 +738,16 @@ __global__ __launch_bounds__(kThreads) void group_norm_backward_sums_kernel(cons
   slope.init(k, c, b);
   ChannelSums<T> sums;
   walk.run(get, [&](const typename SavedT::Raw& raw, int, int) { sums.add(slope, raw); });
+  __shared__ float s_total[2][kThreads * kVector<T>];
   block_sums(sums, c, b, [&](int which, int ch, float v) {
+    s_total[which][ch] = v;
     k.sums[(((int64_t)b.n * c.slices + b.slice) * 2 + which) * c.C + b.c0 + ch] = v;
+  });
+  __syncthreads();
+  block_group_sums(s_total[0], s_total[1], k.weight, c, b, [&](int g, float first, float second) {
+    float* to = k.group_sums + 2 * (((int64_t)b.n * c.G + b.g0 + g) * c.slots() + b.slice * c.parts + b.part);
+    to[0] = first;
+    to[1] = second;
   });
 }
 
@@ -730,25 +765,10 @@ __global__ __launch_bounds__(kThreads) void group_norm_backward_apply_kernel(con
   walk.begin(c, b, get);                                 // (before the sums are joined)
   Slope<T, WHOLE, SILU, CODES> slope;
   slope.init(k, c, b);
-  const Team team(b.groups);
   const float all = 1.0f / ((float)c.pixels * (float)c.width);
-  // a group's means of u and u n from its channels' sums, `rows` of them
-  auto means = [&](int rows, auto sum_of) {
-    for (int g = team.first; g < b.groups; g += team.step) {
-      float first = 0.0f, second = 0.0f;
-      each_entry(team, c, c.width, rows, [&](int j, int in) {
-        const int ch = g * c.width + in;
-        const float w = k.weight ? k.weight[b.g0 * c.width + ch] : 1.0f;
-        first = __builtin_fmaf(w, sum_of(j, 0, ch), first);
-        second = __builtin_fmaf(w, sum_of(j, 1, ch), second);
-      });
-      first = team.sum(first);
-      second = team.sum(second);
-      if (team.lane == 0) {
-        s_mean[0][g] = first * all;
-        s_mean[1][g] = second * all;
-      }
-    }
+  auto means = [&](int g, float first, float second) {
+    s_mean[0][g] = first * all;
+    s_mean[1][g] = second * all;
   };
   if constexpr (ONCE) {
     __shared__ float s_total[2][kThreads * E];
@@ -761,10 +781,20 @@ __global__ __launch_bounds__(kThreads) void group_norm_backward_apply_kernel(con
     });
     __syncthreads();
     if (!dx) return;
-    means(1, [&](int, int which, int ch) { return s_total[which][ch]; });
+    block_group_sums(s_total[0], s_total[1], k.weight, c, b, means);
   } else {
-    const float* sums = k.sums + (int64_t)b.n * c.slices * 2 * c.C + (int64_t)b.g0 * c.width;
-    means(c.slices, [&](int j, int which, int ch) { return sums[(int64_t)(2 * j + which) * c.C + ch]; });
+    const Team team(b.groups);
+    for (int g = team.first; g < b.groups; g += team.step) {
+      const float* from = k.group_sums + 2 * ((int64_t)b.n * c.G + b.g0 + g) * c.slots();
+      float first = 0.0f, second = 0.0f;
+      for (int i = team.lane; i < c.slots(); i += team.size) {
+        first += from[2 * i];
+        second += from[2 * i + 1];
+      }
+      first = team.sum(first);
+      second = team.sum(second);
+      if (team.lane == 0) means(g, first, second);
+    }
   }
   __syncthreads();
   Gradient<T, WHOLE, SILU, CODES> gradient;
@@ -859,7 +889,7 @@ int check(int64_t N, int64_t C, int64_t P, int64_t G, int dtype) {
   return ACTNN_OK;
 }
 int64_t forward_bytes(const Cut& c) { return (int64_t)c.N * c.G * c.slots() * (int64_t)sizeof(Partial); }
-int64_t backward_bytes(const Cut& c) { return (int64_t)c.N * c.slices * 2 * c.C * 4; }
+int64_t backward_bytes(const Cut& c) { return 8 * ((int64_t)c.N * c.slices * c.C + (int64_t)c.N * c.G * c.slots()); }
 // (the table's rows are 32-bit)
 bool too_many(const Cut& c) { return c.blocks() > kMostBlocks || (int64_t)c.N * c.slices > 0x7fffff00LL; }
 
@@ -912,7 +942,8 @@ extern "C" int actnn_group_norm_backward(const void* dy, const int8_t* codes, co
     return ACTNN_EALIGN;
   const Cut c = cut_of(N, C, pixels, groups, dtype == ACTNN_F32 ? 4 : 8);
   if (workspace_bytes < backward_bytes(c) || too_many(c)) return ACTNN_EINVAL;
-  const Backward k{codes, scale, weight, bias, mean, rstd, static_cast<float*>(workspace), dweight, dbias};
+  float* sums = static_cast<float*>(workspace);
+  const Backward k{codes, scale, weight, bias, mean, rstd, sums, sums + 2 * (int64_t)c.N * c.slices * c.C, dweight, dbias};
   hipStream_t s = static_cast<hipStream_t>(stream);
   const bool silu = activation == kSilu;
   if (dtype == ACTNN_F32) return backward<float>(dy, codes ? nullptr : x, dx, k, c, silu, s);

@@ -53,8 +53,19 @@ bool whole_vectors(const Cut& c, int E) {
 
 int gcd(int a, int b) { return b ? gcd(b, a % b) : a; }
 
-// A chunk of whole groups, ending with a vector where it can, of `least` vectors where there are as many channels.
-void cut_channels(Cut& c, int E, int least) {
+// The groups whose channels end with a line of memory (128 bytes) of every pixel, or 0 where those are more than 128 vectors; where
+// the pixels do not begin with lines, all groups.  Blocks that share lines write parts of them, mostly from different XCDs: chunks
+// like these and before, both directions, us: [54, 35 * 35, 768] in 32 groups 166, 220; [28, 61 * 81, 366] in 6 169, 208;
+// [56, 30 * 33, 504] in 24 90, 102.
+constexpr int kWidest = 128;
+int groups_of_lines(const Cut& c, int E) {
+  const int line = 8 * E, groups = c.C % line ? c.G : line / gcd(c.width, line);
+  return (int64_t)groups * c.width <= kWidest * E ? groups : 0;
+}
+
+// A chunk of whole groups, of `least` vectors where there are as many channels, in whole `unit`s of groups where it can; unit 0: ending
+// with a vector.
+void cut_channels(Cut& c, int E, int least, int unit = 0) {
   const int most = kThreads * E;
   if (c.width > most) {
     c.per = 0;
@@ -63,8 +74,8 @@ void cut_channels(Cut& c, int E, int least) {
     if ((int64_t)(c.parts - 1) * ((c.chunk + E - 1) / E * E) <= c.width - E) c.chunk = (c.chunk + E - 1) / E * E;
     c.chunks = c.G * c.parts;
   } else {
-    int unit = E / gcd(c.width, E);
-    if ((int64_t)unit * c.width > most || c.C % E) unit = 1;
+    if (!unit) unit = c.C % E ? 1 : E / gcd(c.width, E);
+    if ((int64_t)unit * c.width > most) unit = 1;
     int per = unit;
     while (per < c.G && (int64_t)per * c.width < least * E && (int64_t)(per + unit) * c.width <= most) per += unit;
     if (per > c.G) per = c.G;
@@ -94,23 +105,37 @@ void cut_pixels(Cut& c, int64_t slices) {
 Cut cut_of(int64_t N, int64_t C, int64_t pixels, int64_t G, int E) {
   Cut c;
   c.N = (int)N; c.C = (int)C; c.G = (int)G; c.width = (int)(C / G); c.pixels = pixels;
-  // Chunks of 32 vectors (512 bytes of a pixel) while that leaves enough blocks, else of 16 or 8; slices for a thousand
-  // blocks, of eight rounds of pixels each at least ([128, 56 * 56, 256] bf16, both directions: 333 us; 2048 blocks 357, 4096
-  // 414, chunks of 8 vectors 351).
+  // Chunks of 32 vectors (512 bytes of a pixel) while that leaves enough blocks, else of 16 or 8.  The chip holds 1024 blocks at a
+  // time; slices for one to eight times as many, of eight rounds of pixels each at least: those with the fewest rounds one after the
+  // other, a block's start and end counted as eight ([128, 56 * 56, 256] bf16, both directions: 1024 blocks 333 us, 2048 357, 4096
+  // 414, chunks of 8 vectors 351; [54, 35 * 35, 768] in 32 groups, 1134 blocks 223 us, 972 219).
   int64_t slices = 1;
-  for (int least = 32; least >= 8; least /= 2) {
-    cut_channels(c, E, least);
+  auto cut = [&](int least, int unit) {
+    cut_channels(c, E, least, unit);
     const int rows = kThreads / c.cols;
-    const int64_t most = (pixels + 8 * rows - 1) / (8 * rows);
-    slices = (1024 + (int64_t)c.N * c.chunks - 1) / ((int64_t)c.N * c.chunks);
-    if (slices > most) slices = most;
-    if (slices > 64) slices = 64;
-    if ((int64_t)c.N * c.chunks * slices >= 768) break;
-  }
-  if ((int64_t)c.N * c.chunks * slices < 768) {          // few blocks: four rounds ([5, 55 * 55, 96] 30.4 us, 27.9 like this)
+    const int64_t planes = (int64_t)c.N * c.chunks;
+    int64_t most = (pixels + 8 * rows - 1) / (8 * rows), fewest = 0;
+    if (most > 64) most = 64;
+    for (int times = 1; times <= 8; ++times) {
+      int64_t n = 1024 * times / planes;
+      n = n < 1 ? 1 : n > most ? most : n;
+      const int64_t cost = (planes * n + 1023) / 1024 * ((pixels + n * rows - 1) / (n * rows) + 8);
+      if (fewest == 0 || cost < fewest) {
+        fewest = cost;
+        slices = n;
+      }
+    }
+    return planes * slices >= 768;
+  };
+  const int lines = groups_of_lines(c, E);
+  bool enough = lines && cut(32, lines);
+  for (int least = 32; !enough && least >= 8; least /= 2) enough = cut(least, 0);
+  if (!enough) {                                         // few blocks: four rounds ([5, 55 * 55, 96] 30.4 us, 27.9 like this)
     const int rows = kThreads / c.cols;
     int64_t most = (pixels + 4 * rows - 1) / (4 * rows);
     if (most > 64) most = 64;
+    const int64_t room = 1024 / ((int64_t)c.N * c.chunks);
+    if (most > room) most = room;
     if (slices < most) slices = most;
   }
   const int64_t needed = (pixels * C >> 30) + 1;        // (offsets inside a slice are 32-bit)
@@ -119,23 +144,31 @@ Cut cut_of(int64_t N, int64_t C, int64_t pixels, int64_t G, int E) {
   return c;
 }
 
-// One kernel: a block to a sample's chunk of 8 vectors at least, where a thread has few pixels ([4, 16 * 16, 320] fp16 both
-// directions 24.9 us, by two kernels each 27.4) or the blocks fill the chip anyway ([64, 28 * 28, 256] bf16 45.9, 67.9; 64 blocks
-// of 32 pixels a thread, [16, 32 * 32, 256]: 47.7, 34.0).  Few blocks with several pixels a thread take chunks of 4 vectors (C
-// entry points, 8 vectors / 4: [4, 16 * 16, 320] 25.2 / 20.7, [32, 22 * 22, 64] in 8 groups 30.6 / 22.7), where those have two
-// groups: a wave adds up a group (forward of one in [4, 16 * 16, 1280] 12.1 / 12.8).  False: the plane is too large, or a group
-// wider than a block.
+// One kernel, a block to a sample's chunk, both directions against two kernels each, us:
+//   * chunks of whole lines whose blocks fill the chip, up to 64 pixels a thread: [64, 28 * 28, 256] bf16 45.9, 67.9 (64 blocks of
+//     32 pixels a thread, [16, 32 * 32, 256]: 47.7, 34.0);
+//   * chunks of 8 vectors at least where a thread has few pixels, unless the tensor is so large that parts of lines cost more than
+//     the launches: [4, 16 * 16, 320] fp16 24.9, 27.4; [190, 8 * 5, 624] in 24 groups 38.7, 50.0; but [200, 16 * 16, 320] 77.3, 62.7.
+//     Few blocks with several pixels a thread take chunks of 4 vectors (8 vectors / 4: [4, 16 * 16, 320] 25.2 / 20.7,
+//     [32, 22 * 22, 64] in 8 groups 30.6 / 22.7) where those have two groups: a wave adds up a group (forward of one in
+//     [4, 16 * 16, 1280] 12.1 / 12.8).
+// False: none of these, or a group wider than a block.
 constexpr int kFewPixels = 16, kSomePixels = 64;
+constexpr int64_t kManyValues = 1 << 23;
 bool cut_once(Cut& c, int E) {
+  if (c.pixels * c.C >> 30) return false;
   Cut once = c;
-  cut_channels(once, E, 8);
-  if (!once.per || c.pixels * c.C >> 30) return false;
-  const int64_t mine = (c.pixels + kThreads / once.cols - 1) / (kThreads / once.cols);
-  const bool few = (int64_t)c.N * once.chunks < 256;
-  if (mine > kFewPixels && (mine > kSomePixels || few)) return false;
-  Cut half = once;
-  cut_channels(half, E, 4);
-  if (mine >= 6 && few && half.per >= 2) once = half;
+  auto cut = [&](int least, int unit) {                  // pixels of a thread
+    cut_channels(once, E, least, unit);
+    return (c.pixels + kThreads / once.cols - 1) / (kThreads / once.cols);
+  };
+  auto blocks = [&] { return (int64_t)c.N * once.chunks; };
+  const int lines = groups_of_lines(c, E);
+  if (!lines || cut(8, lines) > kSomePixels || blocks() < 256) {
+    const int64_t mine = cut(8, 0);
+    if (!once.per || mine > kFewPixels || (lines && blocks() >= 256 && c.N * c.pixels * c.C >= kManyValues)) return false;
+    if (mine >= 6 && blocks() < 256 && (cut(4, 0), once.per < 2)) cut(8, 0);
+  }
   cut_pixels(once, 1);
   if (once.blocks() > kMostBlocks) return false;
   c = once;

@@ -809,40 +809,53 @@ PyObject* linear_tokens_grad_weight(PyObject* const* a, Py_ssize_t n) {
 }
 
 // ---------------------------------------------------------------------------- group norm
-// [N, C, ...] channels last as [N, ..., C], which is how it lies in memory; `dense`: it does
+// [N, C, ...] channels last, [N, ..., C] in memory; `dense`: the tensor lies like that.  (No view is made of one that does: each
+// would take half a microsecond of a short call.)
 struct Pixels {
-  Tensor held;
-  bool dense;
+  Tensor given;
+  bool dense = true;
   int64_t N, C, count = 1;
-  explicit Pixels(const Tensor& t, const char* name) {
+  Pixels(const Tensor& t, const char* name) : given(t) {
     check_float(t, name);
-    set(t, name);
+    set(name);
   }
-  Pixels(const Tensor& t, const char* name, at::ScalarType dtype) {
+  Pixels(const Tensor& t, const char* name, at::ScalarType dtype) : given(t) {
     TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor!");
     TORCH_CHECK(t.scalar_type() == dtype, "The type of ", name, " is not correct!");
-    set(t, name);
+    set(name);
   }
-  // a tensor of the same shape and layout, and its view in the order of the channels first
-  Tensor empty_like(at::ScalarType dtype) const { return empty(held.sizes(), held, dtype); }
-  static Tensor channels_first(const Tensor& t) {
-    if (t.dim() == 2) return t;
-    std::vector<int64_t> order{0, t.dim() - 1};
-    for (int64_t d = 1; d + 1 < t.dim(); ++d) order.push_back(d);
-    return t.permute(order);
+  // a new tensor of the same shape, channels last
+  Tensor empty_like(at::ScalarType dtype) const {
+    return at::empty_strided(given.sizes(), strides, at::TensorOptions().dtype(dtype).device(given.device()));
+  }
+  // the tensor, or a copy that is channels last
+  Tensor laid_out() const {
+    if (dense) return given;
+    const Tensor copy = empty_like(given.scalar_type());
+    return copy.copy_(given.detach());
   }
 
  private:
-  void set(const Tensor& t, const char* name) {
-    TORCH_CHECK(t.dim() >= 2, "The dimension of ", name, " is not correct!");
-    N = t.size(0);
-    C = t.size(1);
-    for (int64_t d = 2; d < t.dim(); ++d) count *= t.size(d);
-    std::vector<int64_t> order{0};
-    for (int64_t d = 2; d < t.dim(); ++d) order.push_back(d);
-    order.push_back(1);
-    held = t.dim() == 2 ? t : t.permute(order);
-    dense = held.is_contiguous();
+  std::vector<int64_t> strides;
+  void set(const char* name) {
+    TORCH_CHECK(given.dim() >= 2, "The dimension of ", name, " is not correct!");
+    const auto size = given.sizes(), stride = given.strides();
+    N = size[0];
+    C = size[1];
+    strides.resize(size.size());
+    int64_t next = 1;
+    auto place = [&](int64_t d) {
+      strides[d] = next;
+      if (size[d] != 1 && stride[d] != next) dense = false;
+      next *= size[d] > 1 ? size[d] : 1;
+    };
+    place(1);
+    for (int64_t d = given.dim() - 1; d >= 2; --d) {
+      count *= size[d];
+      place(d);
+    }
+    place(0);
+    if (given.numel() == 0) dense = true;
   }
 };
 struct GroupNorm {
@@ -857,19 +870,20 @@ struct GroupNorm {
   static Tensor parameter(const Tensor& t, const Pixels& x, const char* name) {
     if (!t.defined()) return t;
     check_float(t, name);
-    TORCH_CHECK(t.device() == x.held.device(), name, " must be on the same device");
+    TORCH_CHECK(t.device() == x.given.device(), name, " must be on the same device");
     TORCH_CHECK(t.numel() == x.C, name, " must have one value for each channel, ", x.C, ", and has ", t.numel());
+    if (t.scalar_type() == at::kFloat && t.is_contiguous()) return t;
     return t.detach().to(at::kFloat).contiguous();
   }
 };
 // (the kernels read 16 bytes: what torch allocates has room for them, a view at the end of a smaller tensor may not)
-Tensor with_room(const Tensor& t) { return t.nbytes() < 16 ? t.clone() : t; }
+Tensor with_room(const Tensor& t) { return t.nbytes() < 16 ? t.detach().clone() : t; }
 
 // input, groups, weight | None, bias | None, eps, activation, whether the input is kept
 //   -> output, mean, rstd, codes | None, scale | None
 PyObject* group_norm_forward(PyObject* const* a, Py_ssize_t n) {
   Args args(a, n, 7);
-  const Tensor input = args.tensor().detach();
+  const Tensor input = args.tensor();
   const int64_t groups = args.integer();
   const Tensor given_weight = args.optional(), given_bias = args.optional();
   const double eps = args.number();
@@ -881,7 +895,7 @@ PyObject* group_norm_forward(PyObject* const* a, Py_ssize_t n) {
   const GroupNorm norm(groups, given_weight, given_bias, activation, x);
   const auto dtype = input.scalar_type();
   const int code = code_of(dtype);
-  const Tensor from = with_room(x.held), y = x.empty_like(dtype);
+  const Tensor from = with_room(input), y = x.empty_like(dtype);
   const Tensor mean = empty({x.N, groups}, input, at::kFloat), rstd = empty({x.N, groups}, input, at::kFloat);
   const Tensor codes = keep ? x.empty_like(at::kChar) : Tensor(), scale = keep ? empty({x.N, groups}, input, at::kFloat) : Tensor();
   const int64_t bytes = actnn_group_norm_workspace_bytes(x.N, x.C, x.count, groups, code, 0);
@@ -896,25 +910,25 @@ PyObject* group_norm_forward(PyObject* const* a, Py_ssize_t n) {
                                     static_cast<int8_t*>(ptr(codes)), f32(scale), x.N, x.C, x.count, groups, eps,
                                     norm.activation, code, ptr(workspace), bytes, stream_of(input));
   });
-  return tuple_of(Pixels::channels_first(y), mean, rstd, keep ? Pixels::channels_first(codes) : Tensor(), scale);
+  return tuple_of(y, mean, rstd, codes, scale);
 }
 
 // grad_output, codes | None, scale | None, input | None, groups, weight | None, bias | None, mean, rstd, activation
 //   -> gradients of the input, the weight and the bias (None where there is none)
 PyObject* group_norm_backward(PyObject* const* a, Py_ssize_t n) {
   Args args(a, n, 10);
-  const Tensor grad_output = args.tensor().detach();
+  const Tensor grad_output = args.tensor();
   const Tensor codes = args.optional(), given_scale = args.optional(), input = args.optional();
   const int64_t groups = args.integer();
   const Tensor given_weight = args.optional(), given_bias = args.optional(), given_mean = args.tensor(), given_rstd = args.tensor();
   const int64_t activation = args.integer();
   TORCH_CHECK(codes.defined() != input.defined() && codes.defined() == given_scale.defined(),
               "group_norm_backward: either codes and scale or the input");
-  Pixels dy(grad_output, "grad_output");
+  const Pixels dy(grad_output, "grad_output");
   const c10::DeviceGuard guard(grad_output.device());
   const auto dtype = grad_output.scalar_type();
   const Tensor& saved = codes.defined() ? codes : input;
-  const Pixels x(saved.detach(), codes.defined() ? "codes" : "input", codes.defined() ? at::kChar : dtype);
+  const Pixels x(saved, codes.defined() ? "codes" : "input", codes.defined() ? at::kChar : dtype);
   TORCH_CHECK(saved.sizes() == grad_output.sizes(), "grad_output ", grad_output.sizes(), " and the saved input ", saved.sizes(),
               " are not of the same shape");
   TORCH_CHECK(saved.device() == grad_output.device(), "the saved input must be on the same device");
@@ -922,7 +936,7 @@ PyObject* group_norm_backward(PyObject* const* a, Py_ssize_t n) {
   const Tensor mean = row_scales(given_mean, dy.N * groups, grad_output, "mean");
   const Tensor rstd = row_scales(given_rstd, dy.N * groups, grad_output, "rstd");
   const Tensor scale = codes.defined() ? row_scales(given_scale, dy.N * groups, grad_output, "scale") : Tensor();
-  const Tensor grad = with_room(dy.held.contiguous()), kept = codes.defined() ? x.held.contiguous() : with_room(x.held.contiguous());
+  const Tensor grad = with_room(dy.laid_out()), kept = codes.defined() ? x.laid_out() : with_room(x.laid_out());
   const Tensor dx = dy.empty_like(dtype);
   const Tensor dweight = norm.weight.defined() ? empty({dy.C}, grad, at::kFloat) : Tensor();
   const Tensor dbias = norm.bias.defined() ? empty({dy.C}, grad, at::kFloat) : Tensor();
@@ -940,7 +954,7 @@ PyObject* group_norm_backward(PyObject* const* a, Py_ssize_t n) {
                                        ptr(workspace), bytes, stream_of(grad));
     });
   }
-  return tuple_of(Pixels::channels_first(dx), dweight, dbias);
+  return tuple_of(dx, dweight, dbias);
 }
 
 template <PyObject* (*F)(PyObject* const*, Py_ssize_t)>

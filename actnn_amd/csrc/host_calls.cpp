@@ -653,9 +653,13 @@ struct NewCodes {
     const int64_t K = size.back();
     size.back() = whole16(K);
     codes = empty(size, like, at::kChar);
+    if (K % 16) {                                        // (the first K of each row; a view would cost a short call a tenth)
+      std::vector<int64_t> strides(codes.strides().begin(), codes.strides().end());
+      size.back() = K;
+      codes.unsafeGetTensorImpl()->set_sizes_and_strides(size, strides);
+    }
     size.pop_back();
     scale = empty(size, like, at::kFloat);
-    if (K % 16) codes = codes.narrow(-1, 0, K);
   }
 };
 

@@ -6,10 +6,9 @@
 // the bias is added, and the result is rounded to the output's type.  Sums that are split over blocks or waves are
 // added as integers: the order does not matter.
 //
-// Three kernels share the work by the number of tokens:
-//   * few tokens: bound by reading the weight once.  No tiles: a wave's lanes load their 16 bytes of 16 channels' rows
-//     straight into the operand registers of v_mfma_i32_16x16x64_i8, the waves of a block share the features of the same
-//     channels and add their sums in LDS.
+// Three kernels share the work:
+//   * few tokens (up to 32): no tiles: a wave's lanes load their 16 bytes of 16 channels' rows straight into the operand
+//     registers of v_mfma_i32_16x16x64_i8, the waves of a block share the features of the same channels and add their sums in LDS.
 //   * tiles of 64, 128 or 256 channels by as many tokens, for everything else: v_mfma_i32_32x32x32_i8 out of LDS.  Four buffers of
 //     64 or 128 features; both operands go from global memory straight into LDS (global_load_lds, 16 bytes a lane), rows as they
 //     lie in memory, their 16-byte chunks permuted so that 16 rows that are read together meet every bank once.
@@ -30,7 +29,7 @@ typedef int i32x16 __attribute__((ext_vector_type(16)));
 constexpr int kThreads = 256;
 constexpr int64_t kMostFeatures = 131071;               // the integer sum of so many products fits 32 bits
 constexpr int64_t kMostStride = 0x7fffff;               // 256 rows of so many bytes stay below 2 GiB
-constexpr int64_t kMostOutputs = 0x3ffffff;             // 16 of them to a block of up to 1024 threads
+constexpr int64_t kMostOutputs = 0x3ffffff;             // 16 of them to a block
 
 // the first `valid` of 16 bytes, the others 0
 ACTNN_DEV u32x4 first_bytes(u32x4 v, int valid) {
@@ -305,67 +304,57 @@ __global__ __launch_bounds__(kThreads, 1) void tokens_tile_kernel(Product p, int
 }
 
 // ------------------------------------------------------------------------------------------
-// Few tokens: 16 NT channels a block, MT tiles of 16 tokens; the waves share the features, a run of pieces of 64 each.  Bound by
-// the weight, which is read once: [24, 4096] -> 16384 takes 16.0 us beside its quantisation, 67 MB at 4.2 TB/s.
+// Few tokens, up to 32: 16 channels a block, MT tiles of 16 tokens; the waves share the features, a run of pieces of 64 each.
+// Bound by the latency of a wave's loads, 4 pieces ahead, and past some 4.5 TB/s of weight by those: [12, 4096] -> 4096 takes 6.0 us.
 // ------------------------------------------------------------------------------------------
-template <typename TY, int MT, int NT, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void tokens_few_kernel(Product p) {
-  constexpr int kAhead = 4;
-  __shared__ i32x4 s_sum[WAVES][NT * MT][64];
+constexpr int kFew = 32;
+template <typename TY, int MT>
+__global__ __launch_bounds__(kThreads) void tokens_few_kernel(Product p) {
+  constexpr int kAhead = 4, WAVES = kThreads / 64;
+  __shared__ i32x4 s_sum[WAVES][MT][64];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int o0 = blockIdx.x * 16 * NT;
+  const int o0 = blockIdx.x * 16;
   const int row = lane & 15, part = lane >> 4;
-  const int8_t *wp[NT], *xp[MT];
-#pragma unroll
-  for (int i = 0; i < NT; ++i) wp[i] = p.w + (int64_t)(o0 + 16 * i + row < p.O ? o0 + 16 * i + row : p.O - 1) * p.ldw;
+  const int8_t *wp = p.w + (int64_t)(o0 + row < p.O ? o0 + row : p.O - 1) * p.ldw, *xp[MT];
 #pragma unroll
   for (int i = 0; i < MT; ++i) xp[i] = p.x + (int64_t)(16 * i + row < p.M ? 16 * i + row : p.M - 1) * p.ldx;
-  i32x4 acc[NT][MT];
+  i32x4 acc[MT];
 #pragma unroll
-  for (int i = 0; i < NT; ++i)
-#pragma unroll
-    for (int j = 0; j < MT; ++j) acc[i][j] = (i32x4){0, 0, 0, 0};
+  for (int i = 0; i < MT; ++i) acc[i] = (i32x4){0, 0, 0, 0};
   const int pieces = (p.K + 63) / 64, per = (pieces + WAVES - 1) / WAVES;
   const int end = (wave + 1) * per < pieces ? (wave + 1) * per : pieces;
   for (int c0 = wave * per; c0 < end; c0 += kAhead) {
-    u32x4 fw[kAhead][NT], fx[kAhead][MT];
+    u32x4 fw[kAhead], fx[kAhead][MT];
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) {
       int k = (c0 + j) * 64 + part * 16;
       k = k < p.K && c0 + j < end ? k : 0;                             // (masked below)
-#pragma unroll
-      for (int i = 0; i < NT; ++i) fw[j][i] = load16(wp[i] + k);
+      fw[j] = load16(wp + k);
 #pragma unroll
       for (int i = 0; i < MT; ++i) fx[j][i] = load16(xp[i] + k);
     }
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) {
       const int left = c0 + j < end ? p.K - (c0 + j) * 64 - part * 16 : 0;
+      const u32x4 w = left < 16 ? first_bytes(fw[j], left) : fw[j];
 #pragma unroll
-      for (int i = 0; i < NT; ++i) {
-        const u32x4 w = left < 16 ? first_bytes(fw[j][i], left) : fw[j][i];
-#pragma unroll
-        for (int t = 0; t < MT; ++t)
-          acc[i][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, w), __builtin_bit_cast(i32x4, fx[j][t]),
-                                                            acc[i][t], 0, 0, 0);
-      }
+      for (int t = 0; t < MT; ++t)
+        acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, w), __builtin_bit_cast(i32x4, fx[j][t]),
+                                                       acc[t], 0, 0, 0);
     }
   }
 #pragma unroll
-  for (int i = 0; i < NT; ++i)
-#pragma unroll
-    for (int t = 0; t < MT; ++t) s_sum[wave][i * MT + t][lane] = acc[i][t];
+  for (int t = 0; t < MT; ++t) s_sum[wave][t][lane] = acc[t];
   __syncthreads();
   // accumulator register c of a lane: channel 4 (lane / 16) + c, token lane % 16
-  for (int i = threadIdx.x; i < NT * MT * 64; i += 64 * WAVES) {
+  for (int i = threadIdx.x; i < MT * 64; i += kThreads) {
     const int tile = i >> 6, in = i & 63;
     i32x4 v = s_sum[0][tile][in];
 #pragma unroll
     for (int w = 1; w < WAVES; ++w) v += s_sum[w][tile][in];
     const int sum[4] = {v.x, v.y, v.z, v.w};
-    const int channel = o0 + 16 * (tile / MT) + 4 * (in >> 4);
-    const int token = 16 * (tile % MT) + (in & 15);
+    const int channel = o0 + 4 * (in >> 4), token = 16 * tile + (in & 15);
     if (channel < p.O && token < p.M) put4<TY>(p, token, channel, sum, p.xs[token]);
   }
 }
@@ -469,15 +458,18 @@ __global__ __launch_bounds__(kThreads) void tokens_sum_slices_kernel(Product p, 
 // end of a block, the fetch of its code among them, `fixed`; slices a second launch of about 4.5, and their sums are written and
 // read back at some 8 TB/s.  Measured, tile 64 by 64 features / 64 by 128 / 128 / 256, us: 256 x 4096 x 4096 (tokens, features,
 // outputs) 12.2, 10.0, 18.9, 42; 1024 x 4096 x 4096 36.1, 29.6, 27.9, 42.8; 8192 x 4096 x 4096 248, 205, 169, 125;
-// 512 x 1024 x 2048 6.3, 6.6, 7.6, 18.8.
+// 512 x 1024 x 2048 6.3, 6.6, 7.6, 18.8.  Few tokens without tiles: 0.7 (1.1 for more than 16) for every 1024 features that its
+// waves walk alone, or the weight at 4.5 TB/s, and 2 for start and end (without tiles / by them: 24 x 4096 x 1024 6.7, 10.8;
+// 24 x 4096 x 16384 21.2, 13.1; 16 x 16384 x 100 15.9, 10.1; 61 x 7326 x 1790, which none of it takes, 15.5, 11.8).
 struct Plan { int tile, slices, steps; };
 struct Tile { int edge, features; double fixed, step_us; };
 constexpr Tile kTiles[] = {{0, 1, 0.0, 0.0}, {64, 64, 3.0, 0.15}, {64, 128, 4.0, 0.25}, {128, 64, 5.0, 0.32},
                            {256, 64, 12.0, 0.88}};
 Plan plan_of(int64_t M, int64_t K, int64_t O) {
-  if (M <= 64) return Plan{0, 1, 0};
   Plan best{0, 1, 0};
-  double least = 0.0;
+  const bool few = M <= kFew;
+  const double alone = (M <= 16 ? 0.7 : 1.1) * (double)K / 1024.0, together = (double)K * (double)O / 4.5e6;
+  double least = 2.0 + (alone > together ? alone : together);
   for (int i = 1; i < (int)(sizeof(kTiles) / sizeof(kTiles[0])); ++i) {
     const Tile& t = kTiles[i];
     const int64_t tiles = ((M + t.edge - 1) / t.edge) * ((O + t.edge - 1) / t.edge), steps = (K + t.features - 1) / t.features;
@@ -486,7 +478,7 @@ Plan plan_of(int64_t M, int64_t K, int64_t O) {
       const double rounds = tiles * n <= 128 ? 0.7 : (double)((tiles * n + 255) / 256);
       const double us = t.fixed + t.step_us * rounds * (double)per +
                         (n > 1 ? 4.5 + 8.0 * (double)n * (double)M * (double)O / 8.0e6 : 0.0);
-      if (best.tile == 0 || us < least) {
+      if ((best.tile == 0 && !few) || us < least) {
         least = us;
         best = Plan{i, (int)((steps + per - 1) / per), (int)per};
       }
@@ -509,24 +501,15 @@ template <typename TY> void launch_tile(const Product& p, const Plan& plan, int6
     default: return launch_tiles<TY, 4>(p, plan, blocks, s);
   }
 }
-template <typename TY, int MT, int NT, int WAVES> void launch_few(const Product& p, hipStream_t s) {
-  tokens_few_kernel<TY, MT, NT, WAVES><<<dim3((unsigned)((p.O + 16LL * NT - 1) / (16 * NT))), dim3(64 * WAVES), 0, s>>>(p);
+template <typename TY, int MT> void launch_few(const Product& p, hipStream_t s) {
+  tokens_few_kernel<TY, MT><<<dim3((unsigned)((p.O + 15LL) / 16)), dim3(kThreads), 0, s>>>(p);
 }
 
 template <typename TY> int product(const Product& p, void* workspace, int64_t workspace_bytes, hipStream_t s) {
   Plan plan = plan_of(p.M, p.K, p.O);
   if (plan.tile == 0) {
-    // More channels to a block re-read the tokens less often, where 64 of them leave blocks for most of the chip; more waves to a
-    // block keep more loads in flight, where each has features enough (us, 16 channels / 64: [24, 4096] -> 16384 23.8 / 16.0,
-    // -> 4096 8.2 / 14.5; 4 waves / 16: [16, 1024] -> 4096 3.0 / 5.7, [32, 4096] -> 4096 by 16 channels 10.1 / 8.2).
-    const bool wide = p.O >= 12288, deep = p.K >= 2048;
-    if (p.M <= 16) launch_few<TY, 1, 1, 4>(p, s);
-    else if (p.M <= 32 && wide) launch_few<TY, 2, 4, 4>(p, s);
-    else if (p.M <= 32 && deep) launch_few<TY, 2, 1, 16>(p, s);
-    else if (p.M <= 32) launch_few<TY, 2, 1, 4>(p, s);
-    else if (wide) launch_few<TY, 4, 4, 4>(p, s);
-    else if (deep) launch_few<TY, 4, 1, 16>(p, s);
-    else launch_few<TY, 4, 1, 4>(p, s);
+    if (p.M <= 16) launch_few<TY, 1>(p, s);
+    else launch_few<TY, 2>(p, s);
     ACTNN_RETURN_LAUNCH_STATUS();
   }
   const int64_t n = (int64_t)p.M * p.O;

@@ -793,12 +793,10 @@ PyObject* linear_tokens_grad_weight(PyObject* const* a, Py_ssize_t n) {
     rows = room;
     ld = width;
   };
-  if (actnn_tokens_grad_weight_wants_chunks(x.M, O, x.K)) {
-    // (two passes over the gradient, where the product would take twice as long; the outputs added are cut off below)
-    if (O % 8 != 0 || ld % 8 != 0 || reinterpret_cast<uintptr_t>(rows.data_ptr()) % 16 != 0) {
-      pad((O + 7) / 8 * 8);
-      O = ld;
-    }
+  const bool chunks = O % 8 == 0 && ld % 8 == 0 && reinterpret_cast<uintptr_t>(rows.data_ptr()) % 16 == 0;
+  if (!chunks && actnn_tokens_grad_weight_wants_chunks(x.M, O, x.K)) {
+    pad((O + 7) / 8 * 8);                                // (the outputs added are cut off below)
+    O = ld;
   } else if ((x.M - 1) * ld + O < 8) {                   // the kernel reads 16 bytes at least
     pad(8);
   }

@@ -470,23 +470,20 @@ __global__ __launch_bounds__(kThreads) void tokens_grad_sum_kernel(const float* 
 // the chip's 256 CUs (the small tiles: two blocks a CU at the same time); the start and the end of a block `fixed`; splits a
 // second launch of about 4.5, and their fp32 tiles are written and read back at some 8 TB/s (mostly in the last cache).  (Measured,
 // large / 128 / 64: one round of 256 steps 250, two of 16 59, one of 16 12.)
-struct Plan { int edge, splits, tokens; };
+struct Plan { int edge, splits, tokens; double us; };
 struct Kernel { int edge, step, unit; double fixed, step_us; int64_t at_once; };
 constexpr Kernel kKernels[] = {{64, 64, 64, 3.0, 0.55, 512}, {128, 64, 64, 4.0, 1.0, 256}, {256, 32, 128, 8.0, 0.9, 256}};
 Plan plan_of(int64_t M, int64_t O, int64_t I, bool aligned) {
-  Plan best{0, 1, 0};
-  double least = 0.0;
+  Plan best{0, 1, 0, 0.0};
   for (const Kernel& k : kKernels) {
     if (k.edge == 256 && (!aligned || M < 512)) continue;
     const int64_t tiles = ((O + k.edge - 1) / k.edge) * ((I + k.edge - 1) / k.edge), units = (M + k.unit - 1) / k.unit;
-    for (int64_t n = 1; n <= 64 && n <= units && (n == 1 || n * tiles <= 1024); n *= 2) {
+    for (int64_t n = 1; n <= 64 && n <= units && (n == 1 || n * tiles <= 1024); n += n < 16 ? 1 : 4) {
+      const double sums = n > 1 ? 4.5 + 8.0 * (double)n * (double)O * (double)I / 8.0e6 : 0.0;
+      if (best.edge != 0 && k.fixed + k.step_us + sums >= best.us) break;
       const int64_t per = (units + n - 1) / n, rounds = (tiles * n + k.at_once - 1) / k.at_once;
-      const double us = k.fixed + k.step_us * (double)(rounds * per * (k.unit / k.step)) +
-                        (n > 1 ? 4.5 + 8.0 * (double)n * (double)O * (double)I / 8.0e6 : 0.0);
-      if (best.edge == 0 || us < least) {
-        least = us;
-        best = Plan{k.edge, (int)((units + per - 1) / per), (int)(per * k.unit)};
-      }
+      const double us = k.fixed + k.step_us * (double)(rounds * per * (k.unit / k.step)) + sums;
+      if (best.edge == 0 || us < best.us) best = Plan{k.edge, (int)((units + per - 1) / per), (int)(per * k.unit), us};
     }
   }
   return best;
@@ -496,7 +493,7 @@ template <typename T, typename TY>
 int launch_grad(Grad p, bool aligned, void* workspace, int64_t workspace_bytes, hipStream_t s) {
   Plan plan = plan_of(p.M, p.O, p.I, aligned);
   const int64_t n = (int64_t)p.O * p.I;
-  if (plan.splits > 1 && (!workspace || workspace_bytes < 4 * n * plan.splits)) plan = Plan{plan.edge, 1, p.M};
+  if (plan.splits > 1 && (!workspace || workspace_bytes < 4 * n * plan.splits)) plan = Plan{plan.edge, 1, p.M, 0.0};
   const int64_t edge = plan.edge, blocks = ((p.O + edge - 1) / edge) * ((p.I + edge - 1) / edge) * plan.splits;
   if (blocks > kMostBlocks) return ACTNN_EINVAL;
   const dim3 grid((unsigned)blocks), blk(kThreads);
@@ -543,7 +540,8 @@ extern "C" int64_t actnn_tokens_grad_weight_workspace_bytes(int64_t M, int64_t O
 extern "C" int actnn_tokens_grad_weight_wants_chunks(int64_t M, int64_t O, int64_t I) {
   using namespace actnn;
   if (M < 1 || O < 1 || I < 1 || M > 0x7fffff00LL || O > 0x7fffff00LL || I > 0x7fffff00LL) return 0;
-  return plan_of(M, O, I, true).edge == 256;
+  // (a copy is two launches, and grad_out is read and written once more, at some 4 TB/s)
+  return plan_of(M, O, I, true).us + 9.0 + 4.0 * (double)M * (double)O / 4.0e6 < plan_of(M, O, I, false).us;
 }
 
 extern "C" int actnn_tokens_grad_weight(const void* grad_out, int64_t ldg, const int8_t* codes, int64_t ldc, const float* scale,

@@ -305,7 +305,7 @@ __global__ __launch_bounds__(kThreads, 1) void tokens_tile_kernel(Product p, int
 
 // ------------------------------------------------------------------------------------------
 // Few tokens, up to 32: 16 channels a block, MT tiles of 16 tokens; the waves share the features, a run of pieces of 64 each.
-// Bound by the latency of a wave's loads, 4 pieces ahead, and past some 4.5 TB/s of weight by those: [12, 4096] -> 4096 takes 6.0 us.
+// Bound by the latency of a wave's loads, 4 pieces ahead, and past some 4.5 TB/s of weight by those: [12, 4096] -> 4096 takes 5.9.
 // ------------------------------------------------------------------------------------------
 constexpr int kFew = 32;
 template <typename TY, int MT>
@@ -454,13 +454,14 @@ __global__ __launch_bounds__(kThreads) void tokens_sum_slices_kernel(Product p, 
 }
 
 // Which kernel - the tile, 0: few tokens - and slices of the features, of `steps` steps each: the cheapest by this estimate, us.
-// A step takes step_us for each round of blocks over the chip's 256 CUs, 0.7 of it for half a round or less; the start and the
-// end of a block, the fetch of its code among them, `fixed`; slices a second launch of about 4.5, and their sums are written and
-// read back at some 8 TB/s.  Measured, tile 64 by 64 features / 64 by 128 / 128 / 256, us: 256 x 4096 x 4096 (tokens, features,
-// outputs) 12.2, 10.0, 18.9, 42; 1024 x 4096 x 4096 36.1, 29.6, 27.9, 42.8; 8192 x 4096 x 4096 248, 205, 169, 125;
-// 512 x 1024 x 2048 6.3, 6.6, 7.6, 18.8.  Few tokens without tiles: 0.7 (1.1 for more than 16) for every 1024 features that its
-// waves walk alone, or the weight at 4.5 TB/s, and 2 for start and end (without tiles / by them: 24 x 4096 x 1024 6.7, 10.8;
-// 24 x 4096 x 16384 21.2, 13.1; 16 x 16384 x 100 15.9, 10.1; 61 x 7326 x 1790, which none of it takes, 15.5, 11.8).
+// A step takes step_us for each round of blocks over the chip's 256 CUs, 0.7 of it for half a round or less (the last round of the
+// smaller tiles, two of which share a CU, may be half a round); the start and the end of a block, the fetch of its code among
+// them, `fixed`; slices a second launch of about 4.5, and their sums are written and read back at some 8 TB/s.  Measured, tile 64
+// by 64 features / 64 by 128 / 128 / 256, us: 256 x 4096 x 4096 (tokens, features, outputs) 12.2, 10.0, 18.9, 42;
+// 1024 x 4096 x 4096 36.1, 29.6, 27.9, 42.8; 8192 x 4096 x 4096 248, 205, 169, 125; 512 x 1024 x 2048 6.3, 6.6, 7.6, 18.8.  Few
+// tokens without tiles: 0.7 (1.1 for more than 16) for every 1024 features that its waves walk alone, or the weight at 4.5 TB/s,
+// and 2 for start and end (without tiles / by them: 24 x 4096 x 1024 6.7, 10.8; 24 x 4096 x 16384 21.2, 13.1; 16 x 16384 x 100
+// 15.9, 10.1; 61 x 7326 x 1790, which none of it takes, 15.5, 11.8).
 struct Plan { int tile, slices, steps; };
 struct Tile { int edge, features; double fixed, step_us; };
 constexpr Tile kTiles[] = {{0, 1, 0.0, 0.0}, {64, 64, 3.0, 0.15}, {64, 128, 4.0, 0.25}, {128, 64, 5.0, 0.32},
@@ -473,11 +474,15 @@ Plan plan_of(int64_t M, int64_t K, int64_t O) {
   for (int i = 1; i < (int)(sizeof(kTiles) / sizeof(kTiles[0])); ++i) {
     const Tile& t = kTiles[i];
     const int64_t tiles = ((M + t.edge - 1) / t.edge) * ((O + t.edge - 1) / t.edge), steps = (K + t.features - 1) / t.features;
-    for (int64_t n = 1; n <= 16 && n <= steps && (n == 1 || n * tiles <= 512); n *= 2) {
+    for (int64_t n = 1; n <= 16 && n <= steps && (n == 1 || n * tiles <= 512); ++n) {
+      const double sums = n > 1 ? 4.5 + 8.0 * (double)n * (double)M * (double)O / 8.0e6 : 0.0;
+      if ((best.tile != 0 || few) && t.fixed + sums >= least) break;
       const int64_t per = (steps + n - 1) / n;
-      const double rounds = tiles * n <= 128 ? 0.7 : (double)((tiles * n + 255) / 256);
-      const double us = t.fixed + t.step_us * rounds * (double)per +
-                        (n > 1 ? 4.5 + 8.0 * (double)n * (double)M * (double)O / 8.0e6 : 0.0);
+      const int64_t blocks = tiles * n;
+      const double rounds = blocks <= 128    ? 0.7
+                            : t.edge == 256 ? (double)((blocks + 255) / 256)
+                                            : 0.5 * (double)((blocks + 127) / 128);
+      const double us = t.fixed + t.step_us * rounds * (double)per + sums;
       if ((best.tile == 0 && !few) || us < least) {
         least = us;
         best = Plan{i, (int)((steps + per - 1) / per), (int)per};

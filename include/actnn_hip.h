@@ -538,8 +538,8 @@ int actnn_tokens_linear_few(const void* data, int64_t ld, const int8_t* weight_c
  * element address; a grad_out of fewer than 8 elements wants ldg >= 8 and that much memory for each row.  M >= 1.
  * Workspace as above. */
 int64_t actnn_tokens_grad_weight_workspace_bytes(int64_t M, int64_t O, int64_t I);
-/* 1: a product so large that its kernel wants grad_out's rows in whole 16-byte chunks (address, ldg and O); others are taken
- * by a slower one. */
+/* 1: a product whose fastest kernel wants grad_out's rows in whole 16-byte chunks (address, ldg and O) and is worth a copy of
+ * them; rows as they are are taken by a slower one. */
 int actnn_tokens_grad_weight_wants_chunks(int64_t M, int64_t O, int64_t I);
 int actnn_tokens_grad_weight(const void* grad_out, int64_t ldg, const int8_t* codes, int64_t ldc, const float* scale,
                              void* grad_w, int64_t M, int64_t O, int64_t I, int go_dtype, int out_dtype, void* workspace,

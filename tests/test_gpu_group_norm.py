@@ -141,6 +141,18 @@ def test_forward_and_backward(shape, groups, dtype):
         check_backward(dy, x, mean, rstd, groups, w, b, activation, full)
 
 
+# blocks enough for the whole chip: chunks of whole lines in one kernel and in two, whole pixels, groups of a chunk and wider ones
+MANY = [((200, 192, 20, 20), 32), ((200, 320, 16, 16), 32), ((130, 1280, 8, 8), 32), ((150, 366, 17, 16), 6), ((60, 770, 14, 14), 1),
+        ((300, 100, 9, 11), 20), ((3, 2056, 30, 30), 1), ((1100, 24, 9, 9), 3), ((1, 640, 300, 70), 2)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape,groups", MANY)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_forward_and_backward_of_many_blocks(shape, groups, dtype):
+    test_forward_and_backward(shape, groups, dtype)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("at", [0, 12345])

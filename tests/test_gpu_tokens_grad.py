@@ -76,6 +76,13 @@ def test_gradient_is_the_formulas_difference():
         assert abs(numeric - gw[o, i].item()) <= 2.0 ** -23 * (M + 2) * (g[:, o].double().abs() @ values[:, i].abs()).item() + 1e-9
 
 
+# splits of any number; gradients whose rows are no whole chunks, copied and as they are
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,O,I", [(1500, 327, 3200), (1156, 673, 1728), (900, 1001, 3000), (4000, 1001, 1024), (5000, 60, 500), (3000, 515, 700)])
+def test_gradient_between_the_kernels(M, O, I):
+    test_gradient(M, O, I, torch.bfloat16)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("M", [70, 700])

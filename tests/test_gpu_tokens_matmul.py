@@ -57,6 +57,14 @@ def test_product(M, K, O):
         check(y, codes, scale, wcodes, wscale, bias, dtype)
 
 
+# few tokens by tiles, with slices of any number; tiles whose last round is half empty
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,K,O", [(5, 16384, 100), (16, 2048, 16400), (24, 4090, 16390), (31, 12300, 70), (33, 512, 40), (48, 9001, 200), (61, 7326, 1790),
+                                   (500, 6100, 450), (700, 14208, 130), (2300, 1024, 1030), (1351, 3000, 720)])
+def test_product_between_the_kernels(M, K, O):
+    test_product(M, K, O)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("M", [2, 20, 65, 300])
 @pytest.mark.parametrize("sign", [1, -1])

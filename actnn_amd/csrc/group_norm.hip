@@ -63,8 +63,8 @@ int groups_of_lines(const Cut& c, int E) {
   return (int64_t)groups * c.width <= kWidest * E ? groups : 0;
 }
 
-// A chunk of whole groups, of `least` vectors where there are as many channels, in whole `unit`s of groups where it can; unit 0: ending
-// with a vector.
+// A chunk of whole groups, of `least` vectors where there are as many channels, in whole `unit`s of groups where it can; unit 0:
+// ending with a vector.
 void cut_channels(Cut& c, int E, int least, int unit = 0) {
   const int most = kThreads * E;
   if (c.width > most) {
@@ -106,9 +106,10 @@ Cut cut_of(int64_t N, int64_t C, int64_t pixels, int64_t G, int E) {
   Cut c;
   c.N = (int)N; c.C = (int)C; c.G = (int)G; c.width = (int)(C / G); c.pixels = pixels;
   // Chunks of 32 vectors (512 bytes of a pixel) while that leaves enough blocks, else of 16 or 8.  The chip holds 1024 blocks at a
-  // time; slices for one to eight times as many, of eight rounds of pixels each at least: those with the fewest rounds one after the
-  // other, a block's start and end counted as eight ([128, 56 * 56, 256] bf16, both directions: 1024 blocks 333 us, 2048 357, 4096
-  // 414, chunks of 8 vectors 351; [54, 35 * 35, 768] in 32 groups, 1134 blocks 223 us, 972 219).
+  // time; slices for one to eight times as many, of eight rounds of pixels each at least: those with the fewest rounds one after
+  // the other, a block's start and end counted as eight (both directions, us: [128, 56 * 56, 256] bf16 with 1024 blocks 333, 2048
+  // 357, 4096 414, chunks of 8 vectors 351; slices for a little over 1024 blocks / a little under: [28, 61 * 81, 366] in 6 groups
+  // 219 / 204, [10, 122 * 122, 340] in 4 214 / 199).
   int64_t slices = 1;
   auto cut = [&](int least, int unit) {
     cut_channels(c, E, least, unit);
@@ -148,7 +149,8 @@ Cut cut_of(int64_t N, int64_t C, int64_t pixels, int64_t G, int E) {
 //   * chunks of whole lines whose blocks fill the chip, up to 64 pixels a thread: [64, 28 * 28, 256] bf16 45.9, 67.9 (64 blocks of
 //     32 pixels a thread, [16, 32 * 32, 256]: 47.7, 34.0);
 //   * chunks of 8 vectors at least where a thread has few pixels, unless the tensor is so large that parts of lines cost more than
-//     the launches: [4, 16 * 16, 320] fp16 24.9, 27.4; [190, 8 * 5, 624] in 24 groups 38.7, 50.0; but [200, 16 * 16, 320] 77.3, 62.7.
+//     the launches: [4, 16 * 16, 320] fp16 24.9, 27.4; [190, 8 * 5, 624] in 24 groups 38.7, 50.0; but [200, 16 * 16, 320] 77.3,
+//     62.7.
 //     Few blocks with several pixels a thread take chunks of 4 vectors (8 vectors / 4: [4, 16 * 16, 320] 25.2 / 20.7,
 //     [32, 22 * 22, 64] in 8 groups 30.6 / 22.7) where those have two groups: a wave adds up a group (forward of one in
 //     [4, 16 * 16, 1280] 12.1 / 12.8).

@@ -1,6 +1,8 @@
 """Plumbing between torch tensors and the C ABI: argument checks that mirror the reference's
 CHECK_CUDA_TENSOR_* macros (cpp_extension/ext_common.h), dtype codes, the current HIP stream
 and the Philox (seed, offset) taken from torch's default device generator."""
+import threading
+
 import torch
 
 from .. import _lib
@@ -14,6 +16,31 @@ def lib():
 
 def host():
     """The module of native calls (csrc/host_calls.cpp), the C library loaded under it."""
+    return _lib.load_host()
+
+
+class _TracedStep(threading.local):
+    """`with traced_step:` - what an autograd Function computes inside, which torch.jit.trace records as one step that calls the
+    Function again."""
+    depth = 0
+
+    def __enter__(self):
+        self.depth += 1
+
+    def __exit__(self, *exc):
+        self.depth -= 1
+        return False
+
+
+traced_step = _TracedStep()
+
+
+def untraced(name):
+    """host() for a call that writes what it allocates with a kernel of its own.  A trace would keep the allocation and lose the
+    kernel, so a call that is no step of a Function is refused while one is recorded."""
+    if torch._C._get_tracing_state() is not None and not traced_step.depth:
+        raise RuntimeError(f"{name} cannot be traced by itself: the tracer does not see its kernels (the layers over it, "
+                           "QInt8Linear and QGroupNorm, can be traced)")
     return _lib.load_host()
 
 

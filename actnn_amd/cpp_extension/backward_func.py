@@ -467,11 +467,12 @@ def hip_group_norm_forward(input, num_groups, weight, bias, eps, activation=None
     [N, C, ...] that is channels last - the channels of a pixel side by side in memory, as in torch.channels_last and in any
     [N, C] tensor.  mean and rstd are fp32 [N, num_groups].  With `keep` the input also comes as int8 codes (laid out like it) with
     one fp32 scale for each sample and group, what hip_group_norm_backward needs of it; None, None otherwise."""
-    return _glue.host().group_norm_forward(input, num_groups, weight, bias, eps, _activation(activation), keep)
+    return _glue.untraced("hip_group_norm_forward").group_norm_forward(input, num_groups, weight, bias, eps,
+                                                                       _activation(activation), keep)
 
 
 def hip_group_norm_backward(grad_output, codes, scale, num_groups, weight, bias, mean, rstd, activation=None, input=None):
     """-> (grad_input, grad_weight, grad_bias) of hip_group_norm_forward, computed at the values the codes stand for, or
     at `input` itself (codes and scale None).  The parameters' gradients are fp32, None without the parameter."""
-    return _glue.host().group_norm_backward(grad_output, codes, scale, input, num_groups, weight, bias, mean, rstd,
-                                            _activation(activation))
+    return _glue.untraced("hip_group_norm_backward").group_norm_backward(grad_output, codes, scale, input, num_groups, weight,
+                                                                         bias, mean, rstd, _activation(activation))

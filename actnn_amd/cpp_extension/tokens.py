@@ -11,6 +11,7 @@ infinity has scale NaN: everything made from it is NaN.
 
 Codes come in rows that begin at multiples of 16 bytes (their stride is K rounded up to 16), the layout the kernels read;
 codes laid out otherwise are taken too, and copied first.  Everything runs on the current stream of the tensors' device.
+torch.jit.trace does not see these calls, which refuse to be recorded; the layers over them can be traced.
 """
 import torch
 
@@ -25,12 +26,12 @@ def _dtype_code(dtype, what):
 
 def quantize_tokens(data):
     """-> (codes, scale): int8 [..., K] and fp32 [...] of a float32, float16 or bfloat16 tensor [..., K]."""
-    return g.host().quantize_tokens(data)
+    return g.untraced("quantize_tokens").quantize_tokens(data)
 
 
 def dequantize_tokens(codes, scale, dtype=torch.float32):
     """codes * scale, rounded once to `dtype`."""
-    return g.host().dequantize_tokens(codes, scale, _dtype_code(dtype, "dequantize_tokens"))
+    return g.untraced("dequantize_tokens").dequantize_tokens(codes, scale, _dtype_code(dtype, "dequantize_tokens"))
 
 
 def matmul_tokens(codes, scale, weight_codes, weight_scale, bias=None, dtype=torch.float32):
@@ -38,13 +39,14 @@ def matmul_tokens(codes, scale, weight_codes, weight_scale, bias=None, dtype=tor
 
     The weight is kept as tokens itself (`quantize_tokens` of a linear layer's [O, K] weight: one scale for each output
     channel).  The sums are 32-bit integers and exact, for up to 131071 features."""
-    return g.host().matmul_tokens(codes, scale, weight_codes, weight_scale, bias, _dtype_code(dtype, "matmul_tokens"))
+    dtype = _dtype_code(dtype, "matmul_tokens")
+    return g.untraced("matmul_tokens").matmul_tokens(codes, scale, weight_codes, weight_scale, bias, dtype)
 
 
 def linear_tokens(data, weight_codes, weight_scale, bias=None, keep=False):
     """matmul_tokens(*quantize_tokens(data), ...) in the type of `data`.  With `keep` also the tokens as they were
     multiplied, which are the checkpoint that linear_tokens_grad_weight reads: (output, codes, scale)."""
-    out, codes, scale = g.host().linear_tokens(data, weight_codes, weight_scale, bias, bool(keep))
+    out, codes, scale = g.untraced("linear_tokens").linear_tokens(data, weight_codes, weight_scale, bias, bool(keep))
     return (out, codes, scale) if keep else out
 
 
@@ -52,5 +54,5 @@ def linear_tokens_grad_weight(grad_output, codes, scale, dtype=None):
     """grad_output[..., O]^T @ (codes * scale)[..., K] -> [O, K], summed over all tokens in fp32: the weight gradient of
     a linear layer from the tokens it kept.  grad_output is float16 or bfloat16 (the values of the codes are rounded to its type
     on their way into the product); the result comes in its type, or with `dtype` in float32."""
-    return g.host().linear_tokens_grad_weight(grad_output, codes, scale,
-                                              None if dtype is None else _dtype_code(dtype, "linear_tokens_grad_weight"))
+    dtype = None if dtype is None else _dtype_code(dtype, "linear_tokens_grad_weight")
+    return g.untraced("linear_tokens_grad_weight").linear_tokens_grad_weight(grad_output, codes, scale, dtype)

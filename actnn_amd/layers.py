@@ -195,8 +195,9 @@ class QLinear(nn.Linear):
         return _autocast_apply(linear, input, self.weight, self.bias, self.scheme)
 
 
-def _wants_grad(*tensors):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+def _wants_function(*tensors):
+    """Whether a call goes through its autograd Function: for a gradient, or to be one step of a trace."""
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors) or torch.jit.is_tracing()
 
 
 class QInt8Linear(nn.Linear):
@@ -238,7 +239,7 @@ class QInt8Linear(nn.Linear):
         return {k: v for k, v in self.__dict__.items() if k != "_held"}
 
     def forward(self, input):
-        if _wants_grad(input, self.weight, self.bias):
+        if _wants_function(input, self.weight, self.bias):
             return _autocast_apply(int8_linear, input, self.weight, self.bias)
         if torch.is_autocast_enabled("cuda"):
             input = input.to(torch.get_autocast_dtype("cuda"))
@@ -252,11 +253,11 @@ class QGroupNorm(nn.GroupNorm):
 
     def forward(self, input, silu=False):
         """`silu`: the SiLU that follows this layer, in the same pass (gn_silu)."""
-        input = to_channels_last(input)
         activation = "silu" if silu else None
-        if _wants_grad(input, self.weight, self.bias):
+        if _wants_function(input, self.weight, self.bias):
             return group_norm.apply(input, self.num_groups, self.weight, self.bias, self.eps, activation)
-        return ext_backward_func.hip_group_norm_forward(input, self.num_groups, self.weight, self.bias, self.eps, activation)[0]
+        return ext_backward_func.hip_group_norm_forward(to_channels_last(input), self.num_groups, self.weight, self.bias,
+                                                        self.eps, activation)[0]
 
 
 def gn_silu(gn, silu, input):

@@ -16,7 +16,7 @@ from .cpp_extension import minimax as ext_minimax
 from .cpp_extension import quantization as ext_quantization
 from .cpp_extension import tokens as ext_tokens
 from .utils import (channels_last_format, compute_tensor_bytes, empty_cache, get_memory_usage,
-                    logical_order, memory_order, swap_to_cpu, swap_to_device)
+                    logical_order, memory_order, swap_to_cpu, swap_to_device, to_channels_last)
 
 
 # ------------------------------------------------------------------------------------------
@@ -545,12 +545,24 @@ class linear(Function):
         return grad_input, grad_weight, grad_bias, None
 
 
+def _one_step(forward):
+    """Forward pass of a Function whose native calls the tracer does not see: a trace records the Function as one step."""
+    @functools.wraps(forward)
+    def run(ctx, *args):
+        if torch._C._get_tracing_state() is None:
+            return forward(ctx, *args)
+        with ext_tokens.g.traced_step:
+            return forward(ctx, *args)
+    return run
+
+
 class int8_linear(Function):
     """Linear layer multiplied in 8-bit integers: the input one scale a token, the weight one an output channel.  The tokens as
     they were multiplied are all that is kept of the input, and the weight's gradient is that of the values they stand for.  To the
     gradients the rounding of either factor is the identity: grad_input = grad_output @ weight."""
 
     @staticmethod
+    @_one_step
     def forward(ctx, input, weight, bias=None):
         weight_codes, weight_scale = ext_tokens.quantize_tokens(weight)
         output, codes, scale = ext_tokens.linear_tokens(input, weight_codes, weight_scale, bias, keep=True)
@@ -889,12 +901,14 @@ class batch_norm_add_relu(Function):
 
 
 class group_norm(Function):
-    """Group norm with its activation (None or "silu") of a channels-last input, of which 8-bit codes with one scale for each
-    sample and group are kept (config.compress_activation off: the input itself).  The gradients are those at the kept
-    values, with the statistics of the input."""
+    """Group norm with its activation (None or "silu"), channels last (other inputs are copied).  Of the input 8-bit codes with
+    one scale for each sample and group are kept (config.compress_activation off: the input itself).  The gradients are those
+    at the kept values, with the statistics of the input."""
 
     @staticmethod
+    @_one_step
     def forward(ctx, input, num_groups, weight, bias, eps, activation=None):
+        input = to_channels_last(input)                 # (here, so that a trace does it too, whatever the layout it was made with)
         keep = config.compress_activation
         output, mean, rstd, codes, scale = ext_backward_func.hip_group_norm_forward(
             input, num_groups, weight, bias, eps, activation, keep)

@@ -12,6 +12,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/Context.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -590,6 +591,15 @@ PyObject* max_pool2d_backward(PyObject* const* a, Py_ssize_t n) {
   return wrap(out);
 }
 
+// ---------------------------------------------------------------------------- derivatives
+// The calls below have none in forward mode, and a result without a tangent would count as a constant.  (While an autograd Function
+// runs its forward pass the mode is off, and what the Function has decides.)
+void no_tangents(const char* what, std::initializer_list<const Tensor*> given) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  for (const Tensor* t : given)
+    TORCH_CHECK(!t->defined() || !t->_fw_grad(0).defined(), what, " has no forward-mode derivative");
+}
+
 // ---------------------------------------------------------------------------- 8-bit tokens
 bool is_float(const Tensor& t) {
   return t.scalar_type() == at::kFloat || t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16;
@@ -667,6 +677,7 @@ struct NewCodes {
 PyObject* quantize_tokens(PyObject* const* a, Py_ssize_t n) {
   Args args(a, n, 1);
   const Tensor data = args.tensor();
+  no_tangents("quantize_tokens", {&data});
   const Rows rows(data, "data");
   const c10::DeviceGuard guard(data.device());
   const NewCodes out(data);
@@ -681,6 +692,7 @@ PyObject* dequantize_tokens(PyObject* const* a, Py_ssize_t n) {
   Args args(a, n, 3);
   const Tensor codes = args.tensor(), given = args.tensor();
   const auto dtype = type_of(args.integer());
+  no_tangents("dequantize_tokens", {&given});
   const CodeRows rows(codes, "codes");
   const Tensor scale = row_scales(given, rows.M, codes, "scale");
   const c10::DeviceGuard guard(codes.device());
@@ -727,6 +739,7 @@ PyObject* matmul_tokens(PyObject* const* a, Py_ssize_t n) {
   Args args(a, n, 6);
   const Tensor codes = args.tensor(), given = args.tensor(), wcodes = args.tensor(), wscale = args.tensor(), bias = args.optional();
   const auto dtype = type_of(args.integer());
+  no_tangents("matmul_tokens", {&given, &wscale, &bias});
   const CodeRows x(codes, "codes");
   const c10::DeviceGuard guard(codes.device());
   const Tensor scale = row_scales(given, x.M, codes, "scale");
@@ -738,6 +751,7 @@ PyObject* linear_tokens(PyObject* const* a, Py_ssize_t n) {
   Args args(a, n, 5);
   const Tensor data = args.tensor(), wcodes = args.tensor(), wscale = args.tensor(), bias = args.optional();
   const bool keep = args.flag();
+  no_tangents("linear_tokens", {&data, &wscale, &bias});
   const Rows rows(data, "data");
   const c10::DeviceGuard guard(data.device());
   const Weight w(wcodes, wscale, bias, data, rows.K);
@@ -766,6 +780,7 @@ PyObject* linear_tokens(PyObject* const* a, Py_ssize_t n) {
 PyObject* linear_tokens_grad_weight(PyObject* const* a, Py_ssize_t n) {
   Args args(a, n, 4);
   const Tensor grad = args.tensor(), codes = args.tensor(), given = args.tensor();
+  no_tangents("linear_tokens_grad_weight", {&grad, &given});
   TORCH_CHECK(grad.is_cuda(), "grad_output must be a CUDA tensor!");
   const auto type = grad.scalar_type();
   TORCH_CHECK(type == at::kHalf || type == at::kBFloat16, "The type of grad_output is not correct!");
@@ -891,6 +906,7 @@ PyObject* group_norm_forward(PyObject* const* a, Py_ssize_t n) {
   const double eps = args.number();
   const int64_t activation = args.integer();
   const bool keep = args.flag();
+  no_tangents("group_norm_forward", {&input, &given_weight, &given_bias});
   const Pixels x(input, "input");
   TORCH_CHECK(x.dense, "input must be channels last: [N, C, ...] with the channels of a pixel side by side in memory");
   const c10::DeviceGuard guard(input.device());
@@ -924,6 +940,8 @@ PyObject* group_norm_backward(PyObject* const* a, Py_ssize_t n) {
   const int64_t groups = args.integer();
   const Tensor given_weight = args.optional(), given_bias = args.optional(), given_mean = args.tensor(), given_rstd = args.tensor();
   const int64_t activation = args.integer();
+  no_tangents("group_norm_backward",
+              {&grad_output, &given_scale, &input, &given_weight, &given_bias, &given_mean, &given_rstd});
   TORCH_CHECK(codes.defined() != input.defined() && codes.defined() == given_scale.defined(),
               "group_norm_backward: either codes and scale or the input");
   const Pixels dy(grad_output, "grad_output");

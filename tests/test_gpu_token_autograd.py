@@ -1,6 +1,8 @@
-"""The 8-bit token calls and the layers over them under the tracer: what it cannot follow is handed to a Function, or refused."""
+"""The 8-bit token calls and the layers over them under the tracer and in forward mode: what these cannot follow is handed to a
+Function, or refused."""
 import pytest
 import torch
+import torch.autograd.forward_ad as fwad
 import torch.nn as nn
 
 from actnn_amd import layers
@@ -59,3 +61,49 @@ def test_calls_by_themselves_are_not_traced():
                  lambda x: bf.hip_group_norm_backward(x, None, None, 2, None, None, m, m, input=x)[0]):
         with pytest.raises(RuntimeError, match="cannot be traced"):
             torch.jit.trace(call, x)
+
+
+def operands():
+    """Every call with its differentiable arguments: name -> (function of them, the arguments)."""
+    torch.manual_seed(2)
+    x, w, b = torch.randn(6, 32, device=DEV), torch.randn(8, 32, device=DEV), torch.randn(8, device=DEV)
+    c, s = tokens.quantize_tokens(x)
+    wc, ws = tokens.quantize_tokens(w)
+    g = torch.randn(6, 8, device=DEV).half()
+    a, d = torch.rand(32, device=DEV) + 0.5, torch.randn(32, device=DEV)
+    y, mean, rstd, codes, scale = bf.hip_group_norm_forward(x, 4, a, d, 1e-5, "silu", keep=True)
+    return {
+        "quantize_tokens": (lambda x: tokens.quantize_tokens(x)[1], (x,)),
+        "dequantize_tokens": (lambda s: tokens.dequantize_tokens(c, s), (s,)),
+        "matmul_tokens": (lambda s, ws, b: tokens.matmul_tokens(c, s, wc, ws, b), (s, ws, b)),
+        "linear_tokens": (lambda x, ws, b: tokens.linear_tokens(x, wc, ws, b), (x, ws, b)),
+        "linear_tokens, kept": (lambda x, ws, b: tokens.linear_tokens(x, wc, ws, b, keep=True)[0], (x, ws, b)),
+        "linear_tokens_grad_weight": (lambda g, s: tokens.linear_tokens_grad_weight(g, c, s), (g, s)),
+        "group_norm_forward": (lambda x, a, d: bf.hip_group_norm_forward(x, 4, a, d, 1e-5, "silu")[0], (x, a, d)),
+        "group_norm_backward": (lambda y, a, d, m, r: bf.hip_group_norm_backward(y, codes, scale, 4, a, d, m, r, "silu")[0],
+                                (y, a, d, mean, rstd)),
+    }
+
+
+@pytest.mark.gpu
+def test_tangents_are_refused():
+    for name, (call, given) in operands().items():
+        for i in range(len(given)):
+            with fwad.dual_level(), torch.no_grad():
+                args = list(given)
+                args[i] = fwad.make_dual(given[i], torch.ones_like(given[i]))
+                with pytest.raises(RuntimeError, match="forward"):
+                    call(*args)
+            assert torch.equal(call(*given), call(*given)), name          # and nothing of it stays
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("frozen", [False, True])
+def test_tangents_are_refused_by_the_layers(frozen):
+    for layer in (layers.QInt8Linear(32, 8).to(DEV), layers.QGroupNorm(4, 32).to(DEV)):
+        layer.requires_grad_(not frozen)
+        x = torch.randn(6, 32, device=DEV)
+        for grad in (True, False):
+            with fwad.dual_level(), torch.set_grad_enabled(grad):
+                with pytest.raises(RuntimeError, match="forward"):
+                    layer(fwad.make_dual(x, torch.ones_like(x)))

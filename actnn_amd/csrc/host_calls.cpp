@@ -16,6 +16,8 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include "../../include/actnn_hip.h"
@@ -599,6 +601,19 @@ void no_tangents(const char* what, std::initializer_list<const Tensor*> given) {
   for (const Tensor* t : given)
     TORCH_CHECK(!t->defined() || !t->_fw_grad(0).defined(), what, " has no forward-mode derivative");
 }
+// Nor is a backward pass recorded here (ops.py has the Functions that do): a result made of what wants a gradient is one whose
+// backward pass says so, as with torch's own operators that have none.
+void no_gradients(const char* what, std::initializer_list<const Tensor*> given, std::initializer_list<const Tensor*> made) {
+  if (!at::GradMode::is_enabled()) return;
+  torch::autograd::edge_list edges;
+  for (const Tensor* t : given)
+    if (t->defined() && t->requires_grad()) edges.push_back(torch::autograd::impl::gradient_edge(*t));
+  if (edges.empty()) return;
+  const std::shared_ptr<torch::autograd::Node> node(new torch::autograd::NotImplemented(what, std::move(edges)),
+                                                    torch::autograd::deleteNode);
+  for (const Tensor* t : made)
+    if (t->defined()) torch::autograd::set_history(*t, node);
+}
 
 // ---------------------------------------------------------------------------- 8-bit tokens
 bool is_float(const Tensor& t) {
@@ -685,6 +700,7 @@ PyObject* quantize_tokens(PyObject* const* a, Py_ssize_t n) {
     return actnn_tokens_quantize(ptr(rows.held), rows.ld, static_cast<int8_t*>(ptr(out.codes)), whole16(rows.K), f32(out.scale),
                                  rows.M, rows.K, code_of(data.scalar_type()), stream_of(data));
   });
+  no_gradients("quantize_tokens", {&data}, {&out.scale});
   return tuple_of(out.codes, out.scale);
 }
 // codes, scale, dtype -> values
@@ -700,6 +716,7 @@ PyObject* dequantize_tokens(PyObject* const* a, Py_ssize_t n) {
   launch("dequantize_tokens", [&] {
     return actnn_tokens_dequantize(rows.data(), rows.ld, f32(scale), ptr(out), rows.M, rows.K, code_of(dtype), stream_of(codes));
   });
+  no_gradients("dequantize_tokens", {&given}, {&out});
   return wrap(out);
 }
 
@@ -744,7 +761,9 @@ PyObject* matmul_tokens(PyObject* const* a, Py_ssize_t n) {
   const c10::DeviceGuard guard(codes.device());
   const Tensor scale = row_scales(given, x.M, codes, "scale");
   const Weight w(wcodes, wscale, bias, codes, x.K);
-  return wrap(product_of(x, scale, w, codes.sizes(), dtype));
+  const Tensor out = product_of(x, scale, w, codes.sizes(), dtype);
+  no_gradients("matmul_tokens", {&given, &wscale, &bias}, {&out});
+  return wrap(out);
 }
 // data, weight codes, weight scale, bias | None, whether the tokens are kept -> product, codes | None, scale | None
 PyObject* linear_tokens(PyObject* const* a, Py_ssize_t n) {
@@ -765,6 +784,7 @@ PyObject* linear_tokens(PyObject* const* a, Py_ssize_t n) {
       return actnn_tokens_linear_few(ptr(rows.held), rows.ld, w.rows.data(), w.rows.ld, f32(w.scale), f32(w.bias), ptr(out), rows.M,
                                      rows.K, w.rows.M, code_of(data.scalar_type()), stream_of(data));
     });
+    no_gradients("linear_tokens", {&data, &wscale, &bias}, {&out});
     return tuple_of(out, Tensor(), Tensor());
   }
   const NewCodes kept(data);
@@ -774,6 +794,7 @@ PyObject* linear_tokens(PyObject* const* a, Py_ssize_t n) {
                                  code_of(data.scalar_type()), stream_of(data));
   });
   const Tensor out = product_of(x, kept.scale, w, data.sizes(), data.scalar_type());
+  no_gradients("linear_tokens", {&data, &wscale, &bias}, {&out, &kept.scale});
   return keep ? tuple_of(out, kept.codes, kept.scale) : tuple_of(out, Tensor(), Tensor());
 }
 // grad_output, codes, scale, dtype -> gradient of the weight
@@ -795,8 +816,9 @@ PyObject* linear_tokens_grad_weight(PyObject* const* a, Py_ssize_t n) {
   const int64_t outputs = grad.size(-1);
   int64_t O = outputs;
   if (O == 0 || x.M == 0) {
-    const Tensor out = empty({O, x.K}, grad, dtype);
-    return wrap(out.zero_());
+    const Tensor out = empty({O, x.K}, grad, dtype).zero_();
+    no_gradients("linear_tokens_grad_weight", {&grad, &given}, {&out});
+    return wrap(out);
   }
   Tensor rows = grad.detach().reshape({x.M, O});
   if (O > 1 && rows.stride(1) != 1) rows = rows.contiguous();
@@ -822,7 +844,9 @@ PyObject* linear_tokens_grad_weight(PyObject* const* a, Py_ssize_t n) {
     return actnn_tokens_grad_weight(ptr(rows), ld, x.data(), x.ld, f32(scale), ptr(out), x.M, O, x.K, code_of(type),
                                     code_of(dtype), ptr(workspace), bytes, stream_of(grad));
   });
-  return wrap(O == outputs ? out : out.narrow(0, 0, outputs));
+  const Tensor made = O == outputs ? out : out.narrow(0, 0, outputs);
+  no_gradients("linear_tokens_grad_weight", {&grad, &given}, {&made});
+  return wrap(made);
 }
 
 // ---------------------------------------------------------------------------- group norm
@@ -928,6 +952,7 @@ PyObject* group_norm_forward(PyObject* const* a, Py_ssize_t n) {
                                     static_cast<int8_t*>(ptr(codes)), f32(scale), x.N, x.C, x.count, groups, eps,
                                     norm.activation, code, ptr(workspace), bytes, stream_of(input));
   });
+  no_gradients("group_norm_forward", {&input, &given_weight, &given_bias}, {&y, &mean, &rstd, &scale});
   return tuple_of(y, mean, rstd, codes, scale);
 }
 
@@ -974,6 +999,8 @@ PyObject* group_norm_backward(PyObject* const* a, Py_ssize_t n) {
                                        ptr(workspace), bytes, stream_of(grad));
     });
   }
+  no_gradients("group_norm_backward", {&grad_output, &given_scale, &input, &given_weight, &given_bias, &given_mean, &given_rstd},
+               {&dx, &dweight, &dbias});
   return tuple_of(dx, dweight, dbias);
 }
 

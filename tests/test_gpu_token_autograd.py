@@ -1,5 +1,5 @@
-"""The 8-bit token calls and the layers over them under the tracer and in forward mode: what these cannot follow is handed to a
-Function, or refused."""
+"""The 8-bit token calls and the layers over them under the tracer, in forward mode and in reverse mode: what these cannot follow
+is handed to a Function that they can, or refused."""
 import pytest
 import torch
 import torch.autograd.forward_ad as fwad
@@ -107,3 +107,32 @@ def test_tangents_are_refused_by_the_layers(frozen):
             with fwad.dual_level(), torch.set_grad_enabled(grad):
                 with pytest.raises(RuntimeError, match="forward"):
                     layer(fwad.make_dual(x, torch.ones_like(x)))
+
+
+@pytest.mark.gpu
+def test_calls_without_a_derivative_say_so_in_the_backward_pass():
+    for name, (call, given) in operands().items():
+        want = call(*given)
+        for i in range(len(given)):
+            args = list(given)
+            args[i] = given[i].clone().requires_grad_()
+            y = call(*args)
+            assert torch.equal(y.detach(), want) and y.requires_grad, name
+            with pytest.raises(RuntimeError, match=f"derivative for {name.split(',')[0]} is not implemented"):
+                y.float().sum().backward()
+            assert args[i].grad is None
+            with torch.no_grad():
+                assert not call(*args).requires_grad
+        assert not call(*given).requires_grad
+
+
+@pytest.mark.gpu
+def test_a_result_cut_out_of_a_larger_one_says_so_too():
+    # (a gradient of odd width whose product runs over whole chunks)
+    c, s = tokens.quantize_tokens(torch.randn(1156, 1728, device=DEV))
+    g = torch.randn(1156, 673, device=DEV).bfloat16()
+    want = tokens.linear_tokens_grad_weight(g, c, s)
+    got = tokens.linear_tokens_grad_weight(g.requires_grad_(), c, s)
+    assert torch.equal(got.detach(), want)
+    with pytest.raises(RuntimeError, match="derivative for linear_tokens_grad_weight is not implemented"):
+        got.float().sum().backward()

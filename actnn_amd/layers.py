@@ -239,10 +239,11 @@ class QInt8Linear(nn.Linear):
         return {k: v for k, v in self.__dict__.items() if k != "_held"}
 
     def forward(self, input):
-        if _wants_function(input, self.weight, self.bias):
-            return _autocast_apply(int8_linear, input, self.weight, self.bias)
-        if torch.is_autocast_enabled("cuda"):
+        if torch.is_autocast_enabled("cuda") and input.is_floating_point():
+            # (the input alone: a weight cast to 16 bits first would be rounded to other codes than the one that is held)
             input = input.to(torch.get_autocast_dtype("cuda"))
+        if _wants_function(input, self.weight, self.bias):
+            return int8_linear.apply(input, self.weight, self.bias)
         return ext_tokens.linear_tokens(input, *self._weight_tokens(), self.bias)
 
 

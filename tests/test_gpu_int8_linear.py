@@ -1,0 +1,47 @@
+"""QInt8Linear in the ways that a model uses it beside plain training: under autocast, frozen, held, without compression."""
+import copy
+
+import pytest
+import torch
+
+from actnn_amd import layers
+from actnn_amd.conf import config
+from actnn_amd.cpp_extension import tokens
+
+DEV = "cuda:0"
+HALF_STEP = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
+
+
+@pytest.fixture(autouse=True)
+def fresh_config():
+    config.reset()
+    yield
+    config.reset()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("M", [3, 200])
+def test_training_and_answering_multiply_the_same_integers_under_autocast(M, dtype):
+    torch.manual_seed(1)
+    layer = layers.QInt8Linear(128, 48).to(DEV)
+    x = torch.randn(M, 128, device=DEV, requires_grad=True)
+    go = torch.randn(M, 48, device=DEV).to(dtype)
+    with torch.autocast("cuda", dtype=dtype):
+        y = layer(x)
+        with torch.no_grad():
+            answer = layer(x)
+            held = copy.deepcopy(layer).hold_weight()(x)
+    assert y.dtype == answer.dtype == dtype and torch.equal(y, answer) and torch.equal(y, held)
+    wc, ws = tokens.quantize_tokens(layer.weight.detach())
+    assert torch.equal(y, tokens.linear_tokens(x.detach().to(dtype), wc, ws, layer.bias.detach()))
+    y.backward(go)
+    # the gradient of the weight in its own type: 16-bit values, sums in 32 bits that are not rounded to 16
+    codes, scale = tokens.quantize_tokens(x.detach().to(dtype))
+    values = codes.double() * scale.double()[:, None]
+    exact, size = go.double().t() @ values, go.double().abs().t() @ values.abs()
+    grad = layer.weight.grad
+    assert grad.dtype == torch.float32 and torch.equal(grad, tokens.linear_tokens_grad_weight(go, codes, scale, torch.float32))
+    assert ((grad.double() - exact).abs() <= (HALF_STEP[dtype] * 1.01 + 2.0 ** -23 * (M + 2)) * size).all()
+    assert layer.bias.grad.dtype == torch.float32 and x.grad.dtype == torch.float32
+    assert ((layer.bias.grad.double() - go.double().sum(0)).abs() <= 2.0 ** -23 * (M + 2) * go.double().abs().sum(0)).all()

@@ -203,11 +203,11 @@ def _wants_function(*tensors):
 class QInt8Linear(nn.Linear):
     """A linear layer that multiplies in 8-bit integers - one scale for each token (row of the input) and each output channel -
     and keeps, of its input, the codes it multiplied: a byte a value.  In training the weight is rounded anew in every forward
-    pass and its gradient is that of the kept values.
+    pass and its gradient is that of the kept values; a frozen weight has none, and nothing is kept for it.
 
-    A layer that only answers rounds its weight once: `hold_weight()`, to be called again after the weight has been replaced
-    (changes in place, load_state_dict, .to() and train() are noticed and end the hold; what is written past autograd, through
-    `weight.data` or into inference tensors, is not)."""
+    A layer that only answers, or whose weight is frozen, rounds it once: `hold_weight()`, to be called again after the weight
+    has been replaced (changes in place, load_state_dict, .to() and train() are noticed and end the hold; what is written past
+    autograd, through `weight.data` or into inference tensors, is not)."""
 
     _held = None
 
@@ -219,12 +219,13 @@ class QInt8Linear(nn.Linear):
             self._held = (self.weight, self._version(), *ext_tokens.quantize_tokens(self.weight))
         return self
 
-    def _weight_tokens(self):
+    def _held_tokens(self):
+        """The tokens of hold_weight() while they are those of the weight, else None, None."""
         held = self._held
         if held is not None and held[0] is self.weight and held[1] == self._version():
             return held[2:]
         self._held = None
-        return ext_tokens.quantize_tokens(self.weight)
+        return None, None
 
     def _apply(self, fn, recurse=True):
         self._held = None
@@ -242,9 +243,12 @@ class QInt8Linear(nn.Linear):
         if torch.is_autocast_enabled("cuda") and input.is_floating_point():
             # (the input alone: a weight cast to 16 bits first would be rounded to other codes than the one that is held)
             input = input.to(torch.get_autocast_dtype("cuda"))
+        codes, scale = self._held_tokens()
         if _wants_function(input, self.weight, self.bias):
-            return int8_linear.apply(input, self.weight, self.bias)
-        return ext_tokens.linear_tokens(input, *self._weight_tokens(), self.bias)
+            return int8_linear.apply(input, self.weight, self.bias, codes, scale)
+        if codes is None:
+            codes, scale = ext_tokens.quantize_tokens(self.weight)
+        return ext_tokens.linear_tokens(input, codes, scale, self.bias)
 
 
 class QGroupNorm(nn.GroupNorm):

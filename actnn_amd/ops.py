@@ -558,17 +558,24 @@ def _one_step(forward):
 
 class int8_linear(Function):
     """Linear layer multiplied in 8-bit integers: the input one scale a token, the weight one an output channel.  The tokens as
-    they were multiplied are all that is kept of the input, and the weight's gradient is that of the values they stand for.  To the
-    gradients the rounding of either factor is the identity: grad_input = grad_output @ weight."""
+    they were multiplied are all that is kept of the input, and the weight's gradient is that of the values they stand for; of a
+    frozen weight's input nothing is kept.  To the gradients the rounding of either factor is the identity: grad_input =
+    grad_output @ weight.  `weight_codes` and `weight_scale` are the weight's tokens where they are at hand."""
 
     @staticmethod
     @_one_step
-    def forward(ctx, input, weight, bias=None):
-        weight_codes, weight_scale = ext_tokens.quantize_tokens(weight)
-        output, codes, scale = ext_tokens.linear_tokens(input, weight_codes, weight_scale, bias, keep=True)
+    def forward(ctx, input, weight, bias=None, weight_codes=None, weight_scale=None):
+        if weight_codes is None:
+            weight_codes, weight_scale = ext_tokens.quantize_tokens(weight)
+        need_input, need_weight = ctx.needs_input_grad[:2]
+        codes = scale = None
+        if need_weight:
+            output, codes, scale = ext_tokens.linear_tokens(input, weight_codes, weight_scale, bias, keep=True)
+        else:
+            output = ext_tokens.linear_tokens(input, weight_codes, weight_scale, bias)
         empty_cache(config.empty_cache_threshold)
-        ctx.save_for_backward(codes, scale, weight)
-        ctx.bias_dtype = None if bias is None else bias.dtype
+        ctx.save_for_backward(codes, scale, weight if need_input else None)
+        ctx.shape, ctx.weight_dtype, ctx.bias_dtype = input.shape, weight.dtype, None if bias is None else bias.dtype
         return output
 
     @staticmethod
@@ -580,15 +587,15 @@ class int8_linear(Function):
         if ctx.needs_input_grad[1]:
             if go.dtype == torch.float32:
                 values = ext_tokens.dequantize_tokens(codes, scale).reshape(-1, codes.shape[-1])
-                grad_weight = go.t().mm(values).to(weight.dtype)
+                grad_weight = go.t().mm(values).to(ctx.weight_dtype)
             else:
                 grad_weight = ext_tokens.linear_tokens_grad_weight(
-                    grad_output, codes, scale, torch.float32 if weight.dtype == torch.float32 else None).to(weight.dtype)
+                    grad_output, codes, scale, torch.float32 if ctx.weight_dtype == torch.float32 else None).to(ctx.weight_dtype)
         if ctx.needs_input_grad[0]:
-            grad_input = go.mm(weight.to(go.dtype)).view(codes.shape)
-        if ctx.bias_dtype is not None and ctx.needs_input_grad[2]:
+            grad_input = go.mm(weight.to(go.dtype)).view(ctx.shape)
+        if ctx.needs_input_grad[2]:
             grad_bias = go.sum(0, dtype=torch.float32).to(ctx.bias_dtype)
-        return grad_input, grad_weight, grad_bias
+        return grad_input, grad_weight, grad_bias, None, None
 
 
 # ------------------------------------------------------------------------------------------

@@ -19,6 +19,15 @@ def fresh_config():
     config.reset()
 
 
+def allocated(f):
+    """What f() returns, and the bytes that live after it and did not before."""
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    out = f()
+    torch.cuda.synchronize()
+    return out, torch.cuda.memory_allocated() - before
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("M", [3, 200])
@@ -45,3 +54,50 @@ def test_training_and_answering_multiply_the_same_integers_under_autocast(M, dty
     assert ((grad.double() - exact).abs() <= (HALF_STEP[dtype] * 1.01 + 2.0 ** -23 * (M + 2)) * size).all()
     assert layer.bias.grad.dtype == torch.float32 and x.grad.dtype == torch.float32
     assert ((layer.bias.grad.double() - go.double().sum(0)).abs() <= 2.0 ** -23 * (M + 2) * go.double().abs().sum(0)).all()
+
+
+@pytest.mark.gpu
+def test_a_frozen_layer_keeps_nothing_of_its_input():
+    layer = layers.QInt8Linear(1024, 64).to(DEV).bfloat16()
+    x = torch.randn(4096, 1024, device=DEV).bfloat16().requires_grad_()
+    layer(x)
+    trained, kept = allocated(lambda: layer(x))
+    assert kept >= 4096 * 1024                                              # (the codes)
+    layer.weight.requires_grad_(False)
+    y, kept = allocated(lambda: layer(x))
+    assert kept <= y.numel() * 2 + 65536 and torch.equal(y, trained)
+    go = torch.randn_like(y)
+    y.backward(go)
+    want = go.double() @ layer.weight.double()
+    size = go.double().abs() @ layer.weight.double().abs()
+    assert ((x.grad.double() - want).abs() <= 2.0 ** -23 * 66 * size + 2.0 ** -8 * want.abs() * 1.01).all()
+    assert layer.weight.grad is None and layer.bias.grad is not None
+    # and where only the weight is trained the gradient of the input is not made
+    layer.weight.requires_grad_(True)
+    layer(x.detach()).backward(go)
+    assert layer.weight.grad is not None
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [2, 70])
+def test_a_frozen_layer_multiplies_the_weight_it_holds(M, monkeypatch):
+    torch.manual_seed(2)
+    layer = layers.QInt8Linear(64, 24).to(DEV)
+    layer.weight.requires_grad_(False)
+    x = torch.randn(M, 64, device=DEV, requires_grad=True)
+    want = layer(x).detach()
+    layer.hold_weight()
+    rounded = []
+    monkeypatch.setattr(tokens, "quantize_tokens", lambda t: rounded.append(t) or 1 / 0)
+    y = layer(x)
+    y.sum().backward()
+    assert not rounded and torch.equal(y.detach(), want) and layer._held is not None
+    monkeypatch.undo()
+    with torch.inference_mode():
+        layer.hold_weight()
+    x.grad = None
+    layer(x).sum().backward()
+    assert x.grad is not None and layer._held is not None
+    with torch.no_grad():
+        layer.weight.mul_(2.0)
+    assert torch.equal(layer(x).detach(), tokens.linear_tokens(x.detach(), *tokens.quantize_tokens(layer.weight), layer.bias.detach()))

@@ -206,8 +206,9 @@ class QInt8Linear(nn.Linear):
     pass and its gradient is that of the kept values; a frozen weight has none, and nothing is kept for it.
 
     A layer that only answers, or whose weight is frozen, rounds it once: `hold_weight()`, to be called again after the weight
-    has been replaced (changes in place, load_state_dict, .to() and train() are noticed and end the hold; what is written past
-    autograd, through `weight.data` or into inference tensors, is not)."""
+    has been replaced (changes in place, load_state_dict, .to(), train() and a forward pass that leads to a gradient of the
+    weight are noticed and end the hold; what is written past autograd - through `weight.data`, into inference tensors, by a
+    replayed graph, by a fused optimizer from gradients that another user of the same weight made - is not)."""
 
     _held = None
 
@@ -223,7 +224,9 @@ class QInt8Linear(nn.Linear):
         """The tokens of hold_weight() while they are those of the weight, else None, None."""
         held = self._held
         if held is not None and held[0] is self.weight and held[1] == self._version():
-            return held[2:]
+            # (a weight on its way to a gradient will be changed, and a fused optimizer's steps count as no change)
+            if not (self.weight.requires_grad and torch.is_grad_enabled()):
+                return held[2:]
         self._held = None
         return None, None
 

@@ -101,3 +101,21 @@ def test_a_frozen_layer_multiplies_the_weight_it_holds(M, monkeypatch):
     with torch.no_grad():
         layer.weight.mul_(2.0)
     assert torch.equal(layer(x).detach(), tokens.linear_tokens(x.detach(), *tokens.quantize_tokens(layer.weight), layer.bias.detach()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("optimizer", [torch.optim.SGD, torch.optim.AdamW])
+def test_a_hold_ends_when_the_weight_is_trained(optimizer):
+    # (a fused optimizer's steps are not counted as changes of the tensor)
+    torch.manual_seed(3)
+    layer = layers.QInt8Linear(64, 24).to(DEV).eval()
+    step = optimizer(layer.parameters(), lr=0.1, fused=True)
+    x = torch.randn(5, 64, device=DEV)
+    with torch.no_grad():
+        before = layer.hold_weight()(x)
+    layer(x).square().sum().backward()
+    step.step()
+    with torch.no_grad():
+        got = layer(x)
+        assert not torch.equal(got, before)
+        assert torch.equal(got, tokens.linear_tokens(x, *tokens.quantize_tokens(layer.weight), layer.bias))

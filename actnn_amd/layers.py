@@ -234,6 +234,10 @@ class QInt8Linear(nn.Linear):
         self._held = None
         return super()._apply(fn, recurse)
 
+    def _load_from_state_dict(self, *args, **kwargs):
+        self._held = None                                 # (weights that are swapped in keep the object and may have its count)
+        super()._load_from_state_dict(*args, **kwargs)
+
     def train(self, mode=True):
         if mode:
             self._held = None

@@ -119,3 +119,16 @@ def test_a_hold_ends_when_the_weight_is_trained(optimizer):
         got = layer(x)
         assert not torch.equal(got, before)
         assert torch.equal(got, tokens.linear_tokens(x, *tokens.quantize_tokens(layer.weight), layer.bias))
+
+
+def test_a_hold_ends_when_weights_are_loaded():
+    # whatever way load_state_dict takes to put them in place
+    for swap in (False, True):
+        torch.__future__.set_swap_module_params_on_conversion(swap)
+        try:
+            layer = layers.QInt8Linear(16, 4)
+            layer._held = (layer.weight, layer._version(), None, None, None)
+            layer.load_state_dict({k: torch.zeros_like(v) for k, v in layer.state_dict().items()})
+            assert layer._held is None
+        finally:
+            torch.__future__.set_swap_module_params_on_conversion(False)

@@ -210,52 +210,70 @@ class QInt8Linear(nn.Linear):
     weight are noticed and end the hold; what is written past autograd - through `weight.data`, into inference tensors, by a
     replayed graph, by a fused optimizer from gradients that another user of the same weight made - is not)."""
 
-    _held = None
+    _held = None                                        # weight, its version, codes, scale
+    _held_bias = None                                   # bias, its version, the same in 32 bits
 
-    def _version(self):
-        return None if self.weight.is_inference() else self.weight._version    # (inference tensors count no changes)
+    @staticmethod
+    def _version(t):
+        return None if t.is_inference() else t._version                       # (inference tensors count no changes)
 
     def hold_weight(self):
         with torch.no_grad():
-            self._held = (self.weight, self._version(), *ext_tokens.quantize_tokens(self.weight))
+            self._held = (self.weight, self._version(self.weight), *ext_tokens.quantize_tokens(self.weight))
+            # (the kernels add 32 bits: a bias of fewer is converted once instead of by a launch in every call)
+            bias = self.bias
+            self._held_bias = None if bias is None else (bias, self._version(bias), bias.detach().float())
         return self
+
+    def _let_go(self):
+        self._held = self._held_bias = None
+
+    def _still(self, held, t):
+        """Whether what is held of a parameter is that of `t`.  (One on its way to a gradient will be changed, and a fused
+        optimizer's steps count as no change.)"""
+        return (held is not None and held[0] is t and held[1] == self._version(t)
+                and not (t.requires_grad and torch.is_grad_enabled()))
 
     def _held_tokens(self):
         """The tokens of hold_weight() while they are those of the weight, else None, None."""
-        held = self._held
-        if held is not None and held[0] is self.weight and held[1] == self._version():
-            # (a weight on its way to a gradient will be changed, and a fused optimizer's steps count as no change)
-            if not (self.weight.requires_grad and torch.is_grad_enabled()):
-                return held[2:]
+        if self._still(self._held, self.weight):
+            return self._held[2:]
         self._held = None
         return None, None
 
+    def _bias(self):
+        if self._still(self._held_bias, self.bias):
+            return self._held_bias[2]
+        self._held_bias = None
+        return self.bias
+
     def _apply(self, fn, recurse=True):
-        self._held = None
+        self._let_go()
         return super()._apply(fn, recurse)
 
     def _load_from_state_dict(self, *args, **kwargs):
-        self._held = None                                 # (weights that are swapped in keep the object and may have its count)
+        self._let_go()                                    # (weights that are swapped in keep the object and may have its count)
         super()._load_from_state_dict(*args, **kwargs)
 
     def train(self, mode=True):
         if mode:
-            self._held = None
+            self._let_go()
         return super().train(mode)
 
     def __getstate__(self):
-        return {k: v for k, v in self.__dict__.items() if k != "_held"}
+        return {k: v for k, v in self.__dict__.items() if k not in ("_held", "_held_bias")}
 
     def forward(self, input):
         if torch.is_autocast_enabled("cuda") and input.is_floating_point():
             # (the input alone: a weight cast to 16 bits first would be rounded to other codes than the one that is held)
             input = input.to(torch.get_autocast_dtype("cuda"))
         codes, scale = self._held_tokens()
-        if _wants_function(input, self.weight, self.bias):
-            return int8_linear.apply(input, self.weight, self.bias, codes, scale)
+        bias = self._bias()
+        if _wants_function(input, self.weight, bias):
+            return int8_linear.apply(input, self.weight, bias, codes, scale)
         if codes is None:
             codes, scale = ext_tokens.quantize_tokens(self.weight)
-        return ext_tokens.linear_tokens(input, codes, scale, self.bias)
+        return ext_tokens.linear_tokens(input, codes, scale, bias)
 
 
 class QGroupNorm(nn.GroupNorm):

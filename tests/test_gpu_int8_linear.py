@@ -3,6 +3,7 @@ import copy
 
 import pytest
 import torch
+import torch.nn as nn
 
 from actnn_amd import layers
 from actnn_amd.conf import config
@@ -127,8 +128,43 @@ def test_a_hold_ends_when_weights_are_loaded():
         torch.__future__.set_swap_module_params_on_conversion(swap)
         try:
             layer = layers.QInt8Linear(16, 4)
-            layer._held = (layer.weight, layer._version(), None, None, None)
+            layer._held = (layer.weight, layer.weight._version, None, None)
             layer.load_state_dict({k: torch.zeros_like(v) for k, v in layer.state_dict().items()})
             assert layer._held is None
         finally:
             torch.__future__.set_swap_module_params_on_conversion(False)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_a_held_16_bit_layer_converts_its_bias_once(dtype, monkeypatch):
+    torch.manual_seed(4)
+    layer = layers.QInt8Linear(64, 24).to(DEV).to(dtype).eval()
+    x = torch.randn(1, 64, device=DEV).to(dtype)
+    given = []
+    real = tokens.linear_tokens
+    monkeypatch.setattr(tokens, "linear_tokens", lambda *a, **k: given.append(a[3]) or real(*a, **k))
+    with torch.no_grad():
+        want = layer(x)
+        layer.hold_weight()
+        assert torch.equal(layer(x), want) and torch.equal(layer(x), want)
+        assert given[-1].dtype == torch.float32 and given[-1] is given[-2]
+        layer.bias.add_(1.0)                                                # noticed
+        after = layer(x)
+        assert torch.equal(after, real(x, *tokens.quantize_tokens(layer.weight), layer.bias)) and not torch.equal(after, want)
+        layer.hold_weight()
+        layer.bias = nn.Parameter(torch.zeros_like(layer.bias))
+        assert torch.equal(layer(x), real(x, *tokens.quantize_tokens(layer.weight), None))
+        layer.hold_weight()
+        layer.bias = None
+        assert torch.equal(layer(x), real(x, *tokens.quantize_tokens(layer.weight), None))
+    # a bias that is trained beside a frozen weight leaves the weight's hold alone
+    layer = layers.QInt8Linear(64, 24).to(DEV).to(dtype)
+    layer.weight.requires_grad_(False)
+    step = torch.optim.SGD([layer.bias], lr=1.0, fused=True)
+    layer.hold_weight()
+    layer(x).sum().backward()
+    step.step()
+    with torch.no_grad():
+        got = layer(x)
+        assert torch.equal(got, real(x, *tokens.quantize_tokens(layer.weight), layer.bias)) and layer._held is not None

@@ -558,9 +558,10 @@ def _one_step(forward):
 
 class int8_linear(Function):
     """Linear layer multiplied in 8-bit integers: the input one scale a token, the weight one an output channel.  The tokens as
-    they were multiplied are all that is kept of the input, and the weight's gradient is that of the values they stand for; of a
-    frozen weight's input nothing is kept.  To the gradients the rounding of either factor is the identity: grad_input =
-    grad_output @ weight.  `weight_codes` and `weight_scale` are the weight's tokens where they are at hand."""
+    they were multiplied are all that is kept of the input, and the weight's gradient is that of the values they stand for
+    (config.compress_activation off: the input itself is kept, and the gradient is its); of a frozen weight's input nothing is
+    kept.  To the gradients the rounding of either factor is the identity: grad_input = grad_output @ weight.  `weight_codes`
+    and `weight_scale` are the weight's tokens where they are at hand."""
 
     @staticmethod
     @_one_step
@@ -569,23 +570,26 @@ class int8_linear(Function):
             weight_codes, weight_scale = ext_tokens.quantize_tokens(weight)
         need_input, need_weight = ctx.needs_input_grad[:2]
         codes = scale = None
-        if need_weight:
+        keep = need_weight and config.compress_activation
+        if keep:
             output, codes, scale = ext_tokens.linear_tokens(input, weight_codes, weight_scale, bias, keep=True)
         else:
             output = ext_tokens.linear_tokens(input, weight_codes, weight_scale, bias)
         empty_cache(config.empty_cache_threshold)
-        ctx.save_for_backward(codes, scale, weight if need_input else None)
+        ctx.save_for_backward(codes, scale, input if need_weight and not keep else None, weight if need_input else None)
         ctx.shape, ctx.weight_dtype, ctx.bias_dtype = input.shape, weight.dtype, None if bias is None else bias.dtype
         return output
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_output):
-        codes, scale, weight = ctx.saved_tensors
+        codes, scale, input, weight = ctx.saved_tensors
         go = grad_output.reshape(-1, grad_output.shape[-1])
         grad_input = grad_weight = grad_bias = None
         if ctx.needs_input_grad[1]:
-            if go.dtype == torch.float32:
+            if codes is None:
+                grad_weight = go.t().mm(input.reshape(-1, input.shape[-1])).to(ctx.weight_dtype)
+            elif go.dtype == torch.float32:
                 values = ext_tokens.dequantize_tokens(codes, scale).reshape(-1, codes.shape[-1])
                 grad_weight = go.t().mm(values).to(ctx.weight_dtype)
             else:

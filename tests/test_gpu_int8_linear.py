@@ -168,3 +168,23 @@ def test_a_held_16_bit_layer_converts_its_bias_once(dtype, monkeypatch):
     with torch.no_grad():
         got = layer(x)
         assert torch.equal(got, real(x, *tokens.quantize_tokens(layer.weight), layer.bias)) and layer._held is not None
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_without_compression_the_input_itself_is_kept(dtype):
+    torch.manual_seed(5)
+    config.compress_activation = False
+    layer = layers.QInt8Linear(256, 48).to(DEV).to(dtype)
+    x = torch.randn(20, 60, 256, device=DEV).to(dtype)
+    go = torch.randn(20, 60, 48, device=DEV).to(dtype)
+    layer(x)
+    y, kept = allocated(lambda: layer(x))
+    assert kept <= y.numel() * y.element_size() + 65536                     # nothing but the input that is there already
+    assert torch.equal(y.detach(), tokens.linear_tokens(x, *tokens.quantize_tokens(layer.weight.detach()), layer.bias.detach()))
+    y.backward(go)
+    g, rows = go.double().reshape(-1, 48), x.double().reshape(-1, 256)
+    exact, size = g.t() @ rows, g.abs().t() @ rows.abs()
+    # exact products, 1200 additions in 32 bits, one rounding
+    bound = 2.0 ** -23 * 1202 * size + HALF_STEP[dtype] * exact.abs() * 1.01 + 2.0 ** -25
+    assert ((layer.weight.grad.double() - exact).abs() <= bound).all()

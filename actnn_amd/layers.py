@@ -202,8 +202,9 @@ def _wants_function(*tensors):
 
 class QInt8Linear(nn.Linear):
     """A linear layer that multiplies in 8-bit integers - one scale for each token (row of the input) and each output channel -
-    and keeps, of its input, the codes it multiplied: a byte a value (config.compress_activation off: the input).  In training the weight is rounded anew in every forward
-    pass and its gradient is that of the kept values; a frozen weight has none, and nothing is kept for it.
+    and keeps, of its input, the codes it multiplied: a byte a value (config.compress_activation off: the input itself).  In
+    training the weight is rounded anew in every forward pass and its gradient is that of the kept values; a frozen weight
+    has none, and nothing is kept for it.
 
     A layer that only answers, or whose weight is frozen, rounds it once: `hold_weight()`, to be called again after the weight
     has been replaced (changes in place, load_state_dict, .to(), train() and a forward pass that leads to a gradient of the

@@ -589,8 +589,8 @@ class int8_linear(Function):
         if ctx.needs_input_grad[1]:
             if codes is None:
                 grad_weight = go.t().mm(input.reshape(-1, input.shape[-1])).to(ctx.weight_dtype)
-            elif go.dtype == torch.float32:
-                values = ext_tokens.dequantize_tokens(codes, scale).reshape(-1, codes.shape[-1])
+            elif go.dtype == torch.float32 or not ext_tokens.g.has_storage(go):      # (no storage: a batch of gradients at once)
+                values = ext_tokens.dequantize_tokens(codes, scale, go.dtype).reshape(-1, codes.shape[-1])
                 grad_weight = go.t().mm(values).to(ctx.weight_dtype)
             else:
                 grad_weight = ext_tokens.linear_tokens_grad_weight(

@@ -188,3 +188,24 @@ def test_without_compression_the_input_itself_is_kept(dtype):
     # exact products, 1200 additions in 32 bits, one rounding
     bound = 2.0 ** -23 * 1202 * size + HALF_STEP[dtype] * exact.abs() * 1.01 + 2.0 ** -25
     assert ((layer.weight.grad.double() - exact).abs() <= bound).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_a_batch_of_gradients_at_once(dtype):
+    torch.manual_seed(6)
+    layer = layers.QInt8Linear(64, 24).to(DEV).to(dtype)
+    x = torch.randn(40, 64, device=DEV).to(dtype).requires_grad_()
+    grads = torch.randn(3, 40, 24, device=DEV).to(dtype)
+    wanted = (x, layer.weight, layer.bias)
+    got = torch.autograd.grad(layer(x), wanted, grads, is_grads_batched=True)
+    codes, scale = tokens.quantize_tokens(x.detach())
+    values = (codes.float() * scale[:, None]).to(dtype).double()
+    for i in range(3):
+        g = grads[i].double()
+        w = layer.weight.detach().double()
+        for a, exact, size in ((got[0][i], g @ w, g.abs() @ w.abs()), (got[1][i], g.t() @ values, g.abs().t() @ values.abs()),
+                               (got[2][i], g.sum(0), g.abs().sum(0))):
+            assert a.dtype == dtype
+            # sums of at most 40 terms in 32 bits, one rounding; fp16's kept values may be rounded by way of 32 bits
+            assert ((a.double() - exact).abs() <= (2.0 ** -23 * 42 + 2.0 ** -23) * size + HALF_STEP[dtype] * exact.abs() * 1.01 + 2.0 ** -25).all()

@@ -30,7 +30,8 @@ def quantize_tokens(data):
 
 
 def dequantize_tokens(codes, scale, dtype=torch.float32):
-    """codes * scale, rounded once to `dtype`."""
+    """codes * scale, rounded to `dtype`: once, for bfloat16 by way of 32 bits.  In 16 bits these are the values that
+    linear_tokens_grad_weight multiplies, bit for bit."""
     return g.untraced("dequantize_tokens").dequantize_tokens(codes, scale, _dtype_code(dtype, "dequantize_tokens"))
 
 

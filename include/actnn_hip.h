@@ -517,7 +517,8 @@ int actnn_batch_norm_backward_packed_add_relu(const int32_t* packed, const int32
 /* data: rows of K elements, `ld` elements apart (any ld >= 0), at any element address. */
 int actnn_tokens_quantize(const void* data, int64_t ld, int8_t* codes, int64_t ldc, float* scale, int64_t M, int64_t K,
                           int dtype, void* stream);
-/* out[M, K] (contiguous, dtype) = codes * scale, rounded once; out at any element address. */
+/* out[M, K] (contiguous, dtype) = codes * scale, rounded once (bf16: to fp32 and then to bf16); out at any element address.  In 16
+ * bits these are the values that actnn_tokens_grad_weight multiplies, bit for bit. */
 int actnn_tokens_dequantize(const int8_t* codes, int64_t ldc, const float* scale, void* out, int64_t M, int64_t K,
                             int dtype, void* stream);
 /* out[M, O] (contiguous, dtype, at any element address) = scale[m] * weight_scale[o] * sum_k codes[m, k] * weight_codes[o, k]

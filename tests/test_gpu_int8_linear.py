@@ -8,6 +8,7 @@ import torch.nn as nn
 from actnn_amd import layers
 from actnn_amd.conf import config
 from actnn_amd.cpp_extension import tokens
+from actnn_amd.utils import to_channels_last
 
 DEV = "cuda:0"
 HALF_STEP = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
@@ -209,3 +210,32 @@ def test_a_batch_of_gradients_at_once(dtype):
             assert a.dtype == dtype
             # sums of at most 40 terms in 32 bits, one rounding; fp16's kept values may be rounded by way of 32 bits
             assert ((a.double() - exact).abs() <= (2.0 ** -23 * 42 + 2.0 ** -23) * size + HALF_STEP[dtype] * exact.abs() * 1.01 + 2.0 ** -25).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_gradients_of_the_kernels_repeat_bit_for_bit(dtype):
+    torch.manual_seed(7)
+    linear, norm = layers.QInt8Linear(96, 200).to(DEV).to(dtype), layers.QGroupNorm(6, 96).to(DEV)
+    rows, go = torch.randn(3000, 96, device=DEV).to(dtype), torch.randn(3000, 200, device=DEV).to(dtype)
+    image, gi = (torch.randn(5, 30, 31, 96, device=DEV).to(dtype).permute(0, 3, 1, 2) for _ in range(2))
+    first = None
+    for _ in range(3):
+        image = image.detach().requires_grad_()
+        linear.zero_grad()
+        norm.zero_grad()
+        linear(rows).backward(go)
+        norm(image, silu=True).backward(gi)
+        got = [image.grad, norm.weight.grad, norm.bias.grad] + ([linear.weight.grad] if dtype != torch.float32 else [])
+        first = first or got
+        assert all(torch.equal(a, b) for a, b in zip(first, got))
+
+
+def test_to_channels_last_of_every_number_of_dimensions():
+    for shape in ((2, 3), (2, 3, 5), (2, 3, 5, 4), (2, 3, 2, 3, 4)):
+        x = torch.randn(shape)
+        y = to_channels_last(x)
+        assert torch.equal(x, y) and y.movedim(1, -1).is_contiguous() and to_channels_last(y) is y
+    x = torch.randn(3, 2).t()
+    y = to_channels_last(x)
+    assert torch.equal(x, y) and y.is_contiguous()

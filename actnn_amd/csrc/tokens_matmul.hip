@@ -53,7 +53,13 @@ struct Product {
   int M, K, O;
 };
 
-ACTNN_DEV float scaled(int sum, float xs, float ws, float bias) { return __builtin_fmaf((float)sum * xs, ws, bias); }
+// The sum times the token's scale times the channel's.  Times a scale above 2^90 it may pass the largest number where the result
+// does not, if the other scale is small: then that one comes first (and if that passes it too, the result does).
+constexpr float kLargeScale = 0x1p90f;
+ACTNN_DEV float scaled_usually(int sum, float xs, float ws, float bias) { return __builtin_fmaf((float)sum * xs, ws, bias); }
+ACTNN_DEV float scaled(int sum, float xs, float ws, float bias) {
+  return xs > kLargeScale ? scaled_usually(sum, ws, xs, bias) : scaled_usually(sum, xs, ws, bias);
+}
 
 // four consecutive channels of a token, from their integer sums
 template <typename TY> ACTNN_DEV void put4(const Product& p, int64_t token, int channel, const int (&sum)[4], float xs) {
@@ -68,8 +74,8 @@ template <typename TY> ACTNN_DEV void put4(const Product& p, int64_t token, int 
   for (int i = 0; i < 4; ++i)
     if (channel + i < p.O) Conv<TY>::store(to, i, v[i]);
 }
-// the integer sums of 16 bytes' worth of channels of a token, of which `valid` exist
-template <typename TY, int V>
+// the integer sums of 16 bytes' worth of channels of a token, of which `valid` exist; LARGE: its scale may be above kLargeScale
+template <typename TY, bool LARGE, int V>
 ACTNN_DEV void put_row(TY* to, int valid, const int (&sum)[V], float xs, const float (&ws)[V], const float (&bias)[V]) {
   u32x4 out;
   if constexpr (std::is_same<TY, int>::value) {
@@ -78,7 +84,7 @@ ACTNN_DEV void put_row(TY* to, int valid, const int (&sum)[V], float xs, const f
   } else {
     float v[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) v[i] = scaled(sum[i], xs, ws[i], bias[i]);
+    for (int i = 0; i < V; ++i) v[i] = LARGE ? scaled(sum[i], xs, ws[i], bias[i]) : scaled_usually(sum[i], xs, ws[i], bias[i]);
     store16_part<false>(to, narrow(static_cast<const TY*>(nullptr), v), valid);
   }
 }
@@ -276,9 +282,14 @@ __global__ __launch_bounds__(kThreads, 1) void tokens_tile_kernel(Product p, int
 #pragma unroll
   for (int e = 0; e < NE; ++e) {
     const int first_token = t0 + wn * 32 * NE + 32 * e + lane / kAcross;
+    auto scale_of = [&](int j) { return p.xs[first_token + j * kDown < p.M ? first_token + j * kDown : p.M - 1]; };
     float xs[32 / kDown];
+    bool large = false;
 #pragma unroll
-    for (int j = 0; j < 32 / kDown; ++j) xs[j] = p.xs[first_token + j * kDown < p.M ? first_token + j * kDown : p.M - 1];
+    for (int j = 0; j < 32 / kDown; ++j) {
+      xs[j] = scale_of(j);
+      large = large || xs[j] > kLargeScale;
+    }
 #pragma unroll
     for (int a = 0; a < NA; ++a)
 #pragma unroll
@@ -287,8 +298,7 @@ __global__ __launch_bounds__(kThreads, 1) void tokens_tile_kernel(Product p, int
                     (u32x4){(uint32_t)acc[e][a][4 * q], (uint32_t)acc[e][a][4 * q + 1], (uint32_t)acc[e][a][4 * q + 2],
                             (uint32_t)acc[e][a][4 * q + 3]});
     wave_lds_fence();
-#pragma unroll
-    for (int j = 0; j < 32 / kDown; ++j) {
+    auto put = [&](int j, float scale, auto LARGE) {
       const int64_t token = first_token + j * kDown;
       const uint32_t at = slab + (uint32_t)((j * kDown + lane / kAcross) * kPitch + lane % kAcross * V * 4);
       int sum[V];
@@ -297,7 +307,15 @@ __global__ __launch_bounds__(kThreads, 1) void tokens_tile_kernel(Product p, int
         const u32x4 v = lds_load<u32x4>(at + 4 * i);
         sum[i] = (int)v.x; sum[i + 1] = (int)v.y; sum[i + 2] = (int)v.z; sum[i + 3] = (int)v.w;
       }
-      put_row<TY>(out + token * p.O, token < p.M ? valid : 0, sum, xs[j], ws, bias);
+      put_row<TY, decltype(LARGE)::value != 0>(out + token * p.O, token < p.M ? valid : 0, sum, scale, ws, bias);
+    };
+    // (a branch of the wave: a choice for each value takes 4 us of the largest tile's 130)
+    if (!std::is_same<TY, int>::value && __builtin_expect(__any(large), 0)) {
+#pragma unroll 1
+      for (int j = 0; j < 32 / kDown; ++j) put(j, scale_of(j), Const<1>{});
+    } else {
+#pragma unroll
+      for (int j = 0; j < 32 / kDown; ++j) put(j, xs[j], Const<0>{});
     }
     wave_lds_fence();
   }

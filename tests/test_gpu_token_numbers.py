@@ -1,4 +1,4 @@
-"""The same values wherever codes of 8-bit tokens are turned back into them."""
+"""8-bit tokens at the ends of the types' ranges, and the same values wherever codes are turned back into them."""
 import numpy as np
 import pytest
 import torch
@@ -31,3 +31,33 @@ def test_what_is_read_back_is_what_the_weight_gradient_multiplies(K, dtype):
         one.zero_()
         one[m:m + 8] = torch.eye(8, device=DEV)
         assert torch.equal(tokens.linear_tokens_grad_weight(one, codes, scale), back[m:m + 8]), m
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,K,O", [(1, 4096, 64), (3, 1003, 40), (20, 4096, 33), (70, 8192, 64), (300, 2048, 300)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_large_tokens_with_small_weights_and_the_other_way_round(M, K, O, dtype):
+    # the sum times one scale passes the largest number, the result does not: y is of order 2^100
+    for by, weight_by in ((2.0 ** 115, 2.0 ** -20), (2.0 ** -20, 2.0 ** 115), (2.0 ** 50, 2.0 ** 50)):
+        x = torch.full((M, K), by, device=DEV).to(dtype)
+        x[:, 1] = -by / 2
+        codes, scale = tokens.quantize_tokens(x)
+        wcodes, wscale = tokens.quantize_tokens(torch.full((O, K), weight_by, device=DEV) * torch.linspace(0.5, 1, O, device=DEV)[:, None])
+        exact = (codes.double() @ wcodes.double().t()) * scale.double()[:, None] * wscale.double()
+        assert exact.abs().max() < 3e38 and exact.abs().max() > 1e27
+        for y in (tokens.linear_tokens(x, wcodes, wscale), tokens.matmul_tokens(codes, scale, wcodes, wscale, None, dtype)):
+            half = 2.0 ** -24 if dtype == torch.float32 else 2.0 ** -8
+            assert ((y.double() - exact).abs() <= (3.01 * 2.0 ** -24 + half * 1.01) * exact.abs()).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [4, 20, 300])
+def test_a_large_token_leaves_its_neighbours_as_they_are(M):
+    torch.manual_seed(M)
+    x = torch.randn(M, 512, device=DEV)
+    wcodes, wscale = tokens.quantize_tokens(torch.randn(300, 512, device=DEV) * 2.0 ** -30)
+    alone = tokens.linear_tokens(x, wcodes, wscale)
+    x[M // 2] *= 2.0 ** 120
+    y = tokens.linear_tokens(x, wcodes, wscale)
+    rest = [m for m in range(M) if m != M // 2]
+    assert torch.equal(y[rest], alone[rest]) and torch.equal(y[M // 2], alone[M // 2] * 2.0 ** 120)

@@ -284,6 +284,8 @@ class QGroupNorm(nn.GroupNorm):
 
     def forward(self, input, silu=False):
         """`silu`: the SiLU that follows this layer, in the same pass (gn_silu)."""
+        if input.numel() == self.num_groups:              # (as nn.GroupNorm: its one value a group would come out as zero)
+            raise ValueError(f"Expected more than 1 value per channel when training, got input size {list(input.shape)}")
         activation = "silu" if silu else None
         if _wants_function(input, self.weight, self.bias):
             return group_norm.apply(input, self.num_groups, self.weight, self.bias, self.eps, activation)

@@ -619,8 +619,13 @@ void no_gradients(const char* what, std::initializer_list<const Tensor*> given, 
 bool is_float(const Tensor& t) {
   return t.scalar_type() == at::kFloat || t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16;
 }
-void check_float(const Tensor& t, const char* name) {
+// (a tensor that stands for a batch of others, or for one without values, has no memory, and may have an address all the same)
+void check_on_gpu(const Tensor& t, const char* name) {
   TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor!");
+  TORCH_CHECK(t.has_storage() && t.storage().device().is_cuda(), name, " has no memory to read");
+}
+void check_float(const Tensor& t, const char* name) {
+  check_on_gpu(t, name);
   TORCH_CHECK(is_float(t), "The type of ", name, " is not correct!");
 }
 int64_t whole16(int64_t n) { return (n + 15) / 16 * 16; }
@@ -645,7 +650,7 @@ struct CodeRows {
   Tensor held;
   int64_t M, K, ld;
   CodeRows(const Tensor& t, const char* name) {
-    TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor!");
+    check_on_gpu(t, name);
     TORCH_CHECK(t.scalar_type() == at::kChar, "The type of ", name, " is not correct!");
     TORCH_CHECK(t.dim() >= 1 && t.size(-1) >= 1, name, " must have rows of at least one code");
     K = t.size(-1);
@@ -666,6 +671,7 @@ struct CodeRows {
 };
 Tensor row_scales(const Tensor& t, int64_t rows, const Tensor& like, const char* name) {
   TORCH_CHECK(t.device() == like.device(), name, " must be on the same device");
+  check_on_gpu(t, name);
   TORCH_CHECK(t.scalar_type() == at::kFloat, "The type of ", name, " is not correct!");
   TORCH_CHECK(t.numel() == rows, name, " must have one value for each row, ", rows, ", and has ", t.numel());
   return t.contiguous();
@@ -802,7 +808,7 @@ PyObject* linear_tokens_grad_weight(PyObject* const* a, Py_ssize_t n) {
   Args args(a, n, 4);
   const Tensor grad = args.tensor(), codes = args.tensor(), given = args.tensor();
   no_tangents("linear_tokens_grad_weight", {&grad, &given});
-  TORCH_CHECK(grad.is_cuda(), "grad_output must be a CUDA tensor!");
+  check_on_gpu(grad, "grad_output");
   const auto type = grad.scalar_type();
   TORCH_CHECK(type == at::kHalf || type == at::kBFloat16, "The type of grad_output is not correct!");
   const auto dtype = args.at[args.i] == Py_None ? type : type_of(args.integer());
@@ -861,7 +867,7 @@ struct Pixels {
     set(name);
   }
   Pixels(const Tensor& t, const char* name, at::ScalarType dtype) : given(t) {
-    TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor!");
+    check_on_gpu(t, name);
     TORCH_CHECK(t.scalar_type() == dtype, "The type of ", name, " is not correct!");
     set(name);
   }

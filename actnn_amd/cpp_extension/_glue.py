@@ -19,6 +19,9 @@ def host():
     return _lib.load_host()
 
 
+tracing = torch._C._get_tracing_state                    # None outside torch.jit.trace
+
+
 class _TracedStep(threading.local):
     """`with traced_step:` - what an autograd Function computes inside, which torch.jit.trace records as one step that calls the
     Function again."""
@@ -38,7 +41,7 @@ traced_step = _TracedStep()
 def untraced(name):
     """host() for a call that writes what it allocates with a kernel of its own.  A trace would keep the allocation and lose the
     kernel, so a call that is no step of a Function is refused while one is recorded."""
-    if torch._C._get_tracing_state() is not None and not traced_step.depth:
+    if tracing() is not None and not traced_step.depth:
         raise RuntimeError(f"{name} cannot be traced by itself: the tracer does not see its kernels (the layers over it, "
                            "QInt8Linear and QGroupNorm, can be traced)")
     return _lib.load_host()

@@ -195,9 +195,16 @@ class QLinear(nn.Linear):
         return _autocast_apply(linear, input, self.weight, self.bias, self.scheme)
 
 
+_tracing = ext_tokens.g.tracing
+
+
 def _wants_function(*tensors):
     """Whether a call goes through its autograd Function: for a gradient, or to be one step of a trace."""
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors) or torch.jit.is_tracing()
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return _tracing() is not None
 
 
 class QInt8Linear(nn.Linear):
@@ -232,21 +239,25 @@ class QInt8Linear(nn.Linear):
     def _still(self, held, t):
         """Whether what is held of a parameter is that of `t`.  (One on its way to a gradient will be changed, and a fused
         optimizer's steps count as no change.)"""
-        return (held is not None and held[0] is t and held[1] == self._version(t)
-                and not (t.requires_grad and torch.is_grad_enabled()))
+        return held[0] is t and held[1] == self._version(t) and not (t.requires_grad and torch.is_grad_enabled())
 
-    def _held_tokens(self):
+    def _tokens_of(self, weight):
         """The tokens of hold_weight() while they are those of the weight, else None, None."""
-        if self._still(self._held, self.weight):
+        if self._held is None:
+            return None, None
+        if self._still(self._held, weight):
             return self._held[2:]
         self._held = None
         return None, None
 
-    def _bias(self):
-        if self._still(self._held_bias, self.bias):
+    def _added(self, bias):
+        """The bias that hold_weight() has in 32 bits while it is that of the layer, else the layer's."""
+        if self._held_bias is None:
+            return bias
+        if self._still(self._held_bias, bias):
             return self._held_bias[2]
         self._held_bias = None
-        return self.bias
+        return bias
 
     def _apply(self, fn, recurse=True):
         self._let_go()
@@ -268,12 +279,13 @@ class QInt8Linear(nn.Linear):
         if torch.is_autocast_enabled("cuda") and input.is_floating_point():
             # (the input alone: a weight cast to 16 bits first would be rounded to other codes than the one that is held)
             input = input.to(torch.get_autocast_dtype("cuda"))
-        codes, scale = self._held_tokens()
-        bias = self._bias()
-        if _wants_function(input, self.weight, bias):
-            return int8_linear.apply(input, self.weight, bias, codes, scale)
+        weight = self.weight
+        codes, scale = self._tokens_of(weight)
+        bias = self._added(self.bias)
+        if _wants_function(input, weight, bias):
+            return int8_linear.apply(input, weight, bias, codes, scale)
         if codes is None:
-            codes, scale = ext_tokens.quantize_tokens(self.weight)
+            codes, scale = ext_tokens.quantize_tokens(weight)
         return ext_tokens.linear_tokens(input, codes, scale, bias)
 
 

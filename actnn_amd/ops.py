@@ -549,7 +549,7 @@ def _one_step(forward):
     """Forward pass of a Function whose native calls the tracer does not see: a trace records the Function as one step."""
     @functools.wraps(forward)
     def run(ctx, *args):
-        if torch._C._get_tracing_state() is None:
+        if ext_tokens.g.tracing() is None:
             return forward(ctx, *args)
         with ext_tokens.g.traced_step:
             return forward(ctx, *args)

@@ -7,10 +7,11 @@
 // added as integers: the order does not matter.
 //
 // Three kernels share the work:
-//   * few tokens (up to 32): no tiles: a wave's lanes load their 16 bytes of 16 channels' rows straight into the operand
-//     registers of v_mfma_i32_16x16x64_i8, the waves of a block share the features of the same channels and add their sums in LDS.
-//   * tiles of 64, 128 or 256 channels by as many tokens, for everything else: v_mfma_i32_32x32x32_i8 out of LDS.  Four buffers of
-//     64 or 128 features; both operands go from global memory straight into LDS (global_load_lds, 16 bytes a lane), rows as they
+//   * few tokens (up to 32, where the estimate below has this cheaper than tiles): a wave's lanes load their 16 bytes of 16
+//     channels' rows straight into the operand registers of v_mfma_i32_16x16x64_i8, the waves of a block share the features of
+//     the same channels and add their sums in LDS.
+//   * tiles of 64, 128 or 256 channels by as many tokens, for everything else ([24, 4096] -> 16384 among it):
+//     v_mfma_i32_32x32x32_i8 out of LDS.  Four buffers of 64 or 128 features; both operands go from global memory straight into LDS (global_load_lds, 16 bytes a lane), rows as they
 //     lie in memory, their 16-byte chunks permuted so that 16 rows that are read together meet every bank once.
 //   * tiles that do not fill the chip take slices of the features; a second kernel adds the slices.
 // Rows and channels past the end are read from the last one and not stored; features past the end are read from the
@@ -93,7 +94,7 @@ ACTNN_DEV void put_row(TY* to, int valid, const int (&sum)[V], float xs, const f
 // Tiles.  Four waves, two by two; a wave has NA x NE fragments of 32 channels x 32 tokens.
 //
 // Bound by the matrix pipes and by what reaches them: a wave of the largest tile holds 128 x 128 sums in its 256 accumulation
-// registers, so that a byte read from LDS meets 64 products.  [8192, 4096] x [4096, 4096] takes 125 to 130 us, 2.1 to 2.2 POPS (the
+// registers, so that a byte read from LDS meets 64 products.  [8192, 4096] x [4096, 4096] takes 131 to 136 us, 2.0 to 2.1 POPS (the
 // library's product of such matrices in bf16: 1.2; the pipes alone, fed from registers, reach 3.2 on such codes, 4.4 on zeros:
 // the clock follows the power).  When it took 136 us, 113 remained without the loads into LDS and 87 without the reads from it.
 // ------------------------------------------------------------------------------------------
@@ -309,7 +310,7 @@ __global__ __launch_bounds__(kThreads, 1) void tokens_tile_kernel(Product p, int
       }
       put_row<TY, decltype(LARGE)::value != 0>(out + token * p.O, token < p.M ? valid : 0, sum, scale, ws, bias);
     };
-    // (a branch of the wave: a choice for each value takes 4 us of the largest tile's 130)
+    // (a branch of the wave: a choice for each value takes 4 of the largest product's 133 us)
     if (!std::is_same<TY, int>::value && __builtin_expect(__any(large), 0)) {
 #pragma unroll 1
       for (int j = 0; j < 32 / kDown; ++j) put(j, scale_of(j), Const<1>{});
@@ -476,7 +477,7 @@ __global__ __launch_bounds__(kThreads) void tokens_sum_slices_kernel(Product p, 
 // smaller tiles, two of which share a CU, may be half a round); the start and the end of a block, the fetch of its code among
 // them, `fixed`; slices a second launch of about 4.5, and their sums are written and read back at some 8 TB/s.  Measured, tile 64
 // by 64 features / 64 by 128 / 128 / 256, us: 256 x 4096 x 4096 (tokens, features, outputs) 12.2, 10.0, 18.9, 42;
-// 1024 x 4096 x 4096 36.1, 29.6, 27.9, 42.8; 8192 x 4096 x 4096 248, 205, 169, 125; 512 x 1024 x 2048 6.3, 6.6, 7.6, 18.8.  Few
+// 1024 x 4096 x 4096 36.1, 29.6, 27.9, 42.8; 8192 x 4096 x 4096 248, 205, 169, 125 (133 now); 512 x 1024 x 2048 6.3, 6.6, 7.6, 18.8.  Few
 // tokens without tiles: 0.7 (1.1 for more than 16) for every 1024 features that its waves walk alone, or the weight at 4.5 TB/s,
 // and 2 for start and end (without tiles / by them: 24 x 4096 x 1024 6.7, 10.8; 24 x 4096 x 16384 21.2, 13.1; 16 x 16384 x 100
 // 15.9, 10.1; 61 x 7326 x 1790, which none of it takes, 15.5, 11.8).
